@@ -719,6 +719,38 @@ int nvc_memory_scan(nvc_ctx* ctx, const nvc_memory_scan_args* p, int B, int max_
 int nvc_gemm_bf16_glu_clamp_mul(nvc_ctx* ctx, const nvc_bf16* A, int lda, const nvc_bf16* W_gu16, nvc_bf16* act, int ldc, int M, int I, int K,
                                 float limit, void* stream);
 
+/* ---- rows and weights in 8 bits, and the products that read them (serving only) ----
+ * A number is kept as an e4m3 byte q and stands for q * scale, one fp32 scale for a block of 128 numbers along a row (a row's last block may be
+ * shorter) or of 128 x 128 in a weight:  scale = max(amax / 448, 2^-126),  q = e4m3(x * (1 / scale)), to nearest even.  Where a block holds a NaN,
+ * that number alone is NaN; where it holds an infinity, everything computed from it is.  Row widths are multiples of 16; pointers to numbers are
+ * 16-byte aligned. */
+typedef uint8_t nvc_fp8;
+enum { NVC_FP8_BLOCK = 128 };
+/* q[i, :H], scale[i, :ceil(H / 128)] = the 8-bit form of f(x[r]), i < N:
+ *   NVC_ACT_NONE: f(v) = v[:H];  NVC_ACT_RELU2: max(v[:H], 0)^2;  NVC_ACT_SILU_MUL, NVC_ACT_GELU_TANH_MUL: act(v[:H]) * v[up_off : up_off + H].
+ * rows == NULL: r = i; else r = rows[i], and a negative one is a row of zeros (rows of experts: src_rows of nvc_moe_sort_padded).  num_rows != NULL: a
+ * count in device memory; rows from it on are left as they are.  x: bf16 or fp32, ldx a multiple of 8; ldq a multiple of 16. */
+int nvc_quant_fp8_rows(nvc_ctx* ctx, const void* x, int x_dtype, int ldx, int act, int up_off, const int32_t* rows, const int32_t* num_rows, nvc_fp8* q,
+                       int ldq, float* scale, int lds, int N, int H, void* stream);
+/* nvc_fused_add_rmsnorm with 8-bit rows behind it, from the fp32 result:
+ *   s = x + residual_in (optional); residual_out = s (optional, may alias);  y = s * rsqrt(mean(s^2) + eps) * w;
+ *   q, scale = the 8-bit form of y;  out = bf16(y) (optional: a router reads it).
+ * x, w: bf16 or fp32; x, residuals, out contiguous.  H <= 16384. */
+int nvc_add_rmsnorm_fp8(nvc_ctx* ctx, const void* x, int x_dtype, const float* residual_in, float* residual_out, const void* w, int w_dtype, float eps,
+                        nvc_fp8* q, int ldq, float* scale, int lds, nvc_bf16* out, int N, int H, void* stream);
+/* Weights w [groups, N, K] (bf16 or fp32, contiguous) -> q [groups, N, K], scale [groups, ceil(N / 128), ceil(K / 128)]; blocks end with their group.
+ * Starts when all earlier work of the stream is done and ends before later work starts: its results are static operands of the products behind it. */
+int nvc_quant_fp8_blocks(nvc_ctx* ctx, const void* w, int w_dtype, nvc_fp8* q, float* scale, int groups, int N, int K, void* stream);
+/* C[M, Nout] = sum over blocks b of K:  a_scale[m, b] * w_scale[n / 128, b] * sum over k in b of A[m, k] * W[n, k], bf16 or fp32.
+ * A: 8-bit rows with scales [M, lds]; W [Nout, K] with scales [ceil(Nout / 128), ceil(K / 128)], both static.  K % 16 == 0, Nout % 16 == 0, lda % 16 == 0,
+ * ldc % 8 == 0. */
+int nvc_gemm_fp8(nvc_ctx* ctx, const nvc_fp8* A, int lda, const float* a_scale, int lds, const nvc_fp8* W, const float* w_scale, void* C, int ldc,
+                 int out_dtype, int M, int Nout, int K, void* stream);
+/* The same for rows sorted by expert (nvc_gemm_bf16_grouped): rows [128 t, 128 t + 128) use W[tile_group[t]] and its scales.  Rows of tiles with a
+ * negative tile_group become zeros (zero != 0) or are left as they are. */
+int nvc_gemm_fp8_grouped(nvc_ctx* ctx, const nvc_fp8* A, int lda, const float* a_scale, int lds, const nvc_fp8* W, const float* w_scale, void* C, int ldc,
+                         int out_dtype, int M_cap, int Nout, int K, const int32_t* tile_group, int groups, int zero, void* stream);
+
 /* K8. Replaces Qwen3ModelRunner::argmax (src/engine/llm_engine.rs:135-142) on device:
  * idx[b] = LAST index of the maximum of logits[b, :] (Iterator::max_by tie rule);
  * val[b] = that maximum.  idx is offset by `index_offset` (TP vocab shard). */

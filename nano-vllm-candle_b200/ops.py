@@ -914,3 +914,148 @@ def prefill_attn_window(ctx, q, k_cache, v_cache, block_tables, context_lens, cu
                                               block_size, k_cache.shape[0] // block_size, scale, window, _ptr(sink), _ptr(out), out.stride(0),
                                               _stream()), "nvc_prefill_attn_paged_window", ctx.h)
     return out
+
+
+# ---------------------------------------------------------------- rows and weights in 8 bits, and the products that read them
+FP8 = torch.float8_e4m3fn
+FP8_BLOCK = 128
+
+
+def _stream_on(ctx):
+    return torch._C._cuda_getCurrentRawStream(ctx.device)
+
+
+def _on(ctx, name: str, t: torch.Tensor, dtype=None):
+    """A tensor on the context's device, of the given type, whose rows lie one number beside the next."""
+    if not t.is_cuda or t.device.index != ctx.device:
+        raise ValueError(f"{name} must be on cuda:{ctx.device} (no CPU fallback on this path)")
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.dim() and t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise ValueError(f"{name}: the last dimension must be contiguous")
+
+
+def _rows(name: str, t: torch.Tensor, n: int, width: int):
+    if t.dim() != 2 or t.shape[0] != n or t.shape[1] != width:
+        raise ValueError(f"{name} must be [{n}, {width}], got {list(t.shape)}")
+
+
+def _whole(name: str, t: torch.Tensor, shape):
+    if tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous {list(shape)}, got {list(t.shape)}")
+
+
+def _fp8_rows_out(ctx, q, scale, n: int, width: int, device):
+    if q is None:
+        q = torch.empty(n, width, dtype=FP8, device=device)
+    else:
+        _on(ctx, "q", q, FP8); _rows("q", q, n, width)
+    blocks = (width + FP8_BLOCK - 1) // FP8_BLOCK
+    if scale is None:
+        scale = torch.empty(n, blocks, dtype=torch.float32, device=device)
+    else:
+        _on(ctx, "scale", scale, torch.float32); _rows("scale", scale, n, blocks)
+    return q, scale
+
+
+def quant_fp8(ctx, x: torch.Tensor, act: int = ACT_NONE, rows=None, num_rows=None, q=None, scale=None):
+    """Rows in 8 bits: (q e4m3 [N, H], scale fp32 [N, ceil(H / 128)]), number = q * scale.
+    x: bf16 or fp32 [*, H], or [*, 2 H] for ACT_SILU_MUL and ACT_GELU_TANH_MUL (act(left half) * right half; ACT_RELU2: max(x, 0)^2).
+    rows: int32 [N], the row of x for each row of the result, negative for zeros (src of moe_sort_padded); num_rows: int32 [1], rows from it on are
+    left as they are (offsets[E:] of moe_sort_padded).  q, scale: where to write."""
+    dt = _dt(x)
+    _on(ctx, "x", x)
+    if x.dim() != 2:
+        raise ValueError("x must be two-dimensional")
+    gated = act in (ACT_SILU_MUL, ACT_GELU_TANH_MUL)
+    H = x.shape[1] // 2 if gated else x.shape[1]
+    if gated and x.shape[1] % 2:
+        raise ValueError("a gated unit takes two halves of equal width")
+    N = x.shape[0]
+    if rows is not None:
+        _on(ctx, "rows", rows, torch.int32)
+        _whole("rows", rows, (rows.numel(),))
+        N = rows.numel()
+    if num_rows is not None:
+        _on(ctx, "num_rows", num_rows, torch.int32)
+        if num_rows.numel() < 1:
+            raise ValueError("num_rows must hold a count")
+    q, scale = _fp8_rows_out(ctx, q, scale, N, H, x.device)
+    if N:
+        check(ctx.l.nvc_quant_fp8_rows(ctx.h, _ptr(x), dt, x.stride(0), act, H, _ptr(rows), _ptr(num_rows), _ptr(q), q.stride(0), _ptr(scale),
+                                       scale.stride(0), N, H, _stream_on(ctx)), "nvc_quant_fp8_rows", ctx.h)
+    return q, scale
+
+
+def quant_fp8_weight(ctx, w: torch.Tensor):
+    """A weight [N, K], or experts' weights [groups, N, K], bf16 or fp32, in 8 bits: (q, scale [(groups,) ceil(N / 128), ceil(K / 128)])."""
+    dt = _dt(w)
+    _on(ctx, "w", w)
+    if w.dim() not in (2, 3) or not w.is_contiguous():
+        raise ValueError("w must be contiguous [N, K] or [groups, N, K]")
+    N, K = w.shape[-2:]
+    groups = w.shape[0] if w.dim() == 3 else 1
+    q = torch.empty(w.shape, dtype=FP8, device=w.device)
+    scale = torch.empty(*w.shape[:-2], (N + FP8_BLOCK - 1) // FP8_BLOCK, (K + FP8_BLOCK - 1) // FP8_BLOCK, dtype=torch.float32, device=w.device)
+    if groups:
+        check(ctx.l.nvc_quant_fp8_blocks(ctx.h, _ptr(w), dt, _ptr(q), _ptr(scale), groups, N, K, _stream_on(ctx)), "nvc_quant_fp8_blocks", ctx.h)
+    return q, scale
+
+
+def add_rmsnorm_fp8(ctx, x: torch.Tensor, w: torch.Tensor, eps: float, residual=None, residual_out=None, want_out: bool = False, q=None, scale=None):
+    """fused_add_rmsnorm with rows in 8 bits behind it: (q, scale, out).  x: bf16 or fp32 [N, H]; w: bf16 or fp32 [H]; residual (added) and residual_out (the
+    sum; may be residual): fp32 [N, H]; out: the normed rows in bf16 when want_out, else None."""
+    dt, wdt = _dt(x), _dt(w)
+    _on(ctx, "x", x); _on(ctx, "w", w)
+    if x.dim() != 2 or not x.is_contiguous():
+        raise ValueError("x must be contiguous [N, H]")
+    N, H = x.shape
+    _whole("w", w, (H,))
+    for name, t in (("residual", residual), ("residual_out", residual_out)):
+        if t is not None:
+            _on(ctx, name, t, torch.float32); _whole(name, t, (N, H))
+    q, scale = _fp8_rows_out(ctx, q, scale, N, H, x.device)
+    out = torch.empty(N, H, dtype=BF16, device=x.device) if want_out else None
+    if N:
+        check(ctx.l.nvc_add_rmsnorm_fp8(ctx.h, _ptr(x), dt, _ptr(residual), _ptr(residual_out), _ptr(w), wdt, eps, _ptr(q), q.stride(0), _ptr(scale),
+                                        scale.stride(0), _ptr(out), N, H, _stream_on(ctx)), "nvc_add_rmsnorm_fp8", ctx.h)
+    return q, scale, out
+
+
+def _fp8_product(ctx, q, scale, wq, wscale, out, out_dtype, lead):
+    _on(ctx, "q", q, FP8); _on(ctx, "scale", scale, torch.float32); _on(ctx, "wq", wq, FP8); _on(ctx, "wscale", wscale, torch.float32)
+    if q.dim() != 2 or wq.dim() != 2 + len(lead) or wq.shape[-1] != q.shape[1] or not wq.is_contiguous():
+        raise ValueError(f"q [M, K] and contiguous wq with rows of K: got {list(q.shape)} and {list(wq.shape)}")
+    M, K = q.shape
+    N = wq.shape[-2]
+    blocks = (K + FP8_BLOCK - 1) // FP8_BLOCK
+    _rows("scale", scale, M, blocks)
+    _whole("wscale", wscale, (*lead, (N + FP8_BLOCK - 1) // FP8_BLOCK, blocks))
+    if out is None:
+        out = torch.empty(M, N, dtype=out_dtype, device=q.device)
+    else:
+        _on(ctx, "out", out); _rows("out", out, M, N)
+    return M, N, K, out, _dt(out)
+
+
+def gemm_fp8(ctx, q, scale, wq, wscale, out_dtype=BF16, out=None) -> torch.Tensor:
+    """[M, N] = rows times weight, both in 8 bits: (q, scale) of quant_fp8 or add_rmsnorm_fp8, (wq, wscale) of quant_fp8_weight; bf16 or fp32."""
+    M, N, K, out, dt = _fp8_product(ctx, q, scale, wq, wscale, out, out_dtype, ())
+    if M:
+        check(ctx.l.nvc_gemm_fp8(ctx.h, _ptr(q), q.stride(0), _ptr(scale), scale.stride(0), _ptr(wq), _ptr(wscale), _ptr(out), out.stride(0), dt, M, N, K,
+                                 _stream_on(ctx)), "nvc_gemm_fp8", ctx.h)
+    return out
+
+
+def gemm_fp8_grouped(ctx, q, scale, wq, wscale, tile_group, out_dtype=BF16, out=None) -> torch.Tensor:
+    """Rows sorted by expert (moe_sort_padded, groups padded to 128 rows) times the experts' weights wq [groups, N, K]: rows of tile t use
+    wq[tile_group[t]].  Rows of tiles without an expert are zeros, or, in a given `out`, left as they are."""
+    M, N, K, out_, dt = _fp8_product(ctx, q, scale, wq, wscale, out, out_dtype, (wq.shape[0],))
+    _on(ctx, "tile_group", tile_group, torch.int32)
+    if M % 128:
+        raise ValueError("rows must be a multiple of 128")
+    _whole("tile_group", tile_group, (M // 128,))
+    if M:
+        check(ctx.l.nvc_gemm_fp8_grouped(ctx.h, _ptr(q), q.stride(0), _ptr(scale), scale.stride(0), _ptr(wq), _ptr(wscale), _ptr(out_), out_.stride(0), dt, M, N, K,
+                                         _ptr(tile_group), wq.shape[0], 1 if out is None else 0, _stream_on(ctx)), "nvc_gemm_fp8_grouped", ctx.h)
+    return out_
