@@ -153,6 +153,7 @@ def _declare(l: C.CDLL) -> None:
         "nvc_quant_fp8_blocks": [_vp, _vp, _i, _vp, _vp, _i, _i, _i, _vp],
         "nvc_add_rmsnorm_fp8": [_vp, _vp, _i, _vp, _vp, _vp, _i, _f, _vp, _i, _vp, _i, _vp, _i, _i, _vp],
         "nvc_gemm_fp8": [_vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp],
+        "nvc_gemm_fp8_ex": [_vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp],
         "nvc_gemm_fp8_grouped": [_vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _i, _i, _vp],
         "nvc_debug_set": [_i, _i],
     }

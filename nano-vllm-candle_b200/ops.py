@@ -919,43 +919,49 @@ def prefill_attn_window(ctx, q, k_cache, v_cache, block_tables, context_lens, cu
 # ---------------------------------------------------------------- rows and weights in 8 bits, and the products that read them
 FP8 = torch.float8_e4m3fn
 FP8_BLOCK = 128
+_DTYPE_CODE = {torch.bfloat16: 0, torch.float32: 1}
 
 
-def _stream_on(ctx):
-    return torch._C._cuda_getCurrentRawStream(ctx.device)
+# The arguments of a call are looked at in one expression, since a short kernel waits for its call (a norm of one row: 13.2 us with a function per argument and property,
+# 9.1 so); only where something is wrong does _refuse look for it one by one.
+def _refuse(ctx, *facts):
+    """facts: (name, tensor, types it may have, shape it has to have or None, whether it has to be contiguous)."""
+    for name, t, types, shape, whole in facts:
+        if t is None:
+            continue
+        if t.dtype not in types:
+            raise TypeError(f"{name} must be {' or '.join(map(str, types))}, got {t.dtype}")
+        if t.get_device() != ctx.device:
+            raise ValueError(f"{name} must be on cuda:{ctx.device} (no CPU fallback on this path)")
+        if shape is not None and tuple(t.shape) != tuple(shape):
+            raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+        if whole and not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+        if t.dim() and t.shape[-1] > 1 and t.stride(-1) != 1:
+            raise ValueError(f"{name}: the last dimension must be contiguous")
+    raise ValueError("arguments of these shapes do not belong together: " + ", ".join(f"{name} {list(t.shape)}" for name, t, *_ in facts if t is not None))
 
 
-def _on(ctx, name: str, t: torch.Tensor, dtype=None):
-    """A tensor on the context's device, of the given type, whose rows lie one number beside the next."""
-    if not t.is_cuda or t.device.index != ctx.device:
-        raise ValueError(f"{name} must be on cuda:{ctx.device} (no CPU fallback on this path)")
-    if dtype is not None and t.dtype != dtype:
-        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.dim() and t.stride(-1) != 1 and t.shape[-1] > 1:
-        raise ValueError(f"{name}: the last dimension must be contiguous")
-
-
-def _rows(name: str, t: torch.Tensor, n: int, width: int):
-    if t.dim() != 2 or t.shape[0] != n or t.shape[1] != width:
-        raise ValueError(f"{name} must be [{n}, {width}], got {list(t.shape)}")
-
-
-def _whole(name: str, t: torch.Tensor, shape):
-    if tuple(t.shape) != tuple(shape) or not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous {list(shape)}, got {list(t.shape)}")
+_ROWS, _F32, _I32, _E4M3 = (torch.bfloat16, torch.float32), (torch.float32,), (torch.int32,), (FP8,)
 
 
 def _fp8_rows_out(ctx, q, scale, n: int, width: int, device):
+    """The rows and scales to write, new ones or those given, and their row strides."""
+    blocks = (width + 127) // 128
+    ldq, lds = width, blocks
     if q is None:
         q = torch.empty(n, width, dtype=FP8, device=device)
     else:
-        _on(ctx, "q", q, FP8); _rows("q", q, n, width)
-    blocks = (width + FP8_BLOCK - 1) // FP8_BLOCK
+        if q.get_device() != ctx.device or q.dtype is not FP8 or q.shape != (n, width) or (width > 1 and q.stride(1) != 1):
+            _refuse(ctx, ("q", q, _E4M3, (n, width), False))
+        ldq = q.stride(0)
     if scale is None:
         scale = torch.empty(n, blocks, dtype=torch.float32, device=device)
     else:
-        _on(ctx, "scale", scale, torch.float32); _rows("scale", scale, n, blocks)
-    return q, scale
+        if scale.get_device() != ctx.device or scale.dtype is not torch.float32 or scale.shape != (n, blocks) or (blocks > 1 and scale.stride(1) != 1):
+            _refuse(ctx, ("scale", scale, _F32, (n, blocks), False))
+        lds = scale.stride(0)
+    return q, scale, ldq, lds
 
 
 def quant_fp8(ctx, x: torch.Tensor, act: int = ACT_NONE, rows=None, num_rows=None, q=None, scale=None):
@@ -963,99 +969,113 @@ def quant_fp8(ctx, x: torch.Tensor, act: int = ACT_NONE, rows=None, num_rows=Non
     x: bf16 or fp32 [*, H], or [*, 2 H] for ACT_SILU_MUL and ACT_GELU_TANH_MUL (act(left half) * right half; ACT_RELU2: max(x, 0)^2).
     rows: int32 [N], the row of x for each row of the result, negative for zeros (src of moe_sort_padded); num_rows: int32 [1], rows from it on are
     left as they are (offsets[E:] of moe_sort_padded).  q, scale: where to write."""
-    dt = _dt(x)
-    _on(ctx, "x", x)
-    if x.dim() != 2:
-        raise ValueError("x must be two-dimensional")
-    gated = act in (ACT_SILU_MUL, ACT_GELU_TANH_MUL)
-    H = x.shape[1] // 2 if gated else x.shape[1]
-    if gated and x.shape[1] % 2:
-        raise ValueError("a gated unit takes two halves of equal width")
-    N = x.shape[0]
+    dt = _DTYPE_CODE.get(x.dtype)
+    if dt is None or x.get_device() != ctx.device or x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
+        _refuse(ctx, ("x", x, _ROWS, None, False))
+    N, H = x.shape
+    if act == ACT_SILU_MUL or act == ACT_GELU_TANH_MUL:
+        if H % 2:
+            raise ValueError("a gated unit takes two halves of equal width")
+        H //= 2
     if rows is not None:
-        _on(ctx, "rows", rows, torch.int32)
-        _whole("rows", rows, (rows.numel(),))
-        N = rows.numel()
-    if num_rows is not None:
-        _on(ctx, "num_rows", num_rows, torch.int32)
-        if num_rows.numel() < 1:
-            raise ValueError("num_rows must hold a count")
-    q, scale = _fp8_rows_out(ctx, q, scale, N, H, x.device)
+        if rows.get_device() != ctx.device or rows.dtype is not torch.int32 or rows.dim() != 1 or not rows.is_contiguous():
+            _refuse(ctx, ("rows", rows, _I32, (rows.numel(),), True))
+        N = rows.shape[0]
+    if num_rows is not None and (num_rows.get_device() != ctx.device or num_rows.dtype is not torch.int32 or num_rows.numel() < 1):
+        _refuse(ctx, ("num_rows", num_rows, _I32, None, False))
+    q, scale, ldq, lds = _fp8_rows_out(ctx, q, scale, N, H, x.device)
     if N:
-        check(ctx.l.nvc_quant_fp8_rows(ctx.h, _ptr(x), dt, x.stride(0), act, H, _ptr(rows), _ptr(num_rows), _ptr(q), q.stride(0), _ptr(scale),
-                                       scale.stride(0), N, H, _stream_on(ctx)), "nvc_quant_fp8_rows", ctx.h)
+        check(ctx.l.nvc_quant_fp8_rows(ctx.h, x.data_ptr(), dt, x.stride(0), act, H, _ptr(rows), _ptr(num_rows), q.data_ptr(), ldq, scale.data_ptr(), lds, N, H,
+                                       torch._C._cuda_getCurrentRawStream(ctx.device)), "nvc_quant_fp8_rows", ctx.h)
     return q, scale
 
 
 def quant_fp8_weight(ctx, w: torch.Tensor):
     """A weight [N, K], or experts' weights [groups, N, K], bf16 or fp32, in 8 bits: (q, scale [(groups,) ceil(N / 128), ceil(K / 128)])."""
-    dt = _dt(w)
-    _on(ctx, "w", w)
-    if w.dim() not in (2, 3) or not w.is_contiguous():
-        raise ValueError("w must be contiguous [N, K] or [groups, N, K]")
+    dt = _DTYPE_CODE.get(w.dtype)
+    if dt is None or w.get_device() != ctx.device or w.dim() not in (2, 3) or not w.is_contiguous():
+        _refuse(ctx, ("w", w, _ROWS, None, True))
     N, K = w.shape[-2:]
     groups = w.shape[0] if w.dim() == 3 else 1
     q = torch.empty(w.shape, dtype=FP8, device=w.device)
-    scale = torch.empty(*w.shape[:-2], (N + FP8_BLOCK - 1) // FP8_BLOCK, (K + FP8_BLOCK - 1) // FP8_BLOCK, dtype=torch.float32, device=w.device)
+    scale = torch.empty(*w.shape[:-2], (N + 127) // 128, (K + 127) // 128, dtype=torch.float32, device=w.device)
     if groups:
-        check(ctx.l.nvc_quant_fp8_blocks(ctx.h, _ptr(w), dt, _ptr(q), _ptr(scale), groups, N, K, _stream_on(ctx)), "nvc_quant_fp8_blocks", ctx.h)
+        check(ctx.l.nvc_quant_fp8_blocks(ctx.h, w.data_ptr(), dt, q.data_ptr(), scale.data_ptr(), groups, N, K, torch._C._cuda_getCurrentRawStream(ctx.device)),
+              "nvc_quant_fp8_blocks", ctx.h)
     return q, scale
 
 
 def add_rmsnorm_fp8(ctx, x: torch.Tensor, w: torch.Tensor, eps: float, residual=None, residual_out=None, want_out: bool = False, q=None, scale=None):
     """fused_add_rmsnorm with rows in 8 bits behind it: (q, scale, out).  x: bf16 or fp32 [N, H]; w: bf16 or fp32 [H]; residual (added) and residual_out (the
     sum; may be residual): fp32 [N, H]; out: the normed rows in bf16 when want_out, else None."""
-    dt, wdt = _dt(x), _dt(w)
-    _on(ctx, "x", x); _on(ctx, "w", w)
-    if x.dim() != 2 or not x.is_contiguous():
-        raise ValueError("x must be contiguous [N, H]")
-    N, H = x.shape
-    _whole("w", w, (H,))
-    for name, t in (("residual", residual), ("residual_out", residual_out)):
-        if t is not None:
-            _on(ctx, name, t, torch.float32); _whole(name, t, (N, H))
-    q, scale = _fp8_rows_out(ctx, q, scale, N, H, x.device)
+    dt, wdt, dev = _DTYPE_CODE.get(x.dtype), _DTYPE_CODE.get(w.dtype), ctx.device
+    shape = x.shape
+    if (dt is None or wdt is None or x.get_device() != dev or w.get_device() != dev or len(shape) != 2 or w.shape != shape[1:] or not x.is_contiguous() or not w.is_contiguous()
+            or (residual is not None and (residual.get_device() != dev or residual.dtype is not torch.float32 or residual.shape != shape or not residual.is_contiguous()))
+            or (residual_out is not None and (residual_out.get_device() != dev or residual_out.dtype is not torch.float32 or residual_out.shape != shape
+                                              or not residual_out.is_contiguous()))):
+        _refuse(ctx, ("x", x, _ROWS, None, True), ("w", w, _ROWS, shape[-1:], True), ("residual", residual, _F32, shape, True),
+                ("residual_out", residual_out, _F32, shape, True))
+    N, H = shape
+    q, scale, ldq, lds = _fp8_rows_out(ctx, q, scale, N, H, x.device)
     out = torch.empty(N, H, dtype=BF16, device=x.device) if want_out else None
     if N:
-        check(ctx.l.nvc_add_rmsnorm_fp8(ctx.h, _ptr(x), dt, _ptr(residual), _ptr(residual_out), _ptr(w), wdt, eps, _ptr(q), q.stride(0), _ptr(scale),
-                                        scale.stride(0), _ptr(out), N, H, _stream_on(ctx)), "nvc_add_rmsnorm_fp8", ctx.h)
+        check(ctx.l.nvc_add_rmsnorm_fp8(ctx.h, x.data_ptr(), dt, _ptr(residual), _ptr(residual_out), w.data_ptr(), wdt, eps, q.data_ptr(), ldq, scale.data_ptr(), lds,
+                                        _ptr(out), N, H, torch._C._cuda_getCurrentRawStream(dev)), "nvc_add_rmsnorm_fp8", ctx.h)
     return q, scale, out
 
 
-def _fp8_product(ctx, q, scale, wq, wscale, out, out_dtype, lead):
-    _on(ctx, "q", q, FP8); _on(ctx, "scale", scale, torch.float32); _on(ctx, "wq", wq, FP8); _on(ctx, "wscale", wscale, torch.float32)
-    if q.dim() != 2 or wq.dim() != 2 + len(lead) or wq.shape[-1] != q.shape[1] or not wq.is_contiguous():
-        raise ValueError(f"q [M, K] and contiguous wq with rows of K: got {list(q.shape)} and {list(wq.shape)}")
-    M, K = q.shape
-    N = wq.shape[-2]
-    blocks = (K + FP8_BLOCK - 1) // FP8_BLOCK
-    _rows("scale", scale, M, blocks)
-    _whole("wscale", wscale, (*lead, (N + FP8_BLOCK - 1) // FP8_BLOCK, blocks))
+def _fp8_product(ctx, q, scale, wq, wscale, out, out_dtype, groups):
+    """Checks of both products: (M, N, K, row strides of q and scale, the result, its row stride and its type's number).  groups: None, or the first dimension of
+    the weights."""
+    dev = ctx.device
+    qs, ws = q.shape, wq.shape
+    M, K = qs if len(qs) == 2 else (0, 0)
+    N, blocks = ws[-2] if len(ws) > 1 else 0, (K + 127) // 128
+    lds, ldq = blocks, K
+    wblocks = ((N + 127) // 128, blocks) if groups is None else (groups, (N + 127) // 128, blocks)
+    good = (q.get_device() == dev and scale.get_device() == dev and wq.get_device() == dev and wscale.get_device() == dev and q.dtype is FP8 and wq.dtype is FP8
+            and scale.dtype is torch.float32 and wscale.dtype is torch.float32 and K and scale.shape == (M, blocks) and wscale.shape == wblocks and wq.is_contiguous()
+            and wscale.is_contiguous() and ws[-1] == K and len(ws) == (2 if groups is None else 3))
+    if good and not q.is_contiguous():
+        ldq, one = q.stride()
+        good = one == 1
+    if good and not scale.is_contiguous():
+        lds, one = scale.stride()
+        good = one == 1 or blocks == 1
     if out is None:
-        out = torch.empty(M, N, dtype=out_dtype, device=q.device)
+        code, ldo = _DTYPE_CODE.get(out_dtype), N
+        if good and code is not None:
+            return M, N, K, ldq, lds, torch.empty(M, N, dtype=out_dtype, device=q.device), ldo, code
+        if code is None:
+            raise TypeError(f"bf16 or fp32 expected, got {out_dtype}")
     else:
-        _on(ctx, "out", out); _rows("out", out, M, N)
-    return M, N, K, out, _dt(out)
+        code = _DTYPE_CODE.get(out.dtype)
+        if good and code is not None and out.get_device() == dev and out.shape == (M, N) and out.stride(1) == 1:
+            return M, N, K, ldq, lds, out, out.stride(0), code
+    _refuse(ctx, ("q", q, _E4M3, (M, K), False), ("scale", scale, _F32, (M, blocks), False), ("wq", wq, _E4M3, (*ws[:0 if groups is None else 1], N, K), True),
+            ("wscale", wscale, _F32, wblocks, True), ("out", out, _ROWS, (M, N), False))
 
 
 def gemm_fp8(ctx, q, scale, wq, wscale, out_dtype=BF16, out=None) -> torch.Tensor:
     """[M, N] = rows times weight, both in 8 bits: (q, scale) of quant_fp8 or add_rmsnorm_fp8, (wq, wscale) of quant_fp8_weight; bf16 or fp32."""
-    M, N, K, out, dt = _fp8_product(ctx, q, scale, wq, wscale, out, out_dtype, ())
+    M, N, K, ldq, lds, out, ldo, dt = _fp8_product(ctx, q, scale, wq, wscale, out, out_dtype, None)
     if M:
-        check(ctx.l.nvc_gemm_fp8(ctx.h, _ptr(q), q.stride(0), _ptr(scale), scale.stride(0), _ptr(wq), _ptr(wscale), _ptr(out), out.stride(0), dt, M, N, K,
-                                 _stream_on(ctx)), "nvc_gemm_fp8", ctx.h)
+        check(ctx.l.nvc_gemm_fp8(ctx.h, q.data_ptr(), ldq, scale.data_ptr(), lds, wq.data_ptr(), wscale.data_ptr(), out.data_ptr(), ldo, dt, M, N, K,
+                                 torch._C._cuda_getCurrentRawStream(ctx.device)), "nvc_gemm_fp8", ctx.h)
     return out
 
 
 def gemm_fp8_grouped(ctx, q, scale, wq, wscale, tile_group, out_dtype=BF16, out=None) -> torch.Tensor:
     """Rows sorted by expert (moe_sort_padded, groups padded to 128 rows) times the experts' weights wq [groups, N, K]: rows of tile t use
     wq[tile_group[t]].  Rows of tiles without an expert are zeros, or, in a given `out`, left as they are."""
-    M, N, K, out_, dt = _fp8_product(ctx, q, scale, wq, wscale, out, out_dtype, (wq.shape[0],))
-    _on(ctx, "tile_group", tile_group, torch.int32)
+    M, N, K, ldq, lds, res, ldo, dt = _fp8_product(ctx, q, scale, wq, wscale, out, out_dtype, wq.shape[0] if wq.dim() else 0)
     if M % 128:
         raise ValueError("rows must be a multiple of 128")
-    _whole("tile_group", tile_group, (M // 128,))
+    if tile_group.get_device() != ctx.device or tile_group.dtype is not torch.int32 or tile_group.shape != (M // 128,) or not tile_group.is_contiguous():
+        _refuse(ctx, ("tile_group", tile_group, _I32, (M // 128,), True))
     if M:
-        check(ctx.l.nvc_gemm_fp8_grouped(ctx.h, _ptr(q), q.stride(0), _ptr(scale), scale.stride(0), _ptr(wq), _ptr(wscale), _ptr(out_), out_.stride(0), dt, M, N, K,
-                                         _ptr(tile_group), wq.shape[0], 1 if out is None else 0, _stream_on(ctx)), "nvc_gemm_fp8_grouped", ctx.h)
-    return out_
+        check(ctx.l.nvc_gemm_fp8_grouped(ctx.h, q.data_ptr(), ldq, scale.data_ptr(), lds, wq.data_ptr(), wscale.data_ptr(), res.data_ptr(), ldo,
+                                         dt, M, N, K, tile_group.data_ptr(), wq.shape[0], 1 if out is None else 0, torch._C._cuda_getCurrentRawStream(ctx.device)),
+              "nvc_gemm_fp8_grouped", ctx.h)
+    return res
