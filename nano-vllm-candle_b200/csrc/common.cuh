@@ -50,6 +50,7 @@ struct nvc_ctx {
   int gemm_num_counters = 0;
   int* pd_counters = nullptr;   // arrival tickets of the work-balanced paged decode kernel (zero between launches)
   int pair_clusters[5] = {0, 0, 0, 0, 0};   // co-resident clusters of 2S CTAs of the pair GEMM, S = 1..4
+  int fp8_clusters[9] = {};                 // co-resident clusters of S = 1..8 CTAs, one per SM, of the 8-bit products
   // tensor-parallel communicator (NULL when tp_size == 1)
   nvc_nccl_api* nccl = nullptr;
   void* nccl_comm = nullptr;

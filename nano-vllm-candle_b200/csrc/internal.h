@@ -34,7 +34,7 @@ int nvc_gemm_pair_swapped(nvc_ctx* ctx, const nvc_bf16* X, int ldx, const nvc_bf
 int nvc_gemm_pair_qk(nvc_ctx* ctx, const nvc_bf16* A, int lda, const nvc_bf16* W, nvc_bf16* C, int ldc, int M, int N, int K,
                      const nvc_bf16* qw, const nvc_bf16* kw, float eps, const float* cos_sin, const int32_t* positions,
                      const int32_t* slot_mapping, nvc_bf16* k_cache, nvc_bf16* v_cache, int nh, int kv, void* stream);
-// nvc_gemm_fp8 with the kernel given: 0 = choose
+// nvc_gemm_fp8 with the kernel (1 - 6: up to 16 rows, up to 32, shared tiles, 128 columns, 256, pairs) * 10 + shares of K given: 0 = choose
 int nvc_gemm_fp8_ex(nvc_ctx* ctx, const uint8_t* A, int lda, const float* a_scale, int lds, const uint8_t* W, const float* w_scale, void* C, int ldc, int out_dtype,
                     int M, int Nout, int K, int force, void* stream);
 int nvc_prefill_attn_init(nvc_ctx* ctx);

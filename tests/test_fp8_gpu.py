@@ -229,20 +229,31 @@ def test_weights(ctx, shape, dtype):
 
 # ----------------------------------------------------------------------------- products
 def _operands(seed, M, N, K, groups=None):
-    q, s = ops_quant_cpu(_randn(seed, M, K))
+    q, s = _rows_8bit(_randn(seed, M, K))
     if groups is None:
-        w = [ops_quant_w(_randn(seed + 1, N, K) * K ** -0.5)]
+        w = [_weight_8bit(_randn(seed + 1, N, K) * K ** -0.5)]
         return q, s, w[0][0], w[0][1]
-    w = [ops_quant_w(_randn(seed + 1 + g, N, K) * K ** -0.5) for g in range(groups)]
+    w = [_weight_8bit(_randn(seed + 1 + g, N, K) * K ** -0.5) for g in range(groups)]
     return q, s, torch.stack([a.view(torch.uint8) for a, _ in w]).view(E4M3), torch.stack([b for _, b in w])
 
 
-def ops_quant_cpu(x):
+def _whole_numbers(seed, M, N, K):
+    """Numbers of -3 to 3 with scales that are powers of two, different for every block."""
+    g = _g(seed)
+    q = torch.randint(-3, 4, (M, K), generator=g, device=DEV).float().to(E4M3)
+    wq = torch.randint(-3, 4, (N, K), generator=g, device=DEV).float().to(E4M3)
+    kb = (K + 127) // 128
+    s = torch.exp2(torch.randint(-2, 3, (M, kb), generator=g, device=DEV).float())
+    ws = torch.exp2(torch.randint(-2, 3, ((N + 127) // 128, kb), generator=g, device=DEV).float())
+    return q, s, wq, ws
+
+
+def _rows_8bit(x):
     s = _scale32(x)
     return (x * _spread(1.0 / s, x.shape[1])).to(E4M3), s
 
 
-def ops_quant_w(x):
+def _weight_8bit(x):
     s = _scale32(x, 128)
     inv = (1.0 / s).repeat_interleave(128, 0)[:x.shape[0]].repeat_interleave(128, 1)[:, :x.shape[1]]
     return (x * inv).to(E4M3), s
@@ -273,14 +284,28 @@ def test_product(ctx, M, N, K, out_dtype):
 @pytest.mark.parametrize("M,N,K", [(1, 272, 1040), (5, 1024, 4096), (64, 640, 2048), (130, 400, 1040), (300, 1040, 2064), (1030, 784, 1040)])
 def test_product_of_whole_numbers_is_exact(ctx, M, N, K):
     """Small whole numbers and scales that are powers of two, different for every block: every sum is exact, so every index is the right one."""
-    g = _g(M)
-    q = torch.randint(-3, 4, (M, K), generator=g, device=DEV).float().to(E4M3)
-    wq = torch.randint(-3, 4, (N, K), generator=g, device=DEV).float().to(E4M3)
-    kb = (K + 127) // 128
-    s = torch.exp2(torch.randint(-2, 3, (M, kb), generator=g, device=DEV).float())
-    ws = torch.exp2(torch.randint(-2, 3, ((N + 127) // 128, kb), generator=g, device=DEV).float())
+    q, s, wq, ws = _whole_numbers(M, M, N, K)
     got = ops.gemm_fp8(ctx, q, s, wq, ws, out_dtype=F32)
     assert torch.equal(got.to(F64), _dequant(q, s) @ _dequant_w(wq, ws).T)
+
+
+ROUTES = [10 * tile + shares for tile in (1, 2, 3) for shares in range(1, 9)] + [41, 51, 61]
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 16, 16), (5, 272, 1040), (17, 640, 2064), (64, 1024, 8192), (130, 400, 1040), (140, 176, 128), (257, 400, 272), (600, 48, 256), (1030, 784, 1040)])
+def test_every_kernel_and_share(ctx, M, N, K):
+    """Every kernel of a dense product with every share of K, for sizes it would not be chosen for too: exact sums, nothing written beside them."""
+    q, s, wq, ws = _whole_numbers(M, M, N, K)
+    want = _dequant(q, s) @ _dequant_w(wq, ws).T
+    for route in ROUTES:
+        for dt in (F32, BF16):
+            c = torch.full((M + 2, N + 8), 7.0, dtype=dt, device=DEV)
+            for _ in range(3):
+                c[1:1 + M, :N] = -1.0
+                assert ctx.l.nvc_gemm_fp8_ex(ctx.h, q.data_ptr(), K, s.data_ptr(), s.shape[1], wq.data_ptr(), ws.data_ptr(), c[1:].data_ptr(), N + 8, int(dt == F32), M, N, K, route,
+                                             torch.cuda.current_stream().cuda_stream) == 0
+                assert torch.equal(c[1:1 + M, :N], want.to(dt)), (route, dt)
+            assert torch.all(c[0] == 7.0) and torch.all(c[1 + M] == 7.0) and torch.all(c[:, N:] == 7.0), (route, dt)
 
 
 @pytest.mark.parametrize("out_dtype", [BF16, F32])
@@ -427,7 +452,7 @@ def test_experts_in_8_bits(ctx):
     for e in range(E):
         f = (a @ _dequant_w(wg[e], sg[e]).T).to(BF16).to(F64)
         u = f[:, :I] * torch.sigmoid(f[:, :I]) * f[:, I:]
-        qe, se = ops_quant_cpu(u.float())
+        qe, se = _rows_8bit(u.float())
         o = _dequant(qe, se) @ _dequant_w(wd[e], sd[e]).T
         weight = torch.where(idx == e, tw, torch.zeros((), device=DEV)).sum(1, keepdim=True).to(F64)
         want += weight * o
