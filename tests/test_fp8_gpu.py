@@ -180,7 +180,7 @@ def test_rows_with_strides(ctx):
 
 
 # ----------------------------------------------------------------------------- norm
-@pytest.mark.parametrize("N,H", [(1, 16), (1, 1024), (2, 128), (3, 1040), (64, 2560), (33, 4096), (5, 12288), (2, 16384)])
+@pytest.mark.parametrize("N,H", [(1, 16), (1, 1024), (2, 128), (3, 1040), (64, 2560), (33, 4096), (5, 12288), (2, 16384), (40000, 16), (2100, 256), (700, 1040), (1000, 4096), (297, 16384)])
 @pytest.mark.parametrize("with_res", [False, True])
 @pytest.mark.parametrize("dtype,wdtype", [(BF16, BF16), (F32, F32), (BF16, F32), (F32, BF16)])
 def test_add_rmsnorm_fp8(ctx, N, H, with_res, dtype, wdtype):
