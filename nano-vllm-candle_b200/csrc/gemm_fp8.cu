@@ -184,6 +184,8 @@ struct Cfg {
   static constexpr int kAcc = BN == 256 ? 2 : 4;                             // accumulators
   static constexpr int kTmemCols = kAcc * BN;
   static constexpr int kThreads = 384;
+  // a k-block's operands are asked for ahead by the warp that issues it: an answer is only unmistakable where it is the same warp that waited for the stage's last use
+  static_assert(kStages % 2 == 0 && kAcc % 2 == 0, "two issuing warps");
   static constexpr int kBufs = 1;                                            // 4 KB each, per epilogue warp
   static constexpr int kOffStaging = kStages * kStageBytes;
   static constexpr int kOffBar = kOffStaging + 8 * kBufs * 4096;
@@ -475,6 +477,7 @@ struct SplitCfg {
   static constexpr int kAcc = 4;
   static constexpr int kTmemCols = kAcc * NT;
   static constexpr int kIssuers = kSwap ? 1 : 2, kFirst = kSwap ? 2 : 4;     // warps that issue products, the first one that sums
+  static_assert(kStages % kIssuers == 0 && kAcc % kIssuers == 0, "as in Cfg");
   static constexpr int kSides = kSwap ? 1 : 2, kCols = NT / kSides, kRead = NT == 32 ? 32 : 16;
   static constexpr int kSumThreads = 128 * kSides, kThreads = 32 * kFirst + kSumThreads;
   static constexpr int kTableKb = 32, kPitch = NT + 4;                       // the table: k-blocks, floats per k-block
@@ -897,7 +900,16 @@ extern "C" int nvc_gemm_fp8_grouped(nvc_ctx* ctx, const nvc_fp8* A, int lda, con
   DeviceGuard guard(ctx->device);
   const Args a = {a_scale, w_scale, tile_group, lds, out_dtype == NVC_DT_F32, M_cap, Nout, (K + BK - 1) / BK, 0, 0, 0, 1, zero != 0, BM};
   const Call c = {A, lda, W, C, ldc, K, groups, nvc_stream(stream)};
-  const int64_t m_tiles = M_cap / BM;
-  if (m_tiles * ((Nout + 255) / 256) <= ctx->num_sms) return launch<128, true>(ctx, c, a);
+  // The times of choose_route over the tiles that there may be: M_cap holds the rows, groups x 127 of padding and up to 127 of rounding; a group of up to 112 rows fills one
+  // tile, a larger one half a tile more than its rows.  128 columns where they promise no more than 6 % above 256, since routers leave some groups empty, and fewer wide tiles
+  // leave SMs idle (us, 128 / 256: 64 tokens, 24 groups, 10 of them used, 1 536 x 2 048 12.8 / 15.1; 600, 8 groups, 4 096 x 1 024 15.2 / 16.3; 2 500, 16 groups, 2 048 x 2 048
+  // 21.8 / 23.6; 8 000, 16 groups, 4 096 x 2 048 89.7 / 83.5)
+  const double rows = std::max((double)M_cap - 127.0 * groups - 64.0, 1.0), per = rows / groups;
+  const double m_tiles = groups * (per <= 112.0 ? std::min(per, 1.0) : per / BM + 0.5), mb = std::min(rows, (double)groups) * Nout * K * 1e-6;
+  auto time = [&](int cols, double start, double wave, double kb, double full, double weights) {
+    const double n = m_tiles * ((Nout + cols - 1) / cols) / ctx->num_sms;
+    return start + std::ceil(n) * (wave + a.num_kb * (kb + full * std::min(n, 1.0))) + weights * mb;
+  };
+  if (time(128, 2.48, 0.61, 0.240, 0.053, 0.0335) <= 1.06 * time(256, 2.71, 1.31, 0.372, 0.104, 0.0438)) return launch<128, true>(ctx, c, a);
   return launch<256, true>(ctx, c, a);
 }

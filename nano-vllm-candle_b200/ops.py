@@ -923,7 +923,7 @@ _DTYPE_CODE = {torch.bfloat16: 0, torch.float32: 1}
 
 
 # The arguments of a call are looked at in one expression, since a short kernel waits for its call (a norm of one row: 13.2 us with a function per argument and property,
-# 9.1 so); only where something is wrong does _refuse look for it one by one.
+# 9.9 so); only where something is wrong does _refuse look for it one by one.
 def _refuse(ctx, *facts):
     """facts: (name, tensor, types it may have, shape it has to have or None, whether it has to be contiguous)."""
     for name, t, types, shape, whole in facts:
@@ -945,23 +945,14 @@ def _refuse(ctx, *facts):
 _ROWS, _F32, _I32, _E4M3 = (torch.bfloat16, torch.float32), (torch.float32,), (torch.int32,), (FP8,)
 
 
-def _fp8_rows_out(ctx, q, scale, n: int, width: int, device):
-    """The rows and scales to write, new ones or those given, and their row strides."""
+def _fp8_rows_given(ctx, q, scale, n: int, width: int):
+    """The row strides of rows and scales that a caller gave to write to."""
     blocks = (width + 127) // 128
-    ldq, lds = width, blocks
-    if q is None:
-        q = torch.empty(n, width, dtype=FP8, device=device)
-    else:
-        if q.get_device() != ctx.device or q.dtype is not FP8 or q.shape != (n, width) or (width > 1 and q.stride(1) != 1):
-            _refuse(ctx, ("q", q, _E4M3, (n, width), False))
-        ldq = q.stride(0)
-    if scale is None:
-        scale = torch.empty(n, blocks, dtype=torch.float32, device=device)
-    else:
-        if scale.get_device() != ctx.device or scale.dtype is not torch.float32 or scale.shape != (n, blocks) or (blocks > 1 and scale.stride(1) != 1):
-            _refuse(ctx, ("scale", scale, _F32, (n, blocks), False))
-        lds = scale.stride(0)
-    return q, scale, ldq, lds
+    if q.get_device() != ctx.device or q.dtype is not FP8 or q.shape != (n, width) or (width > 1 and q.stride(1) != 1):
+        _refuse(ctx, ("q", q, _E4M3, (n, width), False))
+    if scale.get_device() != ctx.device or scale.dtype is not torch.float32 or scale.shape != (n, blocks) or (blocks > 1 and scale.stride(1) != 1):
+        _refuse(ctx, ("scale", scale, _F32, (n, blocks), False))
+    return q.stride(0), scale.stride(0)
 
 
 def quant_fp8(ctx, x: torch.Tensor, act: int = ACT_NONE, rows=None, num_rows=None, q=None, scale=None):
@@ -969,24 +960,41 @@ def quant_fp8(ctx, x: torch.Tensor, act: int = ACT_NONE, rows=None, num_rows=Non
     x: bf16 or fp32 [*, H], or [*, 2 H] for ACT_SILU_MUL and ACT_GELU_TANH_MUL (act(left half) * right half; ACT_RELU2: max(x, 0)^2).
     rows: int32 [N], the row of x for each row of the result, negative for zeros (src of moe_sort_padded); num_rows: int32 [1], rows from it on are
     left as they are (offsets[E:] of moe_sort_padded).  q, scale: where to write."""
+    dev = ctx.device
     dt = _DTYPE_CODE.get(x.dtype)
-    if dt is None or x.get_device() != ctx.device or x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
+    if dt is None or x.get_device() != dev or x.dim() != 2:
         _refuse(ctx, ("x", x, _ROWS, None, False))
     N, H = x.shape
+    ldx = H
+    if not x.is_contiguous():
+        ldx, one = x.stride()
+        if one != 1 and H > 1:
+            _refuse(ctx, ("x", x, _ROWS, None, False))
     if act == ACT_SILU_MUL or act == ACT_GELU_TANH_MUL:
         if H % 2:
             raise ValueError("a gated unit takes two halves of equal width")
         H //= 2
+    rows_at = num_at = None
     if rows is not None:
-        if rows.get_device() != ctx.device or rows.dtype is not torch.int32 or rows.dim() != 1 or not rows.is_contiguous():
+        if rows.get_device() != dev or rows.dtype is not torch.int32 or rows.dim() != 1 or not rows.is_contiguous():
             _refuse(ctx, ("rows", rows, _I32, (rows.numel(),), True))
-        N = rows.shape[0]
-    if num_rows is not None and (num_rows.get_device() != ctx.device or num_rows.dtype is not torch.int32 or num_rows.numel() < 1):
-        _refuse(ctx, ("num_rows", num_rows, _I32, None, False))
-    q, scale, ldq, lds = _fp8_rows_out(ctx, q, scale, N, H, x.device)
+        N, rows_at = rows.numel(), rows.data_ptr()
+    if num_rows is not None:
+        if num_rows.get_device() != dev or num_rows.dtype is not torch.int32 or num_rows.numel() < 1:
+            _refuse(ctx, ("num_rows", num_rows, _I32, None, False))
+        num_at = num_rows.data_ptr()
+    ldq, lds = H, (H + 127) // 128
+    if q is None and scale is None:
+        q, scale = x.new_empty(N, ldq, dtype=FP8), x.new_empty(N, lds, dtype=torch.float32)
+    else:
+        q = x.new_empty(N, H, dtype=FP8) if q is None else q
+        scale = x.new_empty(N, lds, dtype=torch.float32) if scale is None else scale
+        ldq, lds = _fp8_rows_given(ctx, q, scale, N, H)
     if N:
-        check(ctx.l.nvc_quant_fp8_rows(ctx.h, x.data_ptr(), dt, x.stride(0), act, H, _ptr(rows), _ptr(num_rows), q.data_ptr(), ldq, scale.data_ptr(), lds, N, H,
-                                       torch._C._cuda_getCurrentRawStream(ctx.device)), "nvc_quant_fp8_rows", ctx.h)
+        st = ctx.l.nvc_quant_fp8_rows(ctx.h, x.data_ptr(), dt, ldx, act, H, rows_at, num_at, q.data_ptr(), ldq, scale.data_ptr(), lds, N, H,
+                                      torch._C._cuda_getCurrentRawStream(dev))
+        if st:
+            check(st, "nvc_quant_fp8_rows", ctx.h)
     return q, scale
 
 
@@ -1008,20 +1016,34 @@ def quant_fp8_weight(ctx, w: torch.Tensor):
 def add_rmsnorm_fp8(ctx, x: torch.Tensor, w: torch.Tensor, eps: float, residual=None, residual_out=None, want_out: bool = False, q=None, scale=None):
     """fused_add_rmsnorm with rows in 8 bits behind it: (q, scale, out).  x: bf16 or fp32 [N, H]; w: bf16 or fp32 [H]; residual (added) and residual_out (the
     sum; may be residual): fp32 [N, H]; out: the normed rows in bf16 when want_out, else None."""
-    dt, wdt, dev = _DTYPE_CODE.get(x.dtype), _DTYPE_CODE.get(w.dtype), ctx.device
-    shape = x.shape
-    if (dt is None or wdt is None or x.get_device() != dev or w.get_device() != dev or len(shape) != 2 or w.shape != shape[1:] or not x.is_contiguous() or not w.is_contiguous()
-            or (residual is not None and (residual.get_device() != dev or residual.dtype is not torch.float32 or residual.shape != shape or not residual.is_contiguous()))
-            or (residual_out is not None and (residual_out.get_device() != dev or residual_out.dtype is not torch.float32 or residual_out.shape != shape
-                                              or not residual_out.is_contiguous()))):
+    dev, dt, wdt, shape = ctx.device, _DTYPE_CODE.get(x.dtype), _DTYPE_CODE.get(w.dtype), x.shape
+    res_at = res_out_at = None
+    good = dt is not None and wdt is not None and len(shape) == 2 and x.is_contiguous() and w.is_contiguous() and x.get_device() == dev and w.get_device() == dev
+    if good and residual is not None:
+        res_at = residual.data_ptr()
+        good = residual.dtype is torch.float32 and residual.get_device() == dev and residual.shape == shape and residual.is_contiguous()
+    if good and residual_out is not None:
+        res_out_at = residual_out.data_ptr()
+        good = residual_out.dtype is torch.float32 and residual_out.get_device() == dev and residual_out.shape == shape and residual_out.is_contiguous()
+    if not good or w.dim() != 1 or w.numel() != shape[1]:
         _refuse(ctx, ("x", x, _ROWS, None, True), ("w", w, _ROWS, shape[-1:], True), ("residual", residual, _F32, shape, True),
                 ("residual_out", residual_out, _F32, shape, True))
     N, H = shape
-    q, scale, ldq, lds = _fp8_rows_out(ctx, q, scale, N, H, x.device)
-    out = torch.empty(N, H, dtype=BF16, device=x.device) if want_out else None
+    ldq, lds, out, out_at = H, (H + 127) // 128, None, None
+    if q is None and scale is None:
+        q, scale = x.new_empty(N, ldq, dtype=FP8), x.new_empty(N, lds, dtype=torch.float32)
+    else:
+        q = x.new_empty(N, H, dtype=FP8) if q is None else q
+        scale = x.new_empty(N, lds, dtype=torch.float32) if scale is None else scale
+        ldq, lds = _fp8_rows_given(ctx, q, scale, N, H)
+    if want_out:
+        out = x.new_empty(N, H, dtype=BF16)
+        out_at = out.data_ptr()
     if N:
-        check(ctx.l.nvc_add_rmsnorm_fp8(ctx.h, x.data_ptr(), dt, _ptr(residual), _ptr(residual_out), w.data_ptr(), wdt, eps, q.data_ptr(), ldq, scale.data_ptr(), lds,
-                                        _ptr(out), N, H, torch._C._cuda_getCurrentRawStream(dev)), "nvc_add_rmsnorm_fp8", ctx.h)
+        st = ctx.l.nvc_add_rmsnorm_fp8(ctx.h, x.data_ptr(), dt, res_at, res_out_at, w.data_ptr(), wdt, eps, q.data_ptr(), ldq, scale.data_ptr(), lds, out_at, N, H,
+                                       torch._C._cuda_getCurrentRawStream(dev))
+        if st:
+            check(st, "nvc_add_rmsnorm_fp8", ctx.h)
     return q, scale, out
 
 
@@ -1046,7 +1068,7 @@ def _fp8_product(ctx, q, scale, wq, wscale, out, out_dtype, groups):
     if out is None:
         code, ldo = _DTYPE_CODE.get(out_dtype), N
         if good and code is not None:
-            return M, N, K, ldq, lds, torch.empty(M, N, dtype=out_dtype, device=q.device), ldo, code
+            return M, N, K, ldq, lds, q.new_empty(M, N, dtype=out_dtype), ldo, code
         if code is None:
             raise TypeError(f"bf16 or fp32 expected, got {out_dtype}")
     else:
@@ -1061,8 +1083,10 @@ def gemm_fp8(ctx, q, scale, wq, wscale, out_dtype=BF16, out=None) -> torch.Tenso
     """[M, N] = rows times weight, both in 8 bits: (q, scale) of quant_fp8 or add_rmsnorm_fp8, (wq, wscale) of quant_fp8_weight; bf16 or fp32."""
     M, N, K, ldq, lds, out, ldo, dt = _fp8_product(ctx, q, scale, wq, wscale, out, out_dtype, None)
     if M:
-        check(ctx.l.nvc_gemm_fp8(ctx.h, q.data_ptr(), ldq, scale.data_ptr(), lds, wq.data_ptr(), wscale.data_ptr(), out.data_ptr(), ldo, dt, M, N, K,
-                                 torch._C._cuda_getCurrentRawStream(ctx.device)), "nvc_gemm_fp8", ctx.h)
+        st = ctx.l.nvc_gemm_fp8(ctx.h, q.data_ptr(), ldq, scale.data_ptr(), lds, wq.data_ptr(), wscale.data_ptr(), out.data_ptr(), ldo, dt, M, N, K,
+                                torch._C._cuda_getCurrentRawStream(ctx.device))
+        if st:
+            check(st, "nvc_gemm_fp8", ctx.h)
     return out
 
 
