@@ -7,6 +7,10 @@ computation is a call through the C ABI (ops.Context).  No CPU path: a CPU tenso
   SiluAndMul         src/layers/activation.rs:4-18
   *ParallelLinear    src/layers/linear.rs:4-223         load_weights(weight, bias) / forward(x)
   Attention          src/layers/attention.rs:4-16       forward(q, k, v) + per-step Context
+
+Beyond the reference: the linear layers run in 8 bits after to_fp8() (their loaded weights are converted) or load_fp8() (a checkpoint's own e4m3 weights with
+a scale for each 128 x 128), and take rows that are in 8 bits already - (q, scale), as RMSNorm.forward_fp8 and SiluAndMul.forward_fp8 give them - in place of
+a tensor.
 """
 from __future__ import annotations
 
@@ -15,6 +19,7 @@ from typing import List, Optional, Tuple
 
 import torch
 
+from . import ops
 from .tp import TPConfig, get_tp
 
 BF16 = torch.bfloat16
@@ -43,6 +48,18 @@ class RMSNorm:
         new_res = torch.empty_like(r2)
         out = self.ctx.fused_add_rmsnorm(x2, self.weight, self.eps, residual_in=r2, residual_out=new_res)
         return out.reshape(shape), new_res.reshape(shape)
+
+    def forward_fp8(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None):
+        """The same with the normed rows in 8 bits: ((q [rows, hidden], scale [rows, ceil(hidden / 128)]), new_residual f32 or None)."""
+        shape = x.shape
+        x2 = x.reshape(-1, shape[-1]).contiguous()
+        if residual is None:
+            q, scale, _ = ops.add_rmsnorm_fp8(self.ctx, x2, self.weight, self.eps)
+            return (q, scale), None
+        r2 = residual.reshape(-1, shape[-1]).to(torch.float32).contiguous()
+        new_res = torch.empty_like(r2)
+        q, scale, _ = ops.add_rmsnorm_fp8(self.ctx, x2, self.weight, self.eps, residual=r2, residual_out=new_res)
+        return (q, scale), new_res.reshape(shape)
 
 
 class RotaryEmbedding:
@@ -77,6 +94,10 @@ class SiluAndMul:
         out = self.ctx.silu_and_mul(x.reshape(-1, shape[-1]).contiguous())
         return out.reshape(*shape[:-1], shape[-1] // 2)
 
+    def forward_fp8(self, x: torch.Tensor):
+        """The same with rows in 8 bits: (q [rows, width / 2], scale)."""
+        return ops.quant_fp8(self.ctx, x.reshape(-1, x.shape[-1]), act=ops.ACT_SILU_MUL)
+
 
 # ----------------------------------------------------------------------------- linear family
 class LinearBase:
@@ -88,15 +109,37 @@ class LinearBase:
         self.tp_dim, self.tp_rank, self.tp_size = tp_dim, tp.rank, tp.size
         self.input_size, self.output_size = input_size, output_size
         self.weight: Optional[torch.Tensor] = None
+        self.weight_fp8: Optional[Tuple[torch.Tensor, torch.Tensor]] = None       # (e4m3 [out, in], scale [ceil(out / 128), ceil(in / 128)])
+
+    def to_fp8(self) -> "LinearBase":
+        """Converts the loaded weight (this rank's share of it) to 8 bits, once; the bf16 weight is given up."""
+        if self.weight is None:
+            raise RuntimeError("load_weights has not been called")
+        self.weight_fp8, self.weight = ops.quant_fp8_weight(self.ctx, self.weight), None
+        return self
+
+    def load_fp8(self, weight: torch.Tensor, scale: torch.Tensor) -> None:
+        """This rank's weight as e4m3 [out, in] with its scales [ceil(out / 128), ceil(in / 128)]."""
+        n, k = weight.shape
+        if weight.dtype != ops.FP8 or tuple(scale.shape) != ((n + 127) // 128, (k + 127) // 128):
+            raise ValueError("load_fp8: an e4m3 weight [out, in] and scales [ceil(out / 128), ceil(in / 128)]")
+        self.weight_fp8, self.weight = (weight.contiguous(), scale.to(torch.float32).contiguous()), None
 
     def _set(self, w: torch.Tensor, bias):
         if bias is not None:
             raise NotImplementedError("bias: the Qwen3 path has none (every call site passes None, qwen3.rs:121,123)")
-        self.weight = w.to(BF16).contiguous()
+        self.weight, self.weight_fp8 = w.to(BF16).contiguous(), None
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x) -> torch.Tensor:
+        """x: [..., in], or rows in 8 bits (q, scale) for a layer whose weight is in 8 bits."""
+        if self.weight_fp8 is not None:
+            rows = x if isinstance(x, tuple) else ops.quant_fp8(self.ctx, x.reshape(-1, x.shape[-1]))
+            y = ops.gemm_fp8(self.ctx, *rows, *self.weight_fp8)
+            return y if isinstance(x, tuple) else y.reshape(*x.shape[:-1], y.shape[1])
         if self.weight is None:
             raise RuntimeError("load_weights has not been called")
+        if isinstance(x, tuple):
+            raise ValueError("rows in 8 bits need a weight in 8 bits: to_fp8() or load_fp8()")
         shape = x.shape
         y = self.ctx.gemm(x.reshape(-1, shape[-1]), self.weight)
         return y.reshape(*shape[:-1], self.weight.shape[0])
