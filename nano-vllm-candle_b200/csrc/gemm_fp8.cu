@@ -60,11 +60,19 @@ __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
   return ok != 0;
 }
 
+// ptx::mbar_wait without its message: a call in the loop takes registers that hold sums otherwise (8 192 x 24 576 x 4 096 572 us with the message, 535 without)
+__device__ __forceinline__ void wait_quietly(uint32_t bar, uint32_t parity) {
+  uint32_t spins = 0;
+  while (!ptx::mbar_try_wait(bar, parity))
+    if (++spins > NVC_MBAR_SPIN_LIMIT) __trap();
+}
+
 // The epilogue's walk over k-blocks: accumulator it % kAcc of tensor memory (kStride columns each), kCols columns of it in reads of kRead.
 // Two warps of a quarter of the SM share its 512 cycles per k-block of 128 x 256, of which the sums take 330 and the reads 256; one after the other in a warp they take longer
 // than that.  So reads are under way two at a time, the next k-block's first ones between the sums of this one's last, and whether it is there is asked for ahead of time (a
 // barrier's answer takes 100 to 200 cycles beside the tensor core's own reads of shared memory).  8 192 x 24 576 x 4 096, us, numbers of zero, which leave the power cap
-// out: 640 with wait, reads and sums in order, 597 with the reads ahead, 555 with the question ahead; the tensor pipe alone, without sums, 383.
+// out: 640 with wait, reads and sums in order, 597 with the reads ahead, 555 with the question ahead, 535 without a call in the loop; without scales to fetch 487 (from a table that
+// another warp fills they take 607), the tensor pipe alone, without sums, 383.
 // step(kb): before the sums of a k-block; sum(c, v): adds read c; release(i): the accumulator has been read out.
 template <int kCols, int kRead, int kAcc, int kStride, typename Full, typename Release, typename Step, typename Sum>
 __device__ __forceinline__ void walk_sums(int num_kb, uint32_t& it, uint32_t taddr, Full full, Release release, Step step, Sum sum) {
@@ -76,7 +84,7 @@ __device__ __forceinline__ void walk_sums(int num_kb, uint32_t& it, uint32_t tad
     if constexpr (kRead == 16) ptx::tmem_ld_32x32b_x16(t + c * kRead, v[c & 1]);
     else ptx::tmem_ld_32x32b_x32(t + c * kRead, v[c & 1]);
   };
-  ptx::mbar_wait(full(it % kAcc), (it / kAcc) & 1);
+  wait_quietly(full(it % kAcc), (it / kAcc) & 1);
   ptx::tcgen05_fence_after();
   read(0);
   if (kReads > 1) read(1);
@@ -101,7 +109,7 @@ __device__ __forceinline__ void walk_sums(int num_kb, uint32_t& it, uint32_t tad
     if (kReads > 1) sum(kReads - 2, v[0]);
     else sum(0, v[0]);
     if (more) {
-      if (!ready) ptx::mbar_wait(next_bar, next_parity);
+      if (!ready) wait_quietly(next_bar, next_parity);
       ptx::tcgen05_fence_after();
       t = taddr + it % kAcc * kStride;
       read(0);
@@ -262,7 +270,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant
       if (kGrouped && grp < 0) continue;
       for (int kb = 0; kb < a.num_kb; ++kb, ++it) {
         const int s = it % cfg::kStages;
-        ptx::mbar_wait(empty_bar(s), ((it / cfg::kStages) & 1) ^ 1u);      // first lap: falls through
+        wait_quietly(empty_bar(s), ((it / cfg::kStages) & 1) ^ 1u);      // first lap: falls through
         ptx::mbar_arrive_expect_tx(full_bar(s), cfg::kBytesB + a.a_box * BK);        // rows of A behind the box hold what they held: their sums are never stored
         const uint32_t dst = base + s * cfg::kStageBytes;
         ptx::tma_load_2d(dst + cfg::kBytesA, &tma_b, full_bar(s), kb * BK, grp * a.N + at.y * BN);
@@ -281,8 +289,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant
       for (int kb = 0; kb < a.num_kb; ++kb, ++it) {
         if ((it & 1) != (uint32_t)(warp - 1)) continue;
         const uint32_t s = it % cfg::kStages, acc = it % cfg::kAcc;
-        if (!here) ptx::mbar_wait(full_bar(s), (it / cfg::kStages) & 1);
-        if (!free) ptx::mbar_wait(acc_empty(acc), ((it / cfg::kAcc) & 1) ^ 1u);      // its last k-block has been read out
+        if (!here) wait_quietly(full_bar(s), (it / cfg::kStages) & 1);
+        if (!free) wait_quietly(acc_empty(acc), ((it / cfg::kAcc) & 1) ^ 1u);      // its last k-block has been read out
         here = mbar_test(full_bar((it + 2) % cfg::kStages), ((it + 2) / cfg::kStages) & 1);
         free = mbar_test(acc_empty((it + 2) % cfg::kAcc), (((it + 2) / cfg::kAcc) & 1) ^ 1u);
         ptx::tcgen05_fence_after();
@@ -402,7 +410,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
       const int2 at = tile_at(tile, a);
       for (int kb = 0; kb < a.num_kb; ++kb, ++it) {
         const int s = it % cfg::kStages;
-        ptx::mbar_wait(empty_bar(s), ((it / cfg::kStages) & 1) ^ 1u);
+        wait_quietly(empty_bar(s), ((it / cfg::kStages) & 1) ^ 1u);
         if (h == 0) ptx::mbar_arrive_expect_tx(full_bar(s), 2 * cfg::kStageBytes);
         const uint32_t dst = base + s * cfg::kStageBytes;
         tma_load_2d_pair(dst, &tma_a, leader_full0 + 8u * s, kb * BK, at.x * 2 * BM + h * BM);
@@ -418,8 +426,8 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
     for (int tile = cluster; tile < a.num_tiles; tile += clusters) {
       for (int kb = 0; kb < a.num_kb; ++kb, ++it) {
         const uint32_t s = it % cfg::kStages, slot = (it & 1) * 2 + half, step = (s * cfg::kStageBytes) >> 4;
-        ptx::mbar_wait(full_bar(s), (it / cfg::kStages) & 1);
-        ptx::mbar_wait(acc_empty(slot), ((it >> 1) & 1) ^ 1u);
+        wait_quietly(full_bar(s), (it / cfg::kStages) & 1);
+        wait_quietly(acc_empty(slot), ((it >> 1) & 1) ^ 1u);
         ptx::tcgen05_fence_after();
 #pragma unroll
         for (int k = 0; k < BK / 32; ++k)
@@ -543,7 +551,7 @@ gemm_fp8_split_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
       const int s = kb % cfg::kStages;
       const uint32_t dst = base + s * cfg::kStageBytes;
       if (kb >= cfg::kStages) {
-        ptx::mbar_wait(empty_bar(s), ((kb / cfg::kStages) & 1) ^ 1u);
+        wait_quietly(empty_bar(s), ((kb / cfg::kStages) & 1) ^ 1u);
         ptx::mbar_arrive_expect_tx(full_bar(s), stage_tx);
         ptx::tma_load_2d(dst, &tma_w, full_bar(s), (kb0 + kb) * BK, n0);
       }
@@ -555,8 +563,8 @@ gemm_fp8_split_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
     bool here = false, free = false;             // what was asked ahead: the operands, the accumulator of this thread's next k-block
     for (uint32_t kb = warp - 1; kb < (uint32_t)num_kb; kb += cfg::kIssuers) {
       const uint32_t s = kb % cfg::kStages, i = kb % cfg::kAcc, next = kb + cfg::kIssuers;
-      if (!here) ptx::mbar_wait(full_bar(s), (kb / cfg::kStages) & 1);
-      if (!free) ptx::mbar_wait(acc_empty(i), ((kb / cfg::kAcc) & 1) ^ 1u);
+      if (!here) wait_quietly(full_bar(s), (kb / cfg::kStages) & 1);
+      if (!free) wait_quietly(acc_empty(i), ((kb / cfg::kAcc) & 1) ^ 1u);
       here = mbar_test(full_bar(next % cfg::kStages), (next / cfg::kStages) & 1);
       free = mbar_test(acc_empty(next % cfg::kAcc), ((next / cfg::kAcc) & 1) ^ 1u);
       ptx::tcgen05_fence_after();
