@@ -728,9 +728,10 @@ typedef uint8_t nvc_fp8;
 enum { NVC_FP8_BLOCK = 128 };
 /* q[i, :H], scale[i, :ceil(H / 128)] = the 8-bit form of f(x[r]), i < N:
  *   NVC_ACT_NONE: f(v) = v[:H];  NVC_ACT_RELU2: max(v[:H], 0)^2;  NVC_ACT_SILU_MUL, NVC_ACT_GELU_TANH_MUL: act(v[:H]) * v[up_off : up_off + H].
- * rows == NULL: r = i; else r = rows[i], and a negative one is a row of zeros (rows of experts: src_rows of nvc_moe_sort_padded).  num_rows != NULL: a
- * count in device memory; rows from it on are left as they are.  x: bf16 or fp32, ldx a multiple of 8; ldq a multiple of 16. */
-int nvc_quant_fp8_rows(nvc_ctx* ctx, const void* x, int x_dtype, int ldx, int act, int up_off, const int32_t* rows, const int32_t* num_rows, nvc_fp8* q,
+ * rows == NULL: r = i; else r = rows[i], and one that is negative or not below x_rows, the rows of x, is a row of zeros (rows of experts: src_rows of
+ * nvc_moe_sort_padded).  num_rows != NULL: a count in device memory; rows from it on are left as they are.  x: bf16 or fp32, ldx a multiple of 8; ldq a
+ * multiple of 16. */
+int nvc_quant_fp8_rows(nvc_ctx* ctx, const void* x, int x_dtype, int ldx, int x_rows, int act, int up_off, const int32_t* rows, const int32_t* num_rows, nvc_fp8* q,
                        int ldq, float* scale, int lds, int N, int H, void* stream);
 /* nvc_fused_add_rmsnorm with 8-bit rows behind it, from the fp32 result:
  *   s = x + residual_in (optional); residual_out = s (optional, may alias);  y = s * rsqrt(mean(s^2) + eps) * w;
@@ -747,7 +748,7 @@ int nvc_quant_fp8_blocks(nvc_ctx* ctx, const void* w, int w_dtype, nvc_fp8* q, f
 int nvc_gemm_fp8(nvc_ctx* ctx, const nvc_fp8* A, int lda, const float* a_scale, int lds, const nvc_fp8* W, const float* w_scale, void* C, int ldc,
                  int out_dtype, int M, int Nout, int K, void* stream);
 /* The same for rows sorted by expert (nvc_gemm_bf16_grouped): rows [128 t, 128 t + 128) use W[tile_group[t]] and its scales.  Rows of tiles with a
- * negative tile_group become zeros (zero != 0) or are left as they are. */
+ * tile_group that is negative or not below `groups` become zeros (zero != 0) or are left as they are. */
 int nvc_gemm_fp8_grouped(nvc_ctx* ctx, const nvc_fp8* A, int lda, const float* a_scale, int lds, const nvc_fp8* W, const float* w_scale, void* C, int ldc,
                          int out_dtype, int M_cap, int Nout, int K, const int32_t* tile_group, int groups, int zero, void* stream);
 

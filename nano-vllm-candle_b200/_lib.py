@@ -149,7 +149,7 @@ def _declare(l: C.CDLL) -> None:
         "nvc_short_conv_advance": [_vp, _vp, _vp, _i, _i, _vp, _i, _vp, _vp],
         "nvc_memory_scan": [_vp, _vp, _i, _i, _vp],
         "nvc_gemm_bf16_glu_clamp_mul": [_vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _f, _vp],
-        "nvc_quant_fp8_rows": [_vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _vp],
+        "nvc_quant_fp8_rows": [_vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _vp],
         "nvc_quant_fp8_blocks": [_vp, _vp, _i, _vp, _vp, _i, _i, _i, _vp],
         "nvc_add_rmsnorm_fp8": [_vp, _vp, _i, _vp, _vp, _vp, _i, _f, _vp, _i, _vp, _i, _vp, _i, _i, _vp],
         "nvc_gemm_fp8": [_vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp],

@@ -94,7 +94,7 @@ template <> struct HeldOf<__nv_bfloat16> { using type = Packed16; };
 // kFlat: blocks of all rows one behind the other, four to a warp, where stretches would leave lanes without columns (8 191 x 1 040: 6.7 us in stretches).
 template <typename T, int kAct, bool kLoop, bool kFlat>
 __global__ void __launch_bounds__(32 * kRowsPerCta)
-quant_rows_kernel(const T* x, int64_t ldx, int up_off, const int32_t* rows, const int32_t* num_rows, uint8_t* __restrict__ q, int64_t ldq,
+quant_rows_kernel(const T* x, int64_t ldx, int x_rows, int up_off, const int32_t* rows, const int32_t* num_rows, uint8_t* __restrict__ q, int64_t ldq,
                   float* __restrict__ scale, int64_t lds, int N, int H, int parts) {
   using Held = typename HeldOf<T>::type;
   constexpr bool kGated = kAct == NVC_ACT_SILU_MUL || kAct == NVC_ACT_GELU_TANH_MUL;
@@ -123,7 +123,7 @@ quant_rows_kernel(const T* x, int64_t ldx, int up_off, const int32_t* rows, cons
     there = col_next < H;
     if (!there) return;
     const int64_t src = rows ? rows[r_next] : r_next;
-    there = src >= 0;
+    there = src >= 0 && (!rows || src < x_rows);
     if (there) {
       const T* p = x + src * ldx + col_next;
       y_next.load(p);
@@ -360,6 +360,7 @@ quant_blocks_kernel(const T* w, uint8_t* __restrict__ q, float* __restrict__ sca
     }
   }
   if (threadIdx.x == 0) scale[((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x] = s;
+  __threadfence();                               // a product may fetch weights as soon as the last CTA has ended
 }
 
 template <typename T, bool kFlat>
@@ -374,10 +375,11 @@ bool dtype_ok(int dt) { return dt == NVC_DT_BF16 || dt == NVC_DT_F32; }
 
 }  // namespace
 
-extern "C" int nvc_quant_fp8_rows(nvc_ctx* ctx, const void* x, int x_dtype, int ldx, int act, int up_off, const int32_t* rows, const int32_t* num_rows, nvc_fp8* q,
+extern "C" int nvc_quant_fp8_rows(nvc_ctx* ctx, const void* x, int x_dtype, int ldx, int x_rows, int act, int up_off, const int32_t* rows, const int32_t* num_rows, nvc_fp8* q,
                                   int ldq, float* scale, int lds, int N, int H, void* stream) {
   NVC_REQUIRE(ctx, ctx && x && q && scale, NVC_EINVAL, "null pointer");
-  NVC_REQUIRE(ctx, N >= 0 && H > 0 && dtype_ok(x_dtype), NVC_EINVAL, "bad sizes or dtype");
+  NVC_REQUIRE(ctx, N >= 0 && H > 0 && x_rows >= 0 && dtype_ok(x_dtype), NVC_EINVAL, "bad sizes or dtype");
+  NVC_REQUIRE(ctx, rows || N <= x_rows, NVC_EINVAL, "more rows than x has");
   NVC_REQUIRE(ctx, act == NVC_ACT_NONE || act == NVC_ACT_RELU2 || act == NVC_ACT_GELU_TANH_MUL || act == NVC_ACT_SILU_MUL, NVC_EINVAL,
               "act must be NVC_ACT_NONE, _RELU2, _GELU_TANH_MUL or _SILU_MUL");
   const bool gated = act == NVC_ACT_GELU_TANH_MUL || act == NVC_ACT_SILU_MUL;
@@ -397,7 +399,7 @@ extern "C" int nvc_quant_fp8_rows(nvc_ctx* ctx, const void* x, int x_dtype, int 
   DeviceGuard guard(ctx->device);
   NVC_DISPATCH_DT(x_dtype, T, {
     auto* kernel = flat ? rows_kernel<T, true>(act) : rows_kernel<T, false>(act);
-    NVC_CUDA_CHECK(ctx, nvc_launch(ctx, kernel, dim3((unsigned)grid), dim3(32 * kRowsPerCta), 0, nvc_stream(stream), static_cast<const T*>(x), (int64_t)ldx, up_off, rows,
+    NVC_CUDA_CHECK(ctx, nvc_launch(ctx, kernel, dim3((unsigned)grid), dim3(32 * kRowsPerCta), 0, nvc_stream(stream), static_cast<const T*>(x), (int64_t)ldx, x_rows, up_off, rows,
                                    num_rows, q, (int64_t)ldq, scale, (int64_t)lds, N, H, flat ? blocks : stretches));
   });
   NVC_CUDA_CHECK(ctx, cudaGetLastError());

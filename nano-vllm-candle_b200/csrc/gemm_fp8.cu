@@ -207,7 +207,7 @@ struct Args {
   const float* w_scale;
   const int32_t* tile_group;        // nullptr: dense
   int64_t lds;
-  int out_f32, M, N, num_kb, num_tiles, n_tiles, m_tiles, band, zero, a_box;       // a_box: rows of A that a copy brings, 128 or, of fewer, those that exist
+  int out_f32, M, N, num_kb, num_tiles, n_tiles, m_tiles, band, zero, groups, a_box;       // a_box: rows of A that a copy brings, 128 or, of fewer, those that exist
 };
 
 // Tile number -> row tile, column tile: bands of `band` row tiles, the row tiles of a band fastest (band 1: column tiles fastest)
@@ -257,7 +257,11 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(gen + cfg::kOffBar + cfg::kNumBars * 8);
   pdl_wait();
   // every role walks the same tiles; the group of the next one is fetched a tile ahead (past L1: an earlier kernel of the stream wrote the table)
-  auto group_of = [&](int tile) { return !kGrouped ? 0 : (tile < a.num_tiles ? __ldcg(a.tile_group + tile / a.n_tiles) : -1); };
+  auto group_of = [&](int tile) {
+    if (!kGrouped) return 0;
+    const int grp = tile < a.num_tiles ? __ldcg(a.tile_group + tile / a.n_tiles) : -1;
+    return grp < a.groups ? grp : -1;
+  };
   int next = group_of(blockIdx.x);
   // registers: the epilogue's two warpgroups hold up to 128 sums each thread, the first warpgroup next to nothing: 128 x 56 + 256 x 224 = 384 x 168
   if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
@@ -880,7 +884,7 @@ extern "C" int nvc_gemm_fp8_ex(nvc_ctx* ctx, const nvc_fp8* A, int lda, const fl
   int rc = nvc_gemm_fp8_check(ctx, A, lda, a_scale, lds, W, w_scale, C, ldc, out_dtype, M, Nout, K, 1);
   if (rc || M == 0) return rc;
   DeviceGuard guard(ctx->device);
-  const Args a = {a_scale, w_scale, nullptr, lds, out_dtype == NVC_DT_F32, M, Nout, (K + BK - 1) / BK, 0, 0, 0, 1, 0, BM};
+  const Args a = {a_scale, w_scale, nullptr, lds, out_dtype == NVC_DT_F32, M, Nout, (K + BK - 1) / BK, 0, 0, 0, 1, 0, 1, BM};
   const Call c = {A, lda, W, C, ldc, K, 1, nvc_stream(stream)};
   const Route r = force ? Route{force / 10, force % 10} : choose_route(ctx, M, Nout, a.num_kb);
   switch (r.tile) {
@@ -906,7 +910,7 @@ extern "C" int nvc_gemm_fp8_grouped(nvc_ctx* ctx, const nvc_fp8* A, int lda, con
   NVC_REQUIRE(ctx, M_cap % BM == 0, NVC_EINVAL, "M_cap must be a multiple of 128");
   if (M_cap == 0) return NVC_OK;
   DeviceGuard guard(ctx->device);
-  const Args a = {a_scale, w_scale, tile_group, lds, out_dtype == NVC_DT_F32, M_cap, Nout, (K + BK - 1) / BK, 0, 0, 0, 1, zero != 0, BM};
+  const Args a = {a_scale, w_scale, tile_group, lds, out_dtype == NVC_DT_F32, M_cap, Nout, (K + BK - 1) / BK, 0, 0, 0, 1, zero != 0, groups, BM};
   const Call c = {A, lda, W, C, ldc, K, groups, nvc_stream(stream)};
   // The times of choose_route over the tiles that there may be: M_cap holds the rows, groups x 127 of padding and up to 127 of rounding; a group of up to 112 rows fills one
   // tile, a larger one half a tile more than its rows.  128 columns where they promise no more than 6 % above 256, since routers leave some groups empty, and fewer wide tiles

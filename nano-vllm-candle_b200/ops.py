@@ -958,14 +958,14 @@ def _fp8_rows_given(ctx, q, scale, n: int, width: int):
 def quant_fp8(ctx, x: torch.Tensor, act: int = ACT_NONE, rows=None, num_rows=None, q=None, scale=None):
     """Rows in 8 bits: (q e4m3 [N, H], scale fp32 [N, ceil(H / 128)]), number = q * scale.
     x: bf16 or fp32 [*, H], or [*, 2 H] for ACT_SILU_MUL and ACT_GELU_TANH_MUL (act(left half) * right half; ACT_RELU2: max(x, 0)^2).
-    rows: int32 [N], the row of x for each row of the result, negative for zeros (src of moe_sort_padded); num_rows: int32 [1], rows from it on are
+    rows: int32 [N], the row of x for each row of the result, zeros where there is no such row (src of moe_sort_padded); num_rows: int32 [1], rows from it on are
     left as they are (offsets[E:] of moe_sort_padded).  q, scale: where to write."""
     dev = ctx.device
     dt = _DTYPE_CODE.get(x.dtype)
     if dt is None or x.get_device() != dev or x.dim() != 2:
         _refuse(ctx, ("x", x, _ROWS, None, False))
     N, H = x.shape
-    ldx = H
+    ldx, x_rows = H, N
     if not x.is_contiguous():
         ldx, one = x.stride()
         if one != 1 and H > 1:
@@ -991,7 +991,7 @@ def quant_fp8(ctx, x: torch.Tensor, act: int = ACT_NONE, rows=None, num_rows=Non
         scale = x.new_empty(N, lds, dtype=torch.float32) if scale is None else scale
         ldq, lds = _fp8_rows_given(ctx, q, scale, N, H)
     if N:
-        st = ctx.l.nvc_quant_fp8_rows(ctx.h, x.data_ptr(), dt, ldx, act, H, rows_at, num_at, q.data_ptr(), ldq, scale.data_ptr(), lds, N, H,
+        st = ctx.l.nvc_quant_fp8_rows(ctx.h, x.data_ptr(), dt, ldx, x_rows, act, H, rows_at, num_at, q.data_ptr(), ldq, scale.data_ptr(), lds, N, H,
                                       torch._C._cuda_getCurrentRawStream(dev))
         if st:
             check(st, "nvc_quant_fp8_rows", ctx.h)
@@ -1000,16 +1000,19 @@ def quant_fp8(ctx, x: torch.Tensor, act: int = ACT_NONE, rows=None, num_rows=Non
 
 def quant_fp8_weight(ctx, w: torch.Tensor):
     """A weight [N, K], or experts' weights [groups, N, K], bf16 or fp32, in 8 bits: (q, scale [(groups,) ceil(N / 128), ceil(K / 128)])."""
-    dt = _DTYPE_CODE.get(w.dtype)
-    if dt is None or w.get_device() != ctx.device or w.dim() not in (2, 3) or not w.is_contiguous():
+    dt, dims = _DTYPE_CODE.get(w.dtype), w.dim()
+    if dt is None or w.get_device() != ctx.device or dims not in (2, 3) or not w.is_contiguous():
         _refuse(ctx, ("w", w, _ROWS, None, True))
-    N, K = w.shape[-2:]
-    groups = w.shape[0] if w.dim() == 3 else 1
-    q = torch.empty(w.shape, dtype=FP8, device=w.device)
-    scale = torch.empty(*w.shape[:-2], (N + 127) // 128, (K + 127) // 128, dtype=torch.float32, device=w.device)
+    if dims == 2:
+        groups, (N, K) = 1, w.shape
+        q, scale = w.new_empty(N, K, dtype=FP8), w.new_empty((N + 127) // 128, (K + 127) // 128, dtype=torch.float32)
+    else:
+        groups, N, K = w.shape
+        q, scale = w.new_empty(groups, N, K, dtype=FP8), w.new_empty(groups, (N + 127) // 128, (K + 127) // 128, dtype=torch.float32)
     if groups:
-        check(ctx.l.nvc_quant_fp8_blocks(ctx.h, w.data_ptr(), dt, q.data_ptr(), scale.data_ptr(), groups, N, K, torch._C._cuda_getCurrentRawStream(ctx.device)),
-              "nvc_quant_fp8_blocks", ctx.h)
+        st = ctx.l.nvc_quant_fp8_blocks(ctx.h, w.data_ptr(), dt, q.data_ptr(), scale.data_ptr(), groups, N, K, torch._C._cuda_getCurrentRawStream(ctx.device))
+        if st:
+            check(st, "nvc_quant_fp8_blocks", ctx.h)
     return q, scale
 
 

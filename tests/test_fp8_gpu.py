@@ -145,17 +145,17 @@ def test_rows_of_zeros_tiny_and_not_numbers(ctx):
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_rows_gathered_and_limited(ctx, dtype):
-    """Rows taken by index, the same one twice, none for negative ones; rows behind the count stay as they were."""
+    """Rows taken by index, the same one twice, none for negative ones and for those beyond; rows behind the count stay as they were."""
     N, H = 40, 400
     x = _randn(3, N, H).to(dtype)
     rows = torch.randint(0, N, (64,), generator=_g(4), device=DEV, dtype=torch.int32)
-    rows[5], rows[17], rows[6] = -1, -7, rows[7]
+    rows[5], rows[17], rows[6], rows[30], rows[31] = -1, -7, rows[7], N, 2 ** 31 - 1        # none for those that x has not, either
     for used in (0, 1, 50, 64, 100):
         q = torch.full((64, H), 0x33, dtype=torch.uint8, device=DEV).view(E4M3)
         s = torch.full((64, 4), 7.0, device=DEV)
         count = torch.tensor([used], dtype=torch.int32, device=DEV)
         ops.quant_fp8(ctx, x, rows=rows, num_rows=count, q=q, scale=s)
-        f = torch.where(rows[:, None] < 0, torch.zeros((), device=DEV), x.float()[rows.clamp_min(0).long()])
+        f = torch.where((rows[:, None] < 0) | (rows[:, None] >= N), torch.zeros((), device=DEV), x.float()[rows.clamp(0, N - 1).long()])
         want = _scale32(f)
         wq = _bits((f * _spread(1.0 / want, H)).to(E4M3))
         n = min(used, 64)
@@ -385,14 +385,14 @@ def test_grouped_product(ctx, counts, N, K, out_dtype):
 
 def test_grouped_tiles_in_any_order(ctx):
     """Tiles of one expert apart, tiles without one in between."""
-    group = torch.tensor([2, -1, 0, 2, -1, 1, 0], dtype=torch.int32, device=DEV)
+    group = torch.tensor([2, -1, 0, 2, 3, 1, 0], dtype=torch.int32, device=DEV)          # there are three
     N, K = 400, 384
     q, s, wq, ws = _operands(9, 7 * 128, N, K, groups=3)
     got = ops.gemm_fp8_grouped(ctx, q, s, wq, ws, group, out_dtype=F32)
     a = _dequant(q, s)
     for t, e in enumerate(group.tolist()):
         rows = slice(128 * t, 128 * t + 128)
-        if e < 0:
+        if e < 0 or e > 2:
             assert torch.all(got[rows] == 0)
         else:
             _check_product(got[rows], a[rows], _dequant_w(wq[e], ws[e]))

@@ -13,7 +13,7 @@ def test_no_context_is_an_invalid_argument():
     l = _lib.lib()
     assert l.nvc_gemm_fp8(None, 16, 128, 16, 1, 16, 16, 16, 128, 0, 1, 128, 128, None) == -1
     assert l.nvc_gemm_fp8_grouped(None, 16, 128, 16, 1, 16, 16, 16, 128, 0, 128, 128, 128, 16, 1, 0, None) == -1
-    assert l.nvc_quant_fp8_rows(None, 16, 0, 128, 0, 0, None, None, 16, 128, 16, 1, 1, 128, None) == -1
+    assert l.nvc_quant_fp8_rows(None, 16, 0, 128, 1, 0, 0, None, None, 16, 128, 16, 1, 1, 128, None) == -1
     assert l.nvc_quant_fp8_blocks(None, 16, 0, 16, 16, 1, 128, 128, None) == -1
     assert l.nvc_add_rmsnorm_fp8(None, 16, 0, None, None, 16, 0, 1e-6, 16, 128, 16, 1, None, 1, 128, None) == -1
     assert l.nvc_last_error(None)
