@@ -3,10 +3,15 @@
 // The inner sums run on the tensor cores (e4m3 products are exact in fp32) in an accumulator of their own per k-block; the outer sums, whose factors differ
 // from block to block, in fp32 registers.
 //
-// A persistent grid, one CTA per SM, walks tiles of 128 x BN:
-//   warp 0     TMA producer: 128 x 128 bytes of A and BN x 128 of W per k-block into a ring that runs on into the next tile
-//   warp 1     tcgen05.mma M 128, N BN, K 32, four per k-block, into one of two (BN 256) or four accumulators in tensor memory
-//   warps 4-11 two per quadrant of tensor memory, one for either half of the columns: accumulator times scales onto registers, rows through shared memory and TMA
+// What bounds them: the tensor pipe takes 512 cycles for a k-block of 128 x 256, and the epilogue has to read and scale every k-block's sums in the same time.
+// 8 192 x 24 576 x 4 096 bf16: 660 to 680 us in short runs (2.4 PFLOP/s), 792 after seconds of them, which the power cap holds at 1.35 GHz; numbers of zero, which need
+// less power, 535 (3.1) and 595 at 1.77 GHz.  That is 790 to 805 cycles per k-block of a pair's 256 x 256.
+//
+// Three kernels, chosen by choose_route: gemm_fp8_kernel, gemm_fp8_pair_kernel for many tiles, gemm_fp8_split_kernel for few.  The first one, also that of the
+// experts' products, walks tiles of 128 x BN with a persistent grid, one CTA per SM:
+//   warp 0       TMA producer: 128 x 128 bytes of A and BN x 128 of W per k-block into a ring that runs on into the next tile
+//   warps 1, 2   tcgen05.mma M 128, N BN, K 32, four per k-block, every other k-block each, into one of two (BN 256) or four accumulators in tensor memory
+//   warps 4-11   two per quadrant of tensor memory, one for either half of the columns: accumulator times scales onto registers, rows through shared memory and TMA
 #include "fp8.cuh"
 #include "ptx_pair.cuh"
 #include "internal.h"
@@ -245,6 +250,13 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant
         ptx::mbar_init(acc_empty(i), 8);
       }
       ptx::fence_barrier_init();
+      if (!kGrouped) {                           // the first lap's weights in front of the launch wait
+        const int n0 = tile_at(blockIdx.x, a).y * BN;
+        for (int kb = 0; kb < min(a.num_kb, cfg::kStages); ++kb) {
+          ptx::mbar_arrive_expect_tx(full_bar(kb), cfg::kBytesB + a.a_box * BK);
+          ptx::tma_load_2d(base + kb * cfg::kStageBytes + cfg::kBytesA, &tma_b, full_bar(kb), kb * BK, n0);
+        }
+      }
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -274,10 +286,12 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant
       if (kGrouped && grp < 0) continue;
       for (int kb = 0; kb < a.num_kb; ++kb, ++it) {
         const int s = it % cfg::kStages;
-        wait_quietly(empty_bar(s), ((it / cfg::kStages) & 1) ^ 1u);      // first lap: falls through
-        ptx::mbar_arrive_expect_tx(full_bar(s), cfg::kBytesB + a.a_box * BK);        // rows of A behind the box hold what they held: their sums are never stored
         const uint32_t dst = base + s * cfg::kStageBytes;
-        ptx::tma_load_2d(dst + cfg::kBytesA, &tma_b, full_bar(s), kb * BK, grp * a.N + at.y * BN);
+        if (kGrouped || it >= (uint32_t)min(a.num_kb, cfg::kStages)) {
+          wait_quietly(empty_bar(s), ((it / cfg::kStages) & 1) ^ 1u);      // first lap: falls through
+          ptx::mbar_arrive_expect_tx(full_bar(s), cfg::kBytesB + a.a_box * BK);        // rows of A behind the box hold what they held: their sums are never stored
+          ptx::tma_load_2d(dst + cfg::kBytesA, &tma_b, full_bar(s), kb * BK, grp * a.N + at.y * BN);
+        }
         ptx::tma_load_2d(dst, &tma_a, full_bar(s), kb * BK, at.x * BM);
       }
     }
@@ -405,21 +419,32 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
   ptx::tcgen05_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(gen + cfg::kOffBar + cfg::kNumBars * 8);
   ptx::cluster_sync_all();                       // both CTAs' barriers exist before the other's copies and commits reach them
+  const uint32_t leader_full0 = ptx::mapa_u32(full_bar(0), 0);
+  auto load_w = [&](int s, int kb, int col) {
+    const uint32_t dst = base + s * cfg::kStageBytes + cfg::kBytesA;
+    if (h == 0) ptx::mbar_arrive_expect_tx(full_bar(s), 2 * cfg::kStageBytes);
+    tma_load_2d_pair(dst, &tma_b, leader_full0 + 8u * s, kb * BK, col * 256 + h * 64);
+    tma_load_2d_pair(dst + 64 * BK, &tma_b, leader_full0 + 8u * s, kb * BK, col * 256 + 128 + h * 64);
+  };
+  // the first lap's weights in front of the launch wait: behind a norm 256 x 12 288 x 4 096 27.7 -> 27.3 us, 200 x 12 288 x 1 024 11.7 -> 11.0; tiles of one CTA
+  // 64 x 24 576 x 4 096 26.7 -> 25.4, 128 x 6 144 x 2 560 12.7 -> 12.2
+  const int early = min(a.num_kb, cfg::kStages);
+  if (warp == 0 && ptx::elect_one())
+    for (int kb = 0; kb < early; ++kb) load_w(kb, kb, tile_at(cluster, a).y);
+  __syncwarp();
   pdl_wait();
   if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
   if (warp == 0 && ptx::elect_one()) {
-    const uint32_t leader_full0 = ptx::mapa_u32(full_bar(0), 0);
     uint32_t it = 0;
     for (int tile = cluster; tile < a.num_tiles; tile += clusters) {
       const int2 at = tile_at(tile, a);
       for (int kb = 0; kb < a.num_kb; ++kb, ++it) {
         const int s = it % cfg::kStages;
-        wait_quietly(empty_bar(s), ((it / cfg::kStages) & 1) ^ 1u);
-        if (h == 0) ptx::mbar_arrive_expect_tx(full_bar(s), 2 * cfg::kStageBytes);
-        const uint32_t dst = base + s * cfg::kStageBytes;
-        tma_load_2d_pair(dst, &tma_a, leader_full0 + 8u * s, kb * BK, at.x * 2 * BM + h * BM);
-        tma_load_2d_pair(dst + cfg::kBytesA, &tma_b, leader_full0 + 8u * s, kb * BK, at.y * 256 + h * 64);
-        tma_load_2d_pair(dst + cfg::kBytesA + 64 * BK, &tma_b, leader_full0 + 8u * s, kb * BK, at.y * 256 + 128 + h * 64);
+        if (it >= (uint32_t)early) {
+          wait_quietly(empty_bar(s), ((it / cfg::kStages) & 1) ^ 1u);
+          load_w(s, kb, at.y);
+        }
+        tma_load_2d_pair(base + s * cfg::kStageBytes, &tma_a, leader_full0 + 8u * s, kb * BK, at.x * 2 * BM + h * BM);
       }
     }
   } else if ((warp == 1 || warp == 2) && h == 0 && ptx::elect_one()) {
@@ -798,7 +823,7 @@ int nvc_gemm_fp8_check(nvc_ctx* ctx, const nvc_fp8* A, int lda, const float* a_s
               "row strides must cover the rows, A's be a multiple of 16 and C's of 8");
   NVC_REQUIRE(ctx, out_dtype == NVC_DT_BF16 || out_dtype == NVC_DT_F32, NVC_EINVAL, "bad out_dtype");
   NVC_REQUIRE(ctx, ((uintptr_t)A % 16) == 0 && ((uintptr_t)W % 16) == 0 && ((uintptr_t)C % 16) == 0, NVC_EINVAL, "pointers must be 16-byte aligned");
-  NVC_REQUIRE(ctx, (int64_t)Nout * groups <= 0x7fffffffLL && M <= 0x7fffffff - BM, NVC_ESHAPE, "too many rows");
+  NVC_REQUIRE(ctx, (int64_t)Nout * groups <= 0x7fffffffLL && M <= 0x7fffffff - 2 * BM, NVC_ESHAPE, "too many rows");
   NVC_REQUIRE(ctx, ctx->encode_tiled != nullptr, NVC_EDEVICE, "cuTensorMapEncodeTiled unavailable");
   return NVC_OK;
 }
@@ -883,6 +908,7 @@ extern "C" int nvc_gemm_fp8_ex(nvc_ctx* ctx, const nvc_fp8* A, int lda, const fl
                                int M, int Nout, int K, int force, void* stream) {
   int rc = nvc_gemm_fp8_check(ctx, A, lda, a_scale, lds, W, w_scale, C, ldc, out_dtype, M, Nout, K, 1);
   if (rc || M == 0) return rc;
+  NVC_REQUIRE(ctx, force == 0 || (force / 10 >= kFew16 && force / 10 <= kPair && force % 10 >= 1 && force % 10 <= 8), NVC_EINVAL, "bad route");
   DeviceGuard guard(ctx->device);
   const Args a = {a_scale, w_scale, nullptr, lds, out_dtype == NVC_DT_F32, M, Nout, (K + BK - 1) / BK, 0, 0, 0, 1, 0, 1, BM};
   const Call c = {A, lda, W, C, ldc, K, 1, nvc_stream(stream)};

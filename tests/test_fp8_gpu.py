@@ -548,3 +548,17 @@ def test_refusals(ctx):
             ops.gemm_fp8_grouped(ctx, *args)
     with pytest.raises(TypeError):
         ops.gemm_fp8_grouped(ctx, qg, sg, wg, wsg, tiles.long())
+
+
+def test_refusals_of_extents_and_routes(ctx):
+    """More rows than the last tile's row numbers have room for, and routes that do not exist: refused before anything is read."""
+    q, s, wq, ws = _operands(1, 8, 128, 256)
+    c = torch.empty(8, 128, dtype=BF16, device=DEV)
+    l, h = ctx.l, ctx.h
+
+    def product(M=8, route=0):
+        return l.nvc_gemm_fp8_ex(h, q.data_ptr(), 256, s.data_ptr(), 2, wq.data_ptr(), ws.data_ptr(), c.data_ptr(), 128, 0, M, 128, 256, route, 0)
+
+    assert [product(M=2**31 - 1 - d) for d in (0, 128, 255)] == [-2] * 3
+    assert [product(route=r) for r in (1, 10, 19, 40, 60, 71, -11)] == [-1] * 7
+    assert [product(route=r) for r in (0, 11, 28, 32, 41, 51, 61)] == [0] * 7
