@@ -379,7 +379,7 @@ bool dtype_ok(int dt) { return dt == NVC_DT_BF16 || dt == NVC_DT_F32; }
 
 extern "C" int nvc_quant_fp8_rows(nvc_ctx* ctx, const void* x, int x_dtype, int ldx, int x_rows, int act, int up_off, const int32_t* rows, const int32_t* num_rows, nvc_fp8* q,
                                   int ldq, float* scale, int lds, int N, int H, void* stream) {
-  NVC_REQUIRE(ctx, ctx && x && q && scale, NVC_EINVAL, "null pointer");
+  NVC_REQUIRE(ctx, ctx && (x || x_rows == 0) && q && scale, NVC_EINVAL, "null pointer");
   NVC_REQUIRE(ctx, N >= 0 && H > 0 && x_rows >= 0 && dtype_ok(x_dtype), NVC_EINVAL, "bad sizes or dtype");
   NVC_REQUIRE(ctx, rows || N <= x_rows, NVC_EINVAL, "more rows than x has");
   NVC_REQUIRE(ctx, act == NVC_ACT_NONE || act == NVC_ACT_RELU2 || act == NVC_ACT_GELU_TANH_MUL || act == NVC_ACT_SILU_MUL, NVC_EINVAL,

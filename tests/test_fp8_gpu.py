@@ -562,3 +562,14 @@ def test_refusals_of_extents_and_routes(ctx):
     assert [product(M=2**31 - 1 - d) for d in (0, 128, 255)] == [-2] * 3
     assert [product(route=r) for r in (1, 10, 19, 40, 60, 71, -11)] == [-1] * 7
     assert [product(route=r) for r in (0, 11, 28, 32, 41, 51, 61)] == [0] * 7
+
+
+def test_rows_of_nothing(ctx):
+    """A gather from no rows at all (a step without tokens): every row is one that does not exist."""
+    x = torch.empty(0, 256, dtype=BF16, device=DEV)
+    q, s = ops.quant_fp8(ctx, x, rows=torch.full((128,), -1, dtype=torch.int32, device=DEV))
+    assert q.shape == (128, 256) and not q.view(torch.uint8).any() and torch.equal(s, torch.full((128, 2), 2.0**-126, device=DEV))
+    q, s = ops.quant_fp8(ctx, x, act=ops.ACT_SILU_MUL, rows=torch.arange(3, dtype=torch.int32, device=DEV))
+    assert q.shape == (3, 128) and not q.view(torch.uint8).any() and torch.equal(s, torch.full((3, 1), 2.0**-126, device=DEV))
+    q, s = ops.quant_fp8(ctx, x)
+    assert q.shape == (0, 256) and s.shape == (0, 2)
