@@ -96,7 +96,7 @@ class SiluAndMul:
 
     def forward_fp8(self, x: torch.Tensor):
         """The same with rows in 8 bits: (q [rows, width / 2], scale)."""
-        return ops.quant_fp8(self.ctx, x.reshape(-1, x.shape[-1]), act=ops.ACT_SILU_MUL)
+        return ops.quant_fp8(self.ctx, x.reshape(-1, x.shape[-1]).contiguous(), act=ops.ACT_SILU_MUL)
 
 
 # ----------------------------------------------------------------------------- linear family

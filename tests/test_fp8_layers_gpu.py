@@ -73,3 +73,13 @@ def test_a_checkpoints_own_weights_and_refusals(ctx):
     with pytest.raises(ValueError):
         lin.forward(rows)
     assert lin.forward(x).shape == (5, 304)
+
+
+def test_gated_unit_of_any_layout(ctx):
+    """Rows that SiluAndMul.forward takes: a transposed view, rows at an odd distance, three dimensions."""
+    act = L.SiluAndMul(ctx)
+    base = torch.randn(256, 24, device="cuda").to(BF16)
+    for x in (base.t(), torch.randn(7, 261, device="cuda").to(BF16)[:, 3:259], torch.randn(2, 5, 256, device="cuda").to(BF16).transpose(0, 1)):
+        whole = x.reshape(-1, 256).contiguous()
+        want, got = ops.quant_fp8(ctx, whole, act=ops.ACT_SILU_MUL), act.forward_fp8(x)
+        assert all(torch.equal(_bits(a), _bits(b)) for a, b in zip(want, got))
