@@ -573,3 +573,30 @@ def test_rows_of_nothing(ctx):
     assert q.shape == (3, 128) and not q.view(torch.uint8).any() and torch.equal(s, torch.full((3, 1), 2.0**-126, device=DEV))
     q, s = ops.quant_fp8(ctx, x)
     assert q.shape == (0, 256) and s.shape == (0, 2)
+
+
+@pytest.mark.parametrize("route,M", [(11, 9), (14, 9), (21, 30), (24, 30), (31, 150), (32, 150), (41, 150), (51, 300), (61, 300)])
+def test_weights_converted_in_place_between_products(ctx, route, M):
+    """Products fetch weights ahead of their predecessors' end, and weights are converted into the place that the product in front still reads: no product sees another's."""
+    N, K, links = 784, 1296, 8
+    (q, s), l, h = ops.quant_fp8(ctx, _randn(40, M, K).to(BF16)), ctx.l, ctx.h
+    ws = [_randn(50 + i, N, K).to(BF16) for i in range(links)]
+    wq, wscale = ops.quant_fp8_weight(ctx, ws[0])
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def chain(wait):
+        outs = [torch.empty(M, N, dtype=BF16, device=DEV) for _ in ws]
+        torch.cuda.synchronize()
+        for w, c in zip(ws, outs):
+            for call in (lambda: l.nvc_quant_fp8_blocks(h, w.data_ptr(), 0, wq.data_ptr(), wscale.data_ptr(), 1, N, K, stream),
+                         lambda: l.nvc_gemm_fp8_ex(h, q.data_ptr(), K, s.data_ptr(), s.shape[1], wq.data_ptr(), wscale.data_ptr(), c.data_ptr(), N, 0, M, N, K, route, stream)):
+                assert call() == 0
+                if wait:
+                    torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        return outs
+
+    want = chain(True)
+    assert not torch.equal(want[0], want[1])
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(chain(False), want))
