@@ -723,7 +723,8 @@ int nvc_gemm_bf16_glu_clamp_mul(nvc_ctx* ctx, const nvc_bf16* A, int lda, const 
  * A number is kept as an e4m3 byte q and stands for q * scale, one fp32 scale for a block of 128 numbers along a row (a row's last block may be
  * shorter) or of 128 x 128 in a weight:  scale = max(amax / 448, 2^-126),  q = e4m3(x * (1 / scale)), to nearest even.  Where a block holds a NaN,
  * that number alone is NaN; where it holds an infinity, everything computed from it is.  Row widths are multiples of 16; pointers to numbers are
- * 16-byte aligned. */
+ * 16-byte aligned.  These calls have no static operands (launch order, above): weights, norm weights and scales are read behind the wait, and may come from
+ * any earlier work of the stream, kernels of this library included. */
 typedef uint8_t nvc_fp8;
 enum { NVC_FP8_BLOCK = 128 };
 /* q[i, :H], scale[i, :ceil(H / 128)] = the 8-bit form of f(x[r]), i < N:
@@ -740,10 +741,10 @@ int nvc_quant_fp8_rows(nvc_ctx* ctx, const void* x, int x_dtype, int ldx, int x_
 int nvc_add_rmsnorm_fp8(nvc_ctx* ctx, const void* x, int x_dtype, const float* residual_in, float* residual_out, const void* w, int w_dtype, float eps,
                         nvc_fp8* q, int ldq, float* scale, int lds, nvc_bf16* out, int N, int H, void* stream);
 /* Weights w [groups, N, K] (bf16 or fp32, contiguous) -> q [groups, N, K], scale [groups, ceil(N / 128), ceil(K / 128)]; blocks end with their group.
- * Starts when all earlier work of the stream is done and ends before later work starts: its results are static operands of the products behind it. */
+ * Signals no early start. */
 int nvc_quant_fp8_blocks(nvc_ctx* ctx, const void* w, int w_dtype, nvc_fp8* q, float* scale, int groups, int N, int K, void* stream);
 /* C[M, Nout] = sum over blocks b of K:  a_scale[m, b] * w_scale[n / 128, b] * sum over k in b of A[m, k] * W[n, k], bf16 or fp32.
- * A: 8-bit rows with scales [M, lds]; W [Nout, K] with scales [ceil(Nout / 128), ceil(K / 128)], both static.  K % 16 == 0, Nout % 16 == 0, lda % 16 == 0,
+ * A: 8-bit rows with scales [M, lds]; W [Nout, K] with scales [ceil(Nout / 128), ceil(K / 128)].  K % 16 == 0, Nout % 16 == 0, lda % 16 == 0,
  * ldc % 8 == 0. */
 int nvc_gemm_fp8(nvc_ctx* ctx, const nvc_fp8* A, int lda, const float* a_scale, int lds, const nvc_fp8* W, const float* w_scale, void* C, int ldc,
                  int out_dtype, int M, int Nout, int K, void* stream);

@@ -165,7 +165,7 @@ quant_rows_kernel(const T* x, int64_t ldx, int x_rows, int up_off, const int32_t
 // One CTA per row, which stays in registers between the sum of squares and the way out.
 template <typename T, typename W>
 __global__ void __launch_bounds__(1024)
-add_rmsnorm_fp8_kernel(const T* x, const float* res_in, float* res_out, const W* __restrict__ w, float eps, uint8_t* __restrict__ q, int64_t ldq,
+add_rmsnorm_fp8_kernel(const T* x, const float* res_in, float* res_out, const W* w, float eps, uint8_t* __restrict__ q, int64_t ldq,
                        float* __restrict__ scale, int64_t lds, nvc_bf16* __restrict__ out, int H) {
   __shared__ float part[32];
   pdl_trigger();
@@ -173,10 +173,10 @@ add_rmsnorm_fp8_kernel(const T* x, const float* res_in, float* res_out, const W*
   const int64_t r = blockIdx.x, at = r * H + col;
   const bool in = col < H;
   float g[16] = {}, y[16] = {};
-  if (in) load16(reinterpret_cast<const W*>(w) + col, g);      // never written by a kernel: in front of the wait
   pdl_wait();
   float ss = 0.f;
   if (in) {
+    load16(w + col, g);
     load16(x + at, y);
     if (res_in) {
       float a[16];
@@ -224,7 +224,7 @@ __device__ __forceinline__ float4 lds4<__nv_bfloat16>(const uint8_t* p) {
 
 template <typename T, typename W>
 __global__ void __launch_bounds__(1024)
-add_rmsnorm_fp8_ring_kernel(const T* x, const float* res_in, float* res_out, const W* __restrict__ w, float eps, uint8_t* __restrict__ q, int64_t ldq,
+add_rmsnorm_fp8_ring_kernel(const T* x, const float* res_in, float* res_out, const W* w, float eps, uint8_t* __restrict__ q, int64_t ldq,
                             float* __restrict__ scale, int64_t lds, nvc_bf16* __restrict__ out, int N, int H, int stages) {
   extern __shared__ __align__(16) uint8_t ring[];
   __shared__ float part[2][32];
@@ -242,6 +242,11 @@ add_rmsnorm_fp8_ring_kernel(const T* x, const float* res_in, float* res_out, con
     for (int s = 0; s < stages; ++s) ptx::mbar_init(bar0 + 8 * s, 1);
     ptx::fence_barrier_init();
   }
+  __syncthreads();
+  pdl_wait();
+  if (threadIdx.x == 0)
+    for (int s = 0; s < stages; ++s)
+      if ((int64_t)blockIdx.x + (int64_t)s * gridDim.x < N) fetch((int64_t)blockIdx.x + (int64_t)s * gridDim.x, s);
   float4 g[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -249,11 +254,6 @@ add_rmsnorm_fp8_ring_kernel(const T* x, const float* res_in, float* res_out, con
     g[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     if (col < H) g[i] = lds4<W>(reinterpret_cast<const uint8_t*>(w + col));
   }
-  __syncthreads();
-  pdl_wait();
-  if (threadIdx.x == 0)
-    for (int s = 0; s < stages; ++s)
-      if ((int64_t)blockIdx.x + (int64_t)s * gridDim.x < N) fetch((int64_t)blockIdx.x + (int64_t)s * gridDim.x, s);
   // this thread's first number of a row in every operand; its four blocks are 128 numbers apart
   const int col0 = warp * 512 + lane * 4;
   uint32_t in = 0;
@@ -325,8 +325,7 @@ add_rmsnorm_fp8_ring_kernel(const T* x, const float* res_in, float* res_out, con
 }
 
 // One CTA per block of 128 x 128: 32 rows at a time, eight threads each, four times; the numbers stay in registers, bf16 ones as they are (unpacked they took 87
-// registers, two CTAs per SM and 1.8 times as long).  The fence at the end keeps a CTA for a while, so four of them (three for fp32) share an SM: 24 576 x 4 096 bf16 68 us with
-// two, 54 with four, as without the fence.
+// registers, two CTAs per SM and 1.8 times as long).  Four CTAs (three for fp32) share an SM: 24 576 x 4 096 bf16 47.6 us.
 template <typename T, typename Held>
 __global__ void __launch_bounds__(256, (sizeof(T) == 2 ? 4 : 3))
 quant_blocks_kernel(const T* w, uint8_t* __restrict__ q, float* __restrict__ scale, int N, int K) {
@@ -362,7 +361,6 @@ quant_blocks_kernel(const T* w, uint8_t* __restrict__ q, float* __restrict__ sca
     }
   }
   if (threadIdx.x == 0) scale[((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x] = s;
-  __threadfence();                               // a product may fetch weights as soon as the last CTA has ended
 }
 
 template <typename T, bool kFlat>
@@ -454,7 +452,6 @@ extern "C" int nvc_fp8_rows_init(nvc_ctx* ctx) {
   return NVC_OK;
 }
 
-// No early start for the kernel behind it: its results are weights, which the products read ahead of their wait.
 extern "C" int nvc_quant_fp8_blocks(nvc_ctx* ctx, const void* w, int w_dtype, nvc_fp8* q, float* scale, int groups, int N, int K, void* stream) {
   NVC_REQUIRE(ctx, ctx && w && q && scale, NVC_EINVAL, "null pointer");
   NVC_REQUIRE(ctx, groups >= 0 && N > 0 && K > 0 && dtype_ok(w_dtype), NVC_EINVAL, "bad sizes or dtype");

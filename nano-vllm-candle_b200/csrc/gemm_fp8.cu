@@ -190,6 +190,13 @@ __device__ __forceinline__ void store_sums(const CUtensorMap* tma_c, uint32_t bu
   }
 }
 
+// In front of the launch wait: the ring's first lap of weights into L2, where a later write still finds them.  They are read behind the wait, whoever wrote them: a kernel that does
+// not signal its dependents early lets them start when its last CTA has ended, which orders nothing that it wrote.  Behind a norm, read ahead / asked for ahead / neither, us:
+// 64 x 24 576 x 4 096 25.2 / 25.5 / 26.7, 200 x 12 288 x 1 024 10.9 / 11.1 / 11.7, 8 x 4 096 x 4 096 8.3 / 9.0; two laps and more 0.1 to 2 us longer.
+__device__ __forceinline__ void ask_for_weights(const CUtensorMap* w, int kb0, int n, int row) {
+  for (int kb = kb0; kb < kb0 + n; ++kb) ptx::tma_prefetch_l2_2d(w, kb * BK, row);
+}
+
 template <int BN>
 struct Cfg {
   static constexpr int kBytesA = BM * BK, kBytesB = BN * BK, kStageBytes = kBytesA + kBytesB;
@@ -250,13 +257,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant
         ptx::mbar_init(acc_empty(i), 8);
       }
       ptx::fence_barrier_init();
-      if (!kGrouped) {                           // the first lap's weights in front of the launch wait
-        const int n0 = tile_at(blockIdx.x, a).y * BN;
-        for (int kb = 0; kb < min(a.num_kb, cfg::kStages); ++kb) {
-          ptx::mbar_arrive_expect_tx(full_bar(kb), cfg::kBytesB + a.a_box * BK);
-          ptx::tma_load_2d(base + kb * cfg::kStageBytes + cfg::kBytesA, &tma_b, full_bar(kb), kb * BK, n0);
-        }
-      }
+      if (!kGrouped) ask_for_weights(&tma_b, 0, min(a.num_kb, cfg::kStages), tile_at(blockIdx.x, a).y * BN);
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -287,11 +288,9 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant
       for (int kb = 0; kb < a.num_kb; ++kb, ++it) {
         const int s = it % cfg::kStages;
         const uint32_t dst = base + s * cfg::kStageBytes;
-        if (kGrouped || it >= (uint32_t)min(a.num_kb, cfg::kStages)) {
-          wait_quietly(empty_bar(s), ((it / cfg::kStages) & 1) ^ 1u);      // first lap: falls through
-          ptx::mbar_arrive_expect_tx(full_bar(s), cfg::kBytesB + a.a_box * BK);        // rows of A behind the box hold what they held: their sums are never stored
-          ptx::tma_load_2d(dst + cfg::kBytesA, &tma_b, full_bar(s), kb * BK, grp * a.N + at.y * BN);
-        }
+        wait_quietly(empty_bar(s), ((it / cfg::kStages) & 1) ^ 1u);        // first lap: falls through
+        ptx::mbar_arrive_expect_tx(full_bar(s), cfg::kBytesB + a.a_box * BK);          // rows of A behind the box hold what they held: their sums are never stored
+        ptx::tma_load_2d(dst + cfg::kBytesA, &tma_b, full_bar(s), kb * BK, grp * a.N + at.y * BN);
         ptx::tma_load_2d(dst, &tma_a, full_bar(s), kb * BK, at.x * BM);
       }
     }
@@ -420,17 +419,11 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(gen + cfg::kOffBar + cfg::kNumBars * 8);
   ptx::cluster_sync_all();                       // both CTAs' barriers exist before the other's copies and commits reach them
   const uint32_t leader_full0 = ptx::mapa_u32(full_bar(0), 0);
-  auto load_w = [&](int s, int kb, int col) {
-    const uint32_t dst = base + s * cfg::kStageBytes + cfg::kBytesA;
-    if (h == 0) ptx::mbar_arrive_expect_tx(full_bar(s), 2 * cfg::kStageBytes);
-    tma_load_2d_pair(dst, &tma_b, leader_full0 + 8u * s, kb * BK, col * 256 + h * 64);
-    tma_load_2d_pair(dst + 64 * BK, &tma_b, leader_full0 + 8u * s, kb * BK, col * 256 + 128 + h * 64);
-  };
-  // the first lap's weights in front of the launch wait: behind a norm 256 x 12 288 x 4 096 27.7 -> 27.3 us, 200 x 12 288 x 1 024 11.7 -> 11.0; tiles of one CTA
-  // 64 x 24 576 x 4 096 26.7 -> 25.4, 128 x 6 144 x 2 560 12.7 -> 12.2
-  const int early = min(a.num_kb, cfg::kStages);
-  if (warp == 0 && ptx::elect_one())
-    for (int kb = 0; kb < early; ++kb) load_w(kb, kb, tile_at(cluster, a).y);
+  if (warp == 0 && ptx::elect_one()) {
+    const int n0 = tile_at(cluster, a).y * 256 + h * 64, n = min(a.num_kb, cfg::kStages);
+    ask_for_weights(&tma_b, 0, n, n0);
+    ask_for_weights(&tma_b, 0, n, n0 + 128);
+  }
   __syncwarp();
   pdl_wait();
   if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
@@ -440,11 +433,12 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
       const int2 at = tile_at(tile, a);
       for (int kb = 0; kb < a.num_kb; ++kb, ++it) {
         const int s = it % cfg::kStages;
-        if (it >= (uint32_t)early) {
-          wait_quietly(empty_bar(s), ((it / cfg::kStages) & 1) ^ 1u);
-          load_w(s, kb, at.y);
-        }
-        tma_load_2d_pair(base + s * cfg::kStageBytes, &tma_a, leader_full0 + 8u * s, kb * BK, at.x * 2 * BM + h * BM);
+        const uint32_t dst = base + s * cfg::kStageBytes;
+        wait_quietly(empty_bar(s), ((it / cfg::kStages) & 1) ^ 1u);
+        if (h == 0) ptx::mbar_arrive_expect_tx(full_bar(s), 2 * cfg::kStageBytes);
+        tma_load_2d_pair(dst + cfg::kBytesA, &tma_b, leader_full0 + 8u * s, kb * BK, at.y * 256 + h * 64);
+        tma_load_2d_pair(dst + cfg::kBytesA + 64 * BK, &tma_b, leader_full0 + 8u * s, kb * BK, at.y * 256 + 128 + h * 64);
+        tma_load_2d_pair(dst, &tma_a, leader_full0 + 8u * s, kb * BK, at.x * 2 * BM + h * BM);
       }
     }
   } else if ((warp == 1 || warp == 2) && h == 0 && ptx::elect_one()) {
@@ -499,11 +493,11 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
 
 // Few tiles: a cluster of S CTAs shares the k-blocks of one.  Every CTA parks its sums in its idle ring, row by row of A, 128 columns each, and adds up its share of the
 // rows over the cluster, in the order of the ranks.
-//   warp 0         TMA: 128 rows of W and up to NT of A per k-block; W's first lap in front of the launch wait
+//   warp 0         TMA: 128 rows of W and up to NT of A per k-block
 //   warp 1 (and 2) tcgen05.mma; the other warps sums
 // NT 16, 32 (few rows): the operands change places - 128 rows of W are the rows of the product, the rows of A its columns, so that no part of the tensor pipe's and the
 // epilogue's work is done for rows that do not exist.  A thread has a row of W and every row of A; the scales' products lie in a table, filled 32 k-blocks at a time.  The ring
-// is half an SM's shared memory: two CTAs share an SM, and the next product's weights come while this one ends.
+// is half an SM's shared memory: two CTAs share an SM, and the next product starts while this one ends.
 // NT 128: 128 rows of A and 128 columns; a thread has one row, and one scale for all its columns (with the operands changed, reading 64 scales per k-block from
 // shared memory took 1 200 cycles, this 600).
 template <int NT>
@@ -560,10 +554,7 @@ gemm_fp8_split_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
         ptx::mbar_init(acc_empty(i), 4 * cfg::kSides);
       }
       ptx::fence_barrier_init();
-      for (int kb = 0; kb < min(num_kb, cfg::kStages); ++kb) {
-        ptx::mbar_arrive_expect_tx(full_bar(kb), stage_tx);
-        ptx::tma_load_2d(base + kb * cfg::kStageBytes, &tma_w, full_bar(kb), (kb0 + kb) * BK, n0);
-      }
+      ask_for_weights(&tma_w, kb0, min(num_kb, cfg::kStages), n0);
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -579,11 +570,9 @@ gemm_fp8_split_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_co
     for (int kb = 0; kb < num_kb; ++kb) {
       const int s = kb % cfg::kStages;
       const uint32_t dst = base + s * cfg::kStageBytes;
-      if (kb >= cfg::kStages) {
-        wait_quietly(empty_bar(s), ((kb / cfg::kStages) & 1) ^ 1u);
-        ptx::mbar_arrive_expect_tx(full_bar(s), stage_tx);
-        ptx::tma_load_2d(dst, &tma_w, full_bar(s), (kb0 + kb) * BK, n0);
-      }
+      wait_quietly(empty_bar(s), ((kb / cfg::kStages) & 1) ^ 1u);
+      ptx::mbar_arrive_expect_tx(full_bar(s), stage_tx);
+      ptx::tma_load_2d(dst, &tma_w, full_bar(s), (kb0 + kb) * BK, n0);
       ptx::tma_load_2d(dst + cfg::kBytesW, &tma_a, full_bar(s), (kb0 + kb) * BK, m0);
     }
   } else if (warp >= 1 && warp <= cfg::kIssuers && ptx::elect_one()) {

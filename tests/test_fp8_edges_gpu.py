@@ -1,0 +1,75 @@
+"""Rows and weights in 8 bits where it is easy to go wrong: units far from one, numbers that are none, tiles behind the first.
+
+Tolerances come from the roundings in between, each at most 2^-24 of the value in fp32 (the hardware's exponential 2^-22, its reciprocal 2^-23)."""
+import importlib
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+ops = importlib.import_module("nano-vllm-candle_b200.ops")
+BF16, F32, F64, E4M3 = torch.bfloat16, torch.float32, torch.float64, torch.float8_e4m3fn
+DEV = "cuda:0"
+LEAST = 2.0 ** -126
+
+
+def _bits(t):
+    return t.view(torch.uint8) if t.dtype == E4M3 else t
+
+
+def _g(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+# ----------------------------------------------------------------------------- what a call reads, whoever wrote it
+@pytest.mark.parametrize("route,M", [(11, 9), (14, 9), (21, 30), (24, 30), (31, 150), (32, 150), (41, 150), (51, 300), (61, 300)])
+@pytest.mark.parametrize("writer", ["copy", "rows"])
+def test_weights_written_in_front_of_their_product(ctx, route, M, writer):
+    """Weights and scales written over by a kernel that is none of the library's, or by one that lets its followers start early, directly in front of the product that reads them."""
+    N, K, links, l, h = 784, 1296, 8, ctx.l, ctx.h
+    kb, nb = (K + 127) // 128, (N + 127) // 128
+    q, s = ops.quant_fp8(ctx, torch.randn(M, K, generator=_g(1), device=DEV))
+    full = [torch.randn(N, K, generator=_g(2 + i), device=DEV).to(BF16) for i in range(links)]
+    new_q = [ops.quant_fp8(ctx, w)[0].view(torch.uint8) for w in full]
+    new_s = [torch.rand(nb, kb, generator=_g(50 + i), device=DEV) + 0.5 for i in range(links)]
+    wq, ws, beside = new_q[0].clone(), new_s[0].clone(), torch.empty(N, kb, device=DEV)
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def chain(wait):
+        outs = [torch.empty(M, N, dtype=BF16, device=DEV) for _ in full]
+        torch.cuda.synchronize()
+        for i, c in enumerate(outs):
+            ws.copy_(new_s[i])
+            if writer == "copy":
+                wq.copy_(new_q[i])
+            else:
+                assert l.nvc_quant_fp8_rows(h, full[i].data_ptr(), 0, K, N, ops.ACT_NONE, 0, None, None, wq.data_ptr(), K, beside.data_ptr(), kb, N, K, stream) == 0
+            if wait:
+                torch.cuda.synchronize()
+            assert l.nvc_gemm_fp8_ex(h, q.data_ptr(), K, s.data_ptr(), kb, wq.data_ptr(), ws.data_ptr(), c.data_ptr(), N, 0, M, N, K, route, stream) == 0
+            if wait:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        return outs
+
+    want = chain(True)
+    assert not torch.equal(want[0], want[1])
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(chain(False), want))
+
+
+@pytest.mark.parametrize("N,H", [(3, 2048), (1200, 1024)])
+def test_norm_weights_written_in_front_of_their_norm(ctx, N, H):
+    x = torch.randn(N, H, generator=_g(1), device=DEV).to(BF16)
+    new = [torch.randn(H, generator=_g(2 + i), device=DEV).to(BF16) for i in range(12)]
+    w = new[0].clone()
+    want = []
+    for n in new:
+        want.append(ops.add_rmsnorm_fp8(ctx, x, n, 1e-6)[:2])
+    torch.cuda.synchronize()
+    got = []
+    for n in new:
+        w.copy_(n)
+        got.append(ops.add_rmsnorm_fp8(ctx, x, w, 1e-6)[:2])
+    for (q, s), (q0, s0) in zip(got, want):
+        assert torch.equal(_bits(q), _bits(q0)) and torch.equal(s, s0)
