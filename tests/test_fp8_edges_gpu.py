@@ -73,3 +73,36 @@ def test_norm_weights_written_in_front_of_their_norm(ctx, N, H):
         got.append(ops.add_rmsnorm_fp8(ctx, x, w, 1e-6)[:2])
     for (q, s), (q0, s0) in zip(got, want):
         assert torch.equal(_bits(q), _bits(q0)) and torch.equal(s, s0)
+
+
+# ----------------------------------------------------------------------------- gated units, one number to a block
+def _one_to_a_block(ctx, gate, up, act):
+    """gate, up [n] fp32 -> what the scale of a block with nothing else in it says the unit gave, and the sign of its number."""
+    n = gate.numel()
+    x = torch.zeros(n, 256, device=DEV)
+    x[:, 5], x[:, 128 + 5] = gate, up
+    q, s = ops.quant_fp8(ctx, x, act=act)
+    got = q.to(F64)
+    assert torch.all(got[:, :5] == 0) and torch.all(got[:, 6:] == 0)
+    return s.to(F64)[:, 0] * 448, torch.sign(got[:, 5])
+
+
+def _unit64(gate, act):
+    z = gate.to(F64)
+    w = z if act == ops.ACT_SILU_MUL else z * (2 * 0.7978845608028654) * (1 + 0.044715 * z * z)
+    return w, z * torch.sigmoid(w)
+
+
+@pytest.mark.parametrize("act", [ops.ACT_SILU_MUL, ops.ACT_GELU_TANH_MUL])
+def test_tiny_gates_keep_their_digits(ctx, act):
+    """Gates down to the least normal numbers, with an up value that brings their product back: ten roundings of 2^-24 at most, and two of the scale."""
+    gate = torch.tensor([1e-28, 1e-30, 1e-33, 1e-34, 1e-35, 1e-36, 1e-37, 2.4e-38], device=DEV)
+    gate = torch.cat([gate, -gate, gate.to(BF16).float()])
+    for up in (1.0, 1e10, -1e30):
+        u = torch.full_like(gate, up)
+        _, y = _unit64(gate, act)
+        want = y * u.to(F64)
+        keep = want.abs() >= 448 * 2 * LEAST          # else the scale is the least one
+        got, sign = _one_to_a_block(ctx, gate, u, act)
+        assert torch.all(((got - want.abs()).abs() <= (2.0 ** -20 + 2.0 ** -22) * want.abs())[keep]), (got / want.abs()).tolist()
+        assert torch.all((sign == torch.sign(want))[keep])
