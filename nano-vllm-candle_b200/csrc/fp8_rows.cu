@@ -35,21 +35,23 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 }
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
-// z sigmoid(w) = z c / (c (1 + exp(-w))), where w < 0 wherever z is far below 0: exp(-w) = 2^h (1 + r) / c, r = -w - (h - log2 c) ln 2 with the constant in two parts.  c = 2^-32 for
-// w <= -1, so that neither the hardware's exponential nor its reciprocal, which know no denormals here, leave the normal numbers where the result has not; there z is no small
+// z sigmoid(w) = z c / (c (1 + exp(-w))), where w < 0 wherever z is far below 0: exp(-w) = 2^d exp(r), after Cody and Waite: d the multiple of 2^-11 next to -w / ln 2,
+// r = -w - d ln 2 with ln 2 in two parts (to fp32, and the rest), exp(r) = 1 + r as |r| < 2^-12.4.  d and d + log2 c are exact, so the exponential has the hardware's 2^-22, at any w;
+// with it the reciprocal's 2^-23, r^2 / 2 < 2^-25.8 and four roundings: below 2^-20.
+// c = 2^-32 for w <= -1, so that neither the hardware's exponential nor its reciprocal, which know no denormals here, leave the normal numbers where the result has not; there z is no small
 // number, and z c has all its digits.  c = 1 elsewhere, where z may be as small or large as a number can be, and the sigmoid is a quarter or more.  w is held where the result is
 // z or 0 (an infinite z stays one).
 // These units bound their passes: 34 instructions for a number, with exponential and reciprocal for denormals and one number at a time, took 119 us for 8 191 x 12 288
-// gated rows, these 91 (without a choice of c 86, but there 1e-36 had no digits left).
+// gated rows, these 91 (gelu 98; without a choice of c 86, but there 1e-36 had no digits left).
 __device__ __forceinline__ float2 times_sigmoid(float2 z, float2 w) {
   const float2 v = make_float2(fminf(fmaxf(w.x, -120.0f), 88.0f), fminf(fmaxf(w.y, -120.0f), 88.0f));
   float2 near;                                   // 0 for w <= -1, else 1: no number lies between -1 and -1 + 2^-40
   asm("fma.rn.sat.f32 %0, %1, 0f53800000, 0f53800000;" : "=f"(near.x) : "f"(v.x));
   asm("fma.rn.sat.f32 %0, %1, 0f53800000, 0f53800000;" : "=f"(near.y) : "f"(v.y));
   const float2 c = add2(near, both(2.32830644e-10f)), shift = fma2(near, both(32.0f), both(-32.0f));
-  const float2 h = fma2(v, both(-1.44269502f), shift), d = fma2(shift, both(-1.0f), h);
+  const float2 d = add2(fma2(v, both(-1.44269502f), both(6144.0f)), both(-6144.0f)), h = add2(d, shift);          // a number from 4 096 on has whole multiples of 2^-11
   const float2 n = make_float2(-v.x, -v.y);
-  const float2 r = fma2(d, both(-1.42860677e-6f), fma2(d, both(-0.693145752f), n));
+  const float2 r = fma2(d, both(1.90465421e-9f), fma2(d, both(-0.693147182f), n));
   float2 e, q;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(h.x));
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(h.y));

@@ -106,3 +106,21 @@ def test_tiny_gates_keep_their_digits(ctx, act):
         got, sign = _one_to_a_block(ctx, gate, u, act)
         assert torch.all(((got - want.abs()).abs() <= (2.0 ** -20 + 2.0 ** -22) * want.abs())[keep]), (got / want.abs()).tolist()
         assert torch.all((sign == torch.sign(want))[keep])
+
+
+@pytest.mark.parametrize("act", [ops.ACT_SILU_MUL, ops.ACT_GELU_TANH_MUL])
+def test_gates_far_below_zero_keep_their_digits(ctx, act):
+    """A single gate to a block, down to where the sigmoid leaves fp32.  silu: the exponential 2^-22, the reciprocal 2^-23, a second order of 2^-26 and five roundings, below
+    2^-20.  gelu: its exponent is computed, four roundings of 2^-24 of itself, which the part of the sigmoid that falls carries."""
+    most = 102.0 if act == ops.ACT_SILU_MUL else 10.4
+    gate = torch.linspace(-most, 12.0, 20011, device=DEV)
+    w, y = _unit64(gate, act)
+    up = torch.exp2(torch.floor(-torch.log2(y.abs().clamp_min(2.0 ** -148)))).clamp(2.0 ** -20, 2.0 ** 120).float()
+    want = (y * up.to(F64)).abs()
+    got, sign = _one_to_a_block(ctx, gate, up, act)
+    rel = 2.0 ** -20 + (0 if act == ops.ACT_SILU_MUL else 2.0 ** -22) * w.abs() * torch.sigmoid(-w)
+    tol = (rel + 2.0 ** -22) * want + 2.0 ** -149 * up.to(F64) + 448 * LEAST          # the gate itself may be a denormal number
+    err = (got - want).abs()
+    worst = int((err / tol).argmax())
+    assert torch.all(err <= tol), (float(gate[worst]), float(got[worst]), float(want[worst]), float((err / tol)[worst]))
+    assert torch.all((sign == torch.sign(y))[want > 2.0 ** -100])
