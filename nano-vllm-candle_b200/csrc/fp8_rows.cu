@@ -308,8 +308,8 @@ add_rmsnorm_fp8_ring_kernel(const T* x, const float* res_in, float* res_out, con
     for (int i = 0; i < 4; ++i) {
       const float2 lo = mul2(mul2(make_float2(y[i].x, y[i].y), both(rstd)), make_float2(g[i].x, g[i].y)), hi = mul2(mul2(make_float2(y[i].z, y[i].w), both(rstd)), make_float2(g[i].z, g[i].w));
       y[i] = make_float4(lo.x, lo.y, hi.x, hi.y);
-      // magnitudes' bits are in the order of the magnitudes
-      const float m = fmaxf(fmaxf(fabsf(y[i].x), fabsf(y[i].y)), fmaxf(fabsf(y[i].z), fabsf(y[i].w)));
+      // magnitudes' bits are in the order of the magnitudes; four NaN are none
+      const float m = fmaxf(fmaxf(fmaxf(fabsf(y[i].x), fabsf(y[i].y)), fmaxf(fabsf(y[i].z), fabsf(y[i].w))), 0.f);
       const uint32_t all = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
       if ((lane & 3) == i) top = __uint_as_float(all);
     }

@@ -124,3 +124,22 @@ def test_gates_far_below_zero_keep_their_digits(ctx, act):
     worst = int((err / tol).argmax())
     assert torch.all(err <= tol), (float(gate[worst]), float(got[worst]), float(want[worst]), float((err / tol)[worst]))
     assert torch.all((sign == torch.sign(y))[want > 2.0 ** -100])
+
+
+# ----------------------------------------------------------------------------- numbers that are none
+@pytest.mark.parametrize("N,H", [(4, 1024), (2100, 256), (1000, 1040), (600, 4096)])
+@pytest.mark.parametrize("where", [(8,), (8, 9, 10, 11), (6, 7, 8, 9, 10, 11, 12, 13), tuple(range(128))])
+def test_a_norm_keeps_a_nan_to_itself(ctx, N, H, where):
+    """Weights that are no numbers, alone, four neighbouring ones and a whole block: every other number has the bits that it has where they count for nothing."""
+    x = torch.randn(N, H, generator=_g(N + H), device=DEV).to(BF16)
+    w = 1 + 0.2 * torch.randn(H, generator=_g(7), device=DEV)
+    at = torch.tensor(where, device=DEV) + 128
+    nan, zero = w.clone(), w.clone()
+    nan[at], zero[at] = float("nan"), 0.0
+    q, s, out = ops.add_rmsnorm_fp8(ctx, x, nan, 1e-6, want_out=True)
+    q0, s0, out0 = ops.add_rmsnorm_fp8(ctx, x, zero, 1e-6, want_out=True)
+    assert torch.equal(s, s0)
+    assert torch.all(torch.isnan(q.float()[:, at])) and torch.all(torch.isnan(out[:, at]))
+    rest = torch.ones(H, dtype=torch.bool, device=DEV)
+    rest[at] = False
+    assert torch.equal(_bits(q)[:, rest], _bits(q0)[:, rest]) and torch.equal(out[:, rest], out0[:, rest])
