@@ -149,7 +149,7 @@ quant_rows_kernel(const T* x, int64_t ldx, int x_rows, int up_off, const int32_t
       } else if (kAct == NVC_ACT_RELU2) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const float v = fmaxf(y[i], 0.f);
+          const float v = y[i] < 0.f ? 0.f : y[i];           // a NaN stays one
           y[i] = v * v;
         }
       }

@@ -143,3 +143,19 @@ def test_a_norm_keeps_a_nan_to_itself(ctx, N, H, where):
     rest = torch.ones(H, dtype=torch.bool, device=DEV)
     rest[at] = False
     assert torch.equal(_bits(q)[:, rest], _bits(q0)[:, rest]) and torch.equal(out[:, rest], out0[:, rest])
+
+
+@pytest.mark.parametrize("act", [ops.ACT_NONE, ops.ACT_RELU2, ops.ACT_SILU_MUL, ops.ACT_GELU_TANH_MUL])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_units_keep_a_nan(ctx, act, dtype):
+    """A NaN stays one through every unit, from either half of a gated one, and counts for no scale."""
+    gated = act in (ops.ACT_SILU_MUL, ops.ACT_GELU_TANH_MUL)
+    x = torch.randn(9, 512 if gated else 256, generator=_g(5), device=DEV).abs().to(dtype)
+    q0, s0 = ops.quant_fp8(ctx, torch.where(torch.arange(x.shape[1], device=DEV) % 256 == 40, torch.zeros((), dtype=dtype, device=DEV), x), act=act)
+    for col in (40, 256 + 40) if gated else (40,):
+        y = x.clone()
+        y[:, col] = float("nan")
+        q, s = ops.quant_fp8(ctx, y, act=act)
+        assert torch.all(torch.isnan(q.float()[:, 40])), col
+        assert torch.equal(s, s0)
+        assert torch.equal(_bits(q)[:, :40], _bits(q0)[:, :40]) and torch.equal(_bits(q)[:, 41:], _bits(q0)[:, 41:])
