@@ -952,7 +952,7 @@ def _fp8_rows_given(ctx, q, scale, n: int, width: int):
         _refuse(ctx, ("q", q, _E4M3, (n, width), False))
     if scale.get_device() != ctx.device or scale.dtype is not torch.float32 or scale.shape != (n, blocks) or (blocks > 1 and scale.stride(1) != 1):
         _refuse(ctx, ("scale", scale, _F32, (n, blocks), False))
-    return q.stride(0), scale.stride(0)
+    return (q.stride(0), scale.stride(0)) if n > 1 else (width, blocks)          # a single row's distance to the next says nothing
 
 
 def quant_fp8(ctx, x: torch.Tensor, act: int = ACT_NONE, rows=None, num_rows=None, q=None, scale=None):
@@ -1077,7 +1077,7 @@ def _fp8_product(ctx, q, scale, wq, wscale, out, out_dtype, groups):
     else:
         code = _DTYPE_CODE.get(out.dtype)
         if good and code is not None and out.get_device() == dev and out.shape == (M, N) and out.stride(1) == 1:
-            return M, N, K, ldq, lds, out, out.stride(0), code
+            return M, N, K, ldq, lds, out, out.stride(0) if M > 1 else N, code
     _refuse(ctx, ("q", q, _E4M3, (M, K), False), ("scale", scale, _F32, (M, blocks), False), ("wq", wq, _E4M3, (*ws[:0 if groups is None else 1], N, K), True),
             ("wscale", wscale, _F32, wblocks, True), ("out", out, _ROWS, (M, N), False))
 

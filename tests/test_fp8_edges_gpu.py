@@ -159,3 +159,20 @@ def test_units_keep_a_nan(ctx, act, dtype):
         assert torch.all(torch.isnan(q.float()[:, 40])), col
         assert torch.equal(s, s0)
         assert torch.equal(_bits(q)[:, :40], _bits(q0)[:, :40]) and torch.equal(_bits(q)[:, 41:], _bits(q0)[:, 41:])
+
+
+# ----------------------------------------------------------------------------- strides that are never used, sizes that pass 31 bits
+def test_one_row_of_any_stride(ctx):
+    """A single row's distance to the next one says nothing: a column seen as a row is as good as any."""
+    x, w = torch.randn(1, 256, generator=_g(1), device=DEV), torch.ones(256, device=DEV)
+    wq, ws = ops.quant_fp8_weight(ctx, torch.randn(160, 256, generator=_g(2), device=DEV))
+    q = torch.empty(256, 1, dtype=torch.uint8, device=DEV).view(E4M3).t()
+    s, c = torch.empty(2, 1, device=DEV).t(), torch.empty(160, 1, device=DEV).t()
+    assert q.stride() == (1, 1) and s.stride() == (1, 1) and c.stride() == (1, 1)
+    want = ops.quant_fp8(ctx, x)
+    ops.quant_fp8(ctx, x, q=q, scale=s)
+    assert torch.equal(_bits(q), _bits(want[0])) and torch.equal(s, want[1])
+    assert torch.equal(ops.gemm_fp8(ctx, q, s, wq, ws, out=c), ops.gemm_fp8(ctx, *want, wq, ws, out_dtype=F32))
+    want = ops.add_rmsnorm_fp8(ctx, x, w, 1e-6)
+    ops.add_rmsnorm_fp8(ctx, x, w, 1e-6, q=q, scale=s)
+    assert torch.equal(_bits(q), _bits(want[0])) and torch.equal(s, want[1])

@@ -1,0 +1,39 @@
+"""What the 8-bit entry points and layers decide before they reach a device, with a library that only notes its calls."""
+import importlib
+import types
+
+import pytest
+import torch
+
+ops = importlib.import_module("nano-vllm-candle_b200.ops")
+E4M3 = torch.float8_e4m3fn
+
+
+class _Calls(list):
+    def __getattr__(self, name):
+        def call(*args):
+            self.append((name, args))
+            return 0
+        return call
+
+
+@pytest.fixture
+def fake(monkeypatch):
+    """A context on no device: its tensors have memory or none ("meta"), its library notes calls."""
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: 0, raising=False)
+    return types.SimpleNamespace(device=-1, h=0, l=_Calls(), tp_size=1, tp_rank=0)
+
+
+def _meta(*shape, dtype=torch.bfloat16):
+    return torch.empty(*shape, dtype=dtype, device="meta")
+
+
+def test_one_row_has_its_own_width_as_distance(fake):
+    """A column seen as a row: what its stride says is not handed on."""
+    x, q, s, c = torch.zeros(1, 256), torch.zeros(256, 1, dtype=torch.uint8).view(E4M3).t(), torch.zeros(2, 1).t(), torch.zeros(160, 1).t()
+    assert q.stride() == (1, 1) and s.stride() == (1, 1) and c.stride() == (1, 1)
+    ops.quant_fp8(fake, x, q=q, scale=s)
+    ops.add_rmsnorm_fp8(fake, x, torch.ones(256), 1e-6, q=q, scale=s)
+    ops.gemm_fp8(fake, q, s, torch.zeros(160, 256, dtype=torch.uint8).view(E4M3), torch.zeros(2, 2), out=c)
+    (_, rows), (_, norm), (_, product) = fake.l
+    assert (rows[10], rows[12]) == (256, 2) and (norm[9], norm[11]) == (256, 2) and (product[2], product[4], product[8]) == (256, 2, 160)
