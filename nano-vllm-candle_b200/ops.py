@@ -943,6 +943,7 @@ def _refuse(ctx, *facts):
 
 
 _ROWS, _F32, _I32, _E4M3 = (torch.bfloat16, torch.float32), (torch.float32,), (torch.int32,), (FP8,)
+_TOO_FAR = "sizes and row strides have to fit 31 bits"          # the library takes them as 32-bit numbers, and ctypes would drop what is above
 
 
 def _fp8_rows_given(ctx, q, scale, n: int, width: int):
@@ -990,6 +991,8 @@ def quant_fp8(ctx, x: torch.Tensor, act: int = ACT_NONE, rows=None, num_rows=Non
         q = x.new_empty(N, H, dtype=FP8) if q is None else q
         scale = x.new_empty(N, lds, dtype=torch.float32) if scale is None else scale
         ldq, lds = _fp8_rows_given(ctx, q, scale, N, H)
+    if (N | x_rows | ldx | ldq | lds) >> 31:
+        raise ValueError(_TOO_FAR)
     if N:
         st = ctx.l.nvc_quant_fp8_rows(ctx.h, x.data_ptr(), dt, ldx, x_rows, act, H, rows_at, num_at, q.data_ptr(), ldq, scale.data_ptr(), lds, N, H,
                                       torch._C._cuda_getCurrentRawStream(dev))
@@ -1009,6 +1012,8 @@ def quant_fp8_weight(ctx, w: torch.Tensor):
     else:
         groups, N, K = w.shape
         q, scale = w.new_empty(groups, N, K, dtype=FP8), w.new_empty(groups, (N + 127) // 128, (K + 127) // 128, dtype=torch.float32)
+    if (groups | N | K) >> 31:
+        raise ValueError(_TOO_FAR)
     if groups:
         st = ctx.l.nvc_quant_fp8_blocks(ctx.h, w.data_ptr(), dt, q.data_ptr(), scale.data_ptr(), groups, N, K, torch._C._cuda_getCurrentRawStream(ctx.device))
         if st:
@@ -1042,6 +1047,8 @@ def add_rmsnorm_fp8(ctx, x: torch.Tensor, w: torch.Tensor, eps: float, residual=
     if want_out:
         out = x.new_empty(N, H, dtype=BF16)
         out_at = out.data_ptr()
+    if (N | H | ldq | lds) >> 31:
+        raise ValueError(_TOO_FAR)
     if N:
         st = ctx.l.nvc_add_rmsnorm_fp8(ctx.h, x.data_ptr(), dt, res_at, res_out_at, w.data_ptr(), wdt, eps, q.data_ptr(), ldq, scale.data_ptr(), lds, out_at, N, H,
                                        torch._C._cuda_getCurrentRawStream(dev))
@@ -1085,6 +1092,8 @@ def _fp8_product(ctx, q, scale, wq, wscale, out, out_dtype, groups):
 def gemm_fp8(ctx, q, scale, wq, wscale, out_dtype=BF16, out=None) -> torch.Tensor:
     """[M, N] = rows times weight, both in 8 bits: (q, scale) of quant_fp8 or add_rmsnorm_fp8, (wq, wscale) of quant_fp8_weight; bf16 or fp32."""
     M, N, K, ldq, lds, out, ldo, dt = _fp8_product(ctx, q, scale, wq, wscale, out, out_dtype, None)
+    if (M | N | ldq | lds | ldo) >> 31:
+        raise ValueError(_TOO_FAR)
     if M:
         st = ctx.l.nvc_gemm_fp8(ctx.h, q.data_ptr(), ldq, scale.data_ptr(), lds, wq.data_ptr(), wscale.data_ptr(), out.data_ptr(), ldo, dt, M, N, K,
                                 torch._C._cuda_getCurrentRawStream(ctx.device))
@@ -1099,6 +1108,8 @@ def gemm_fp8_grouped(ctx, q, scale, wq, wscale, tile_group, out_dtype=BF16, out=
     M, N, K, ldq, lds, res, ldo, dt = _fp8_product(ctx, q, scale, wq, wscale, out, out_dtype, wq.shape[0] if wq.dim() else 0)
     if M % 128:
         raise ValueError("rows must be a multiple of 128")
+    if (M | N | ldq | lds | ldo | wq.shape[0]) >> 31:
+        raise ValueError(_TOO_FAR)
     if tile_group.get_device() != ctx.device or tile_group.dtype is not torch.int32 or tile_group.shape != (M // 128,) or not tile_group.is_contiguous():
         _refuse(ctx, ("tile_group", tile_group, _I32, (M // 128,), True))
     if M:

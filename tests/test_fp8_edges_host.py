@@ -37,3 +37,38 @@ def test_one_row_has_its_own_width_as_distance(fake):
     ops.gemm_fp8(fake, q, s, torch.zeros(160, 256, dtype=torch.uint8).view(E4M3), torch.zeros(2, 2), out=c)
     (_, rows), (_, norm), (_, product) = fake.l
     assert (rows[10], rows[12]) == (256, 2) and (norm[9], norm[11]) == (256, 2) and (product[2], product[4], product[8]) == (256, 2, 160)
+
+
+BIG = 2 ** 32 + 128                              # 128, if only its lowest 32 bits are looked at
+
+
+def test_sizes_beyond_31_bits_are_refused(fake):
+    """Sizes and strides go to the library as 32-bit numbers: one that does not fit is refused, where its low bits named another call."""
+    wq, ws = _meta(128, 256, dtype=E4M3), _meta(1, 2, dtype=torch.float32)
+    far = lambda n, w, dtype: torch.empty_strided((n, w), (BIG, 1), dtype=dtype, device="meta")
+    f32 = torch.float32
+    for call in (
+        lambda: ops.quant_fp8(fake, _meta(BIG, 256)),
+        lambda: ops.quant_fp8(fake, far(4, 256, torch.bfloat16)),
+        lambda: ops.quant_fp8(fake, _meta(BIG, 256), rows=_meta(4, dtype=torch.int32)),
+        lambda: ops.quant_fp8(fake, _meta(4, 256), rows=_meta(BIG, dtype=torch.int32)),
+        lambda: ops.quant_fp8(fake, _meta(1, BIG)),
+        lambda: ops.quant_fp8(fake, _meta(4, 256), q=far(4, 256, E4M3)),
+        lambda: ops.quant_fp8(fake, _meta(4, 256), scale=far(4, 2, f32)),
+        lambda: ops.quant_fp8_weight(fake, _meta(BIG, 256)),
+        lambda: ops.quant_fp8_weight(fake, _meta(BIG, 16, 256)),
+        lambda: ops.add_rmsnorm_fp8(fake, _meta(BIG, 256), _meta(256), 1e-6),
+        lambda: ops.add_rmsnorm_fp8(fake, _meta(4, 256), _meta(256), 1e-6, q=far(4, 256, E4M3)),
+        lambda: ops.gemm_fp8(fake, _meta(BIG, 256, dtype=E4M3), _meta(BIG, 2, dtype=f32), wq, ws),
+        lambda: ops.gemm_fp8(fake, far(4, 256, E4M3), _meta(4, 2, dtype=f32), wq, ws),
+        lambda: ops.gemm_fp8(fake, _meta(4, 256, dtype=E4M3), _meta(4, 2, dtype=f32), _meta(BIG, 256, dtype=E4M3), _meta(BIG // 128, 2, dtype=f32)),
+        lambda: ops.gemm_fp8(fake, _meta(4, 256, dtype=E4M3), _meta(4, 2, dtype=f32), wq, ws, out=far(4, 128, f32)),
+        lambda: ops.gemm_fp8_grouped(fake, _meta(BIG, 256, dtype=E4M3), _meta(BIG, 2, dtype=f32), wq[None], ws[None], _meta(BIG // 128, dtype=torch.int32)),
+        lambda: ops.gemm_fp8_grouped(fake, _meta(128, 256, dtype=E4M3), _meta(128, 2, dtype=f32), _meta(BIG, 128, 256, dtype=E4M3), _meta(BIG, 1, 2, dtype=f32),
+                                     _meta(1, dtype=torch.int32)),
+    ):
+        with pytest.raises(ValueError, match="31 bits"):
+            call()
+    assert not fake.l
+    ops.quant_fp8(fake, _meta(128, 256))
+    assert len(fake.l) == 1
