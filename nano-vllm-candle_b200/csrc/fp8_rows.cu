@@ -391,6 +391,7 @@ extern "C" int nvc_quant_fp8_rows(nvc_ctx* ctx, const void* x, int x_dtype, int 
   NVC_REQUIRE(ctx, act == NVC_ACT_NONE || act == NVC_ACT_RELU2 || act == NVC_ACT_GELU_TANH_MUL || act == NVC_ACT_SILU_MUL, NVC_EINVAL,
               "act must be NVC_ACT_NONE, _RELU2, _GELU_TANH_MUL or _SILU_MUL");
   const bool gated = act == NVC_ACT_GELU_TANH_MUL || act == NVC_ACT_SILU_MUL;
+  NVC_REQUIRE(ctx, H <= 0x7fffffff - 512, NVC_ESHAPE, "too many rows or too wide");          // column numbers of the last stretch
   NVC_REQUIRE(ctx, H % 16 == 0, NVC_ESHAPE, "H must be a multiple of 16");
   NVC_REQUIRE(ctx, !gated || (up_off >= H && up_off % 16 == 0), NVC_ESHAPE, "the second half must start at a multiple of 16 behind the first");
   NVC_REQUIRE(ctx, ldx % 8 == 0 && ldx >= (gated ? (int64_t)up_off + H : H) && ldq % 16 == 0 && ldq >= H && lds >= (H + kFp8Block - 1) / kFp8Block, NVC_ESHAPE,
@@ -463,8 +464,9 @@ extern "C" int nvc_fp8_rows_init(nvc_ctx* ctx) {
 extern "C" int nvc_quant_fp8_blocks(nvc_ctx* ctx, const void* w, int w_dtype, nvc_fp8* q, float* scale, int groups, int N, int K, void* stream) {
   NVC_REQUIRE(ctx, ctx && w && q && scale, NVC_EINVAL, "null pointer");
   NVC_REQUIRE(ctx, groups >= 0 && N > 0 && K > 0 && dtype_ok(w_dtype), NVC_EINVAL, "bad sizes or dtype");
+  NVC_REQUIRE(ctx, N <= 65535 * kFp8Block && K <= 0x7fffffff - kFp8Block && groups <= 65535, NVC_ESHAPE, "too many rows or too wide: groups and N / 128 are at most 65 535");
+  NVC_REQUIRE(ctx, K % 16 == 0, NVC_ESHAPE, "K must be a multiple of 16");
   const int rows = (N + kFp8Block - 1) / kFp8Block;
-  NVC_REQUIRE(ctx, K % 16 == 0 && rows <= 65535 && groups <= 65535, NVC_ESHAPE, "K must be a multiple of 16, groups and N / 128 at most 65 535");
   NVC_REQUIRE(ctx, aligned16(w) && aligned16(q), NVC_EINVAL, "pointers must be 16-byte aligned");
   if (groups == 0) return NVC_OK;
   const dim3 grid((K + kFp8Block - 1) / kFp8Block, rows, groups);

@@ -807,12 +807,13 @@ int nvc_gemm_fp8_check(nvc_ctx* ctx, const nvc_fp8* A, int lda, const float* a_s
           int K, int groups) {
   NVC_REQUIRE(ctx, ctx && A && a_scale && W && w_scale && C, NVC_EINVAL, "null pointer");
   NVC_REQUIRE(ctx, M >= 0 && Nout > 0 && K > 0 && groups > 0, NVC_EINVAL, "bad sizes");
+  // row and column numbers of the last tiles
+  NVC_REQUIRE(ctx, (int64_t)Nout * groups <= 0x7fffffff - 2 * BM && M <= 0x7fffffff - 2 * BM && K <= 0x7fffffff - BK, NVC_ESHAPE, "too many rows or too wide");
   NVC_REQUIRE(ctx, K % 16 == 0 && Nout % 16 == 0, NVC_ESHAPE, "K and Nout must be multiples of 16");
   NVC_REQUIRE(ctx, lda % 16 == 0 && lda >= K && ldc % 8 == 0 && ldc >= Nout && lds >= (K + BK - 1) / BK, NVC_ESHAPE,
               "row strides must cover the rows, A's be a multiple of 16 and C's of 8");
   NVC_REQUIRE(ctx, out_dtype == NVC_DT_BF16 || out_dtype == NVC_DT_F32, NVC_EINVAL, "bad out_dtype");
   NVC_REQUIRE(ctx, ((uintptr_t)A % 16) == 0 && ((uintptr_t)W % 16) == 0 && ((uintptr_t)C % 16) == 0, NVC_EINVAL, "pointers must be 16-byte aligned");
-  NVC_REQUIRE(ctx, (int64_t)Nout * groups <= 0x7fffffffLL && M <= 0x7fffffff - 2 * BM, NVC_ESHAPE, "too many rows");
   NVC_REQUIRE(ctx, ctx->encode_tiled != nullptr, NVC_EDEVICE, "cuTensorMapEncodeTiled unavailable");
   return NVC_OK;
 }

@@ -176,3 +176,20 @@ def test_one_row_of_any_stride(ctx):
     want = ops.add_rmsnorm_fp8(ctx, x, w, 1e-6)
     ops.add_rmsnorm_fp8(ctx, x, w, 1e-6, q=q, scale=s)
     assert torch.equal(_bits(q), _bits(want[0])) and torch.equal(s, want[1])
+
+
+def test_refusals_of_widths(ctx):
+    """Widths and rows whose number of blocks passes 31 bits on the way: refused before anything is read, where it became a negative number."""
+    q, s = torch.empty(4, 256, dtype=torch.uint8, device=DEV), torch.ones(4, 2, device=DEV)
+    w, l, h = torch.ones(128, 256, dtype=BF16, device=DEV), ctx.l, ctx.h
+    top = 2 ** 31 - 16                               # the largest multiple of 16
+    p, sp, wp = q.data_ptr(), s.data_ptr(), w.data_ptr()
+    calls = [lambda: l.nvc_quant_fp8_rows(h, wp, 0, top, 4, ops.ACT_NONE, 0, None, None, p, top, sp, 2, 0, top, 0),
+             lambda: l.nvc_quant_fp8_blocks(h, wp, 0, p, sp, 0, 2 ** 31 - 1, 256, 0), lambda: l.nvc_quant_fp8_blocks(h, wp, 0, p, sp, 0, 256, top, 0),
+             lambda: l.nvc_gemm_fp8_grouped(h, p, 256, sp, 2, p, sp, wp, 128, 0, 0, 128, 256, sp, 2 ** 24 - 1, 0, 0)]
+    for N, K in ((128, top), (top, 256)):
+        calls += [lambda N=N, K=K: l.nvc_gemm_fp8(h, p, K, sp, 2, p, sp, wp, N, 0, 0, N, K, 0),
+                  lambda N=N, K=K: l.nvc_gemm_fp8_grouped(h, p, K, sp, 2, p, sp, wp, N, 0, 0, N, K, sp, 1, 0, 0)]
+    for i, call in enumerate(calls):                 # none of them has rows: nothing would be launched
+        assert call() == -2, i
+        assert b"too many rows or too wide" in l.nvc_last_error(h), i
