@@ -112,11 +112,15 @@ class LinearBase:
         self.weight_fp8: Optional[Tuple[torch.Tensor, torch.Tensor]] = None       # (e4m3 [out, in], scale [ceil(out / 128), ceil(in / 128)])
 
     def to_fp8(self) -> "LinearBase":
-        """Converts the loaded weight (this rank's share of it) to 8 bits, once; the bf16 weight is given up."""
+        """Converts the loaded weight (this rank's share of it) to 8 bits, once; the bf16 weight is given up, and the shards it came from: to load one again takes all."""
         if self.weight is None:
             raise RuntimeError("load_weights has not been called")
         self.weight_fp8, self.weight = ops.quant_fp8_weight(self.ctx, self.weight), None
+        self._forget_shards()
         return self
+
+    def _forget_shards(self) -> None:
+        """Layers that are loaded in shards hold them until all are there, and after: a shard may be loaded again."""
 
     def load_fp8(self, weight: torch.Tensor, scale: torch.Tensor) -> None:
         """This rank's weight as e4m3 [out, in] with its scales [ceil(out / 128), ceil(in / 128)]."""
@@ -124,6 +128,7 @@ class LinearBase:
         if weight.dtype != ops.FP8 or tuple(scale.shape) != ((n + 127) // 128, (k + 127) // 128):
             raise ValueError("load_fp8: an e4m3 weight [out, in] and scales [ceil(out / 128), ceil(in / 128)]")
         self.weight_fp8, self.weight = (weight.contiguous(), scale.to(torch.float32).contiguous()), None
+        self._forget_shards()
 
     def _set(self, w: torch.Tensor, bias):
         if bias is not None:
@@ -181,6 +186,9 @@ class MergedColumnParallelLinear(LinearBase):
         if all(p is not None for p in self._parts):
             self._set(torch.cat(self._parts, dim=0), bias)
 
+    def _forget_shards(self):
+        self._parts = [None] * len(self.output_sizes)
+
 
 class QKVParallelLinear(LinearBase):
     """Fused q/k/v rows, sharded by head group (linear.rs:121-176)."""
@@ -196,6 +204,9 @@ class QKVParallelLinear(LinearBase):
         self._parts[shard_id] = w[self.tp_rank * n:(self.tp_rank + 1) * n]
         if len(self._parts) == 3:
             self._set(torch.cat([self._parts["q"], self._parts["k"], self._parts["v"]], dim=0), None)
+
+    def _forget_shards(self):
+        self._parts = {}
 
     def load_weights(self, weight, bias=None):
         """Full fused [q; k; v] weight (qwen3.rs:171-173)."""

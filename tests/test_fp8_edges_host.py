@@ -72,3 +72,46 @@ def test_sizes_beyond_31_bits_are_refused(fake):
     assert not fake.l
     ops.quant_fp8(fake, _meta(128, 256))
     assert len(fake.l) == 1
+
+
+# ----------------------------------------------------------------------------- layers
+layers = importlib.import_module("nano-vllm-candle_b200.layers")
+tp = importlib.import_module("nano-vllm-candle_b200.tp")
+
+
+def _loaded(ctx, kind):
+    """A layer of 64 inputs with its weight loaded shard by shard, and how to load its first shard again."""
+    full = torch.randn(96, 64)
+    if kind == "merged":
+        layer = layers.MergedColumnParallelLinear(ctx, 64, [48, 48])
+        layer.load_weights(full[:48], loaded_shard_id=0)
+        layer.load_weights(full[48:], loaded_shard_id=1)
+        return layer, lambda w: layer.load_weights(w, loaded_shard_id=0), full
+    layer = layers.QKVParallelLinear(ctx, 64, 16, 4, 1)
+    for name, w in zip("qkv", full.split([64, 16, 16])):
+        layer.load_qkv_weight(w, name)
+    return layer, lambda w: layer.load_qkv_weight(w, "q"), full
+
+
+@pytest.mark.parametrize("kind", ["merged", "qkv"])
+@pytest.mark.parametrize("how", ["to_fp8", "load_fp8"])
+def test_8_bits_give_up_the_loaded_shards(fake, kind, how):
+    """Merged layers hold their shards, views of whole tensors: converted, they hold none of them; a later load starts with all of them."""
+    import gc
+    import weakref
+    layer, again, full = _loaded(fake, kind)
+    parts = [weakref.ref(p) for p in (layer._parts if kind == "merged" else layer._parts.values())]
+    assert all(p() is not None for p in parts)
+    if how == "to_fp8":
+        assert layer.to_fp8() is layer
+    else:
+        layer.load_fp8(torch.zeros(96, 64, dtype=torch.uint8).view(E4M3), torch.ones(1, 1))
+    gc.collect()
+    assert layer.weight is None and layer.weight_fp8[0].shape == (96, 64) and not any(p() is not None for p in parts)
+    again(torch.randn(48 if kind == "merged" else 64, 64))
+    assert layer.weight is None and layer.weight_fp8 is not None          # the other shards are gone
+    if kind == "merged":
+        layer.load_weights(torch.randn(48, 64), loaded_shard_id=1)
+    else:
+        layer.load_weights(torch.randn(96, 64))
+    assert layer.weight.shape == (96, 64) and layer.weight_fp8 is None
