@@ -119,14 +119,21 @@ class LinearBase:
         self._forget_shards()
         return self
 
+    def _share(self) -> Tuple[int, int]:
+        """(out, in) of the weight that this rank has."""
+        return self.output_size, self.input_size
+
     def _forget_shards(self) -> None:
         """Layers that are loaded in shards hold them until all are there, and after: a shard may be loaded again."""
 
     def load_fp8(self, weight: torch.Tensor, scale: torch.Tensor) -> None:
-        """This rank's weight as e4m3 [out, in] with its scales [ceil(out / 128), ceil(in / 128)]."""
-        n, k = weight.shape
-        if weight.dtype != ops.FP8 or tuple(scale.shape) != ((n + 127) // 128, (k + 127) // 128):
-            raise ValueError("load_fp8: an e4m3 weight [out, in] and scales [ceil(out / 128), ceil(in / 128)]")
+        """This rank's share of the weight as e4m3 [out, in] with its scales [ceil(out / 128), ceil(in / 128)], on the context's device."""
+        n, k = self._share()
+        if weight.dtype != ops.FP8 or tuple(weight.shape) != (n, k) or not scale.is_floating_point() or tuple(scale.shape) != ((n + 127) // 128, (k + 127) // 128):
+            raise ValueError(f"load_fp8: this rank has an e4m3 weight [{n}, {k}] and scales [{(n + 127) // 128}, {(k + 127) // 128}], "
+                             f"got {weight.dtype} {list(weight.shape)} and {scale.dtype} {list(scale.shape)}")
+        if weight.get_device() != self.ctx.device or scale.get_device() != self.ctx.device:
+            raise ValueError(f"load_fp8: weight and scales must be on cuda:{self.ctx.device}")
         self.weight_fp8, self.weight = (weight.contiguous(), scale.to(torch.float32).contiguous()), None
         self._forget_shards()
 
@@ -170,6 +177,9 @@ class ColumnParallelLinear(LinearBase):
         n = weight.shape[0] // self.tp_size
         self._set(weight[self.tp_rank * n:(self.tp_rank + 1) * n], bias)
 
+    def _share(self):
+        return self.output_size // self.tp_size, self.input_size
+
 
 class MergedColumnParallelLinear(LinearBase):
     """Several column-parallel matrices fused along the output dim (gate_up): each is sharded
@@ -185,6 +195,9 @@ class MergedColumnParallelLinear(LinearBase):
         self._parts[loaded_shard_id] = weight[self.tp_rank * n:(self.tp_rank + 1) * n]
         if all(p is not None for p in self._parts):
             self._set(torch.cat(self._parts, dim=0), bias)
+
+    def _share(self):
+        return sum(n // self.tp_size for n in self.output_sizes), self.input_size
 
     def _forget_shards(self):
         self._parts = [None] * len(self.output_sizes)
@@ -204,6 +217,9 @@ class QKVParallelLinear(LinearBase):
         self._parts[shard_id] = w[self.tp_rank * n:(self.tp_rank + 1) * n]
         if len(self._parts) == 3:
             self._set(torch.cat([self._parts["q"], self._parts["k"], self._parts["v"]], dim=0), None)
+
+    def _share(self):
+        return (self.num_heads // self.tp_size + 2 * (self.num_kv_heads // self.tp_size)) * self.head_size, self.input_size
 
     def _forget_shards(self):
         self._parts = {}
@@ -227,6 +243,9 @@ class RowParallelLinear(LinearBase):
     def load_weights(self, weight, bias=None):
         n = weight.shape[1] // self.tp_size
         self._set(weight[:, self.tp_rank * n:(self.tp_rank + 1) * n], bias)
+
+    def _share(self):
+        return self.output_size, self.input_size // self.tp_size
 
     def forward(self, x):
         y = super().forward(x)

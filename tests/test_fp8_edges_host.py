@@ -115,3 +115,42 @@ def test_8_bits_give_up_the_loaded_shards(fake, kind, how):
     else:
         layer.load_weights(torch.randn(96, 64))
     assert layer.weight.shape == (96, 64) and layer.weight_fp8 is None
+
+
+def _layer_of(ctx, kind, size, rank):
+    cfg = tp.TPConfig(size, rank, 0)
+    return {"replicated": lambda: layers.ReplicatedLinear(ctx, 256, 384),
+            "column": lambda: layers.ColumnParallelLinear(ctx, 256, 384, cfg),
+            "merged": lambda: layers.MergedColumnParallelLinear(ctx, 256, [256, 128], cfg),
+            "qkv": lambda: layers.QKVParallelLinear(ctx, 256, 32, 8, 2, cfg),
+            "row": lambda: layers.RowParallelLinear(ctx, 256, 384, cfg)}[kind]()
+
+
+@pytest.mark.parametrize("kind", ["replicated", "column", "merged", "qkv", "row"])
+@pytest.mark.parametrize("size", [1, 2])
+def test_load_fp8_takes_this_ranks_share_alone(fake, kind, size):
+    """Another layer's weight, a whole one for a rank's share, one that lies on its side, wrong scales, another device: refused, and the weight of before stays."""
+    n, k = {"replicated": (384, 256), "row": (384, 256 // size)}.get(kind, (384 // size, 256))
+    weight = lambda n, k, device="cpu": torch.zeros(n, k, dtype=torch.uint8, device=device).view(E4M3)
+    scale = lambda n, k, device="cpu": torch.ones((n + 127) // 128, (k + 127) // 128, device=device)
+    layer = _layer_of(fake, kind, size, size - 1)
+    before = torch.zeros(n, k, dtype=torch.bfloat16)
+    layer._set(before, None)
+    others = {(384, 256), (256, 384), (192, 256), (384, 128), (n + 128, k), (n, k + 128), (n // 2, k)} - {(n, k)}
+    for shape in sorted(others):
+        with pytest.raises(ValueError):
+            layer.load_fp8(weight(*shape), scale(*shape))
+    for w, s in ((weight(n, k), scale(n + 128, k)), (weight(n, k), scale(n, k).T.contiguous()[:, :1]), (weight(n, k).view(torch.uint8), scale(n, k)),
+                 (weight(n, k, "meta"), scale(n, k)), (weight(n, k)[None], scale(n, k)), (weight(n, k), scale(n, k).to(torch.int32))):
+        if w.device.type == "meta":
+            fake.device = 0                      # a tensor of no device of ours
+        with pytest.raises(ValueError):
+            layer.load_fp8(w, s)
+        fake.device = -1
+    assert torch.equal(layer.weight, before) and layer.weight_fp8 is None
+    layer.load_fp8(weight(n, k), scale(n, k).to(torch.bfloat16))
+    assert layer.weight is None and layer.weight_fp8[1].dtype == torch.float32
+    kept = layer.weight_fp8
+    with pytest.raises(ValueError):
+        layer.load_fp8(weight(k, n + 16), scale(k, n + 16))
+    assert layer.weight_fp8 is kept
