@@ -115,9 +115,15 @@ class LinearBase:
         """Converts the loaded weight (this rank's share of it) to 8 bits, once; the bf16 weight is given up, and the shards it came from: to load one again takes all."""
         if self.weight is None:
             raise RuntimeError("load_weights has not been called")
+        self._multiples_of_16("to_fp8", *self.weight.shape)
         self.weight_fp8, self.weight = ops.quant_fp8_weight(self.ctx, self.weight), None
         self._forget_shards()
         return self
+
+    @staticmethod
+    def _multiples_of_16(name: str, n: int, k: int) -> None:
+        if n % 16 or k % 16:
+            raise ValueError(f"{name}: products in 8 bits take multiples of 16, the weight is [{n}, {k}]")
 
     def _share(self) -> Tuple[int, int]:
         """(out, in) of the weight that this rank has."""
@@ -132,6 +138,7 @@ class LinearBase:
         if weight.dtype != ops.FP8 or tuple(weight.shape) != (n, k) or not scale.is_floating_point() or tuple(scale.shape) != ((n + 127) // 128, (k + 127) // 128):
             raise ValueError(f"load_fp8: this rank has an e4m3 weight [{n}, {k}] and scales [{(n + 127) // 128}, {(k + 127) // 128}], "
                              f"got {weight.dtype} {list(weight.shape)} and {scale.dtype} {list(scale.shape)}")
+        self._multiples_of_16("load_fp8", n, k)
         if weight.get_device() != self.ctx.device or scale.get_device() != self.ctx.device:
             raise ValueError(f"load_fp8: weight and scales must be on cuda:{self.ctx.device}")
         self.weight_fp8, self.weight = (weight.contiguous(), scale.to(torch.float32).contiguous()), None

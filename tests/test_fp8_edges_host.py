@@ -154,3 +154,17 @@ def test_load_fp8_takes_this_ranks_share_alone(fake, kind, size):
     with pytest.raises(ValueError):
         layer.load_fp8(weight(k, n + 16), scale(k, n + 16))
     assert layer.weight_fp8 is kept
+
+
+@pytest.mark.parametrize("n,k", [(300, 256), (304, 264)])
+def test_to_fp8_keeps_a_weight_that_no_product_takes(fake, n, k):
+    """Products take sizes that are multiples of 16: refused where the bf16 weight is still there, not at the first product."""
+    layer = layers.ReplicatedLinear(fake, k, n)
+    weight = torch.randn(n, k).to(torch.bfloat16)
+    layer.load_weights(weight)
+    with pytest.raises(ValueError, match="multiples of 16"):
+        layer.to_fp8()
+    assert torch.equal(layer.weight, weight) and layer.weight_fp8 is None
+    with pytest.raises(ValueError, match="multiples of 16"):
+        layer.load_fp8(torch.zeros(n, k, dtype=torch.uint8).view(E4M3), torch.ones(3, 3 if k > 256 else 2))
+    assert torch.equal(layer.weight, weight) and not fake.l
