@@ -193,3 +193,117 @@ def test_refusals_of_widths(ctx):
     for i, call in enumerate(calls):                 # none of them has rows: nothing would be launched
         assert call() == -2, i
         assert b"too many rows or too wide" in l.nvc_last_error(h), i
+
+
+# ----------------------------------------------------------------------------- tiles behind the first, bands, loops
+def _whole(seed, M, N, K, groups=None):
+    """Numbers of -3 to 3 with scales that are powers of two, different for every block, and the product in 64 bits' arguments: every sum is exact in fp32."""
+    g, kb, nb = _g(seed), (K + 127) // 128, (N + 127) // 128
+    lead = () if groups is None else (groups,)
+    whole = lambda *shape: torch.randint(-3, 4, shape, generator=g, device=DEV).float()
+    two = lambda *shape: torch.exp2(torch.randint(-2, 3, shape, generator=g, device=DEV).float())
+    q, s, wq, ws = whole(M, K), two(M, kb), whole(*lead, N, K), two(*lead, nb, kb)
+    a = q.to(F64) * s.to(F64).repeat_interleave(128, -1)[:, :K]
+    w = wq.to(F64) * ws.to(F64).repeat_interleave(128, -2)[..., :N, :].repeat_interleave(128, -1)[..., :K]
+    return q.to(E4M3), s, wq.to(E4M3), ws, a, w
+
+
+def _forced(ctx, route, q, s, wq, ws, dtype):
+    (M, K), N = q.shape, wq.shape[0]
+    c = torch.full((M + 1, N + 8), 7.0, dtype=dtype, device=DEV)
+    assert ctx.l.nvc_gemm_fp8_ex(ctx.h, q.data_ptr(), K, s.data_ptr(), s.shape[1], wq.data_ptr(), ws.data_ptr(), c.data_ptr(), N + 8, int(dtype == F32), M, N, K, route,
+                                 torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.all(c[M] == 7.0) and torch.all(c[:, N:] == 7.0)
+    return c[:M, :N]
+
+
+@pytest.mark.parametrize("K", [128, 272, 1040])
+@pytest.mark.parametrize("route", [41, 51, 61])
+def test_several_tiles_to_a_cta(ctx, route, K):
+    """Two and more tiles to every CTA, or pair of them: ring, accumulators and what was asked ahead go on from tile to tile.  More k-blocks than stages, and fewer."""
+    M, N = 2500, 5008                            # 400 tiles of 128 x 256, 200 of 256 x 256
+    q, s, wq, ws, a, w = _whole(K, M, N, K)
+    want = a @ w.T
+    for dtype in (F32, BF16):
+        for _ in range(2):
+            assert torch.equal(_forced(ctx, route, q, s, wq, ws, dtype), want.to(F32).to(dtype))
+    assert torch.equal(ops.gemm_fp8(ctx, q, s, wq, ws, out_dtype=F32), want.to(F32))
+
+
+@pytest.mark.parametrize("M,N,K", [(4764, 8208, 4112), (6300, 2064, 16400)])
+def test_bands_of_row_tiles(ctx, M, N, K):
+    """Weights above 32 MB are walked in bands of row tiles: 19 in two bands, 25 in three, the last one shorter."""
+    q, s, wq, ws, a, w = _whole(M, M, N, K)
+    want = (a @ w.T).to(F32)
+    assert torch.equal(_forced(ctx, 61, q, s, wq, ws, F32), want)
+    assert torch.equal(ops.gemm_fp8(ctx, q, s, wq, ws, out_dtype=F32), want)
+    assert torch.equal(ops.gemm_fp8(ctx, q, s, wq, ws), want.to(BF16))
+
+
+@pytest.mark.parametrize("counts,N,K", [([2000, 1500, 0, 77, 3000], 4112, 272), ([130] * 9 + [0, 1000], 2064, 1040), ([5] * 40, 1040, 144)])
+def test_several_tiles_of_experts_to_a_cta(ctx, counts, N, K):
+    tiles = sum([[e] * ((n + 127) // 128) for e, n in enumerate(counts)], [])
+    tiles.insert(len(tiles) // 2, -1)
+    tiles += [-1, -1]
+    q, s, wq, ws, a, w = _whole(N, 128 * len(tiles), N, K, len(counts))
+    group = torch.tensor(tiles, dtype=torch.int32, device=DEV)
+    for dtype in (F32, BF16):
+        got = ops.gemm_fp8_grouped(ctx, q, s, wq, ws, group, out_dtype=dtype)
+        for t, e in enumerate(tiles):
+            rows = slice(128 * t, 128 * t + 128)
+            assert torch.equal(got[rows], (a[rows] @ w[e].T).to(F32).to(dtype) if e >= 0 else torch.zeros_like(got[rows])), t
+
+
+@pytest.mark.parametrize("act", [ops.ACT_SILU_MUL, ops.ACT_GELU_TANH_MUL])
+@pytest.mark.parametrize("N,H,dtype", [(1000, 12288, BF16), (9001, 1040, BF16), (4000, 3088, F32)])
+def test_gated_rows_of_large_inputs(ctx, act, N, H, dtype):
+    """Above 16 CTAs per SM a warp goes on from part to part: the bits that a hundred rows at a time give, which need no second part."""
+    x = (3 * torch.randn(N, 2 * H, generator=_g(N), device=DEV)).to(dtype)
+    q, s = ops.quant_fp8(ctx, x, act=act)
+    for at in range(0, N, 100):
+        q1, s1 = ops.quant_fp8(ctx, x[at:at + 100], act=act)
+        assert torch.equal(_bits(q)[at:at + 100], _bits(q1)) and torch.equal(s[at:at + 100], s1), at
+
+
+@pytest.mark.parametrize("act", [ops.ACT_NONE, ops.ACT_RELU2, ops.ACT_SILU_MUL])
+@pytest.mark.parametrize("M,H", [(64, 144), (70, 1040), (9100, 1040), (20, 16)])
+def test_rows_gathered_where_blocks_go_one_behind_the_other(ctx, act, M, H):
+    """Widths whose blocks do not fill a warp's stretches, with rows by number and a count of them: what a gather in front gives, nothing behind the count."""
+    x = torch.randn(40, 2 * H if act == ops.ACT_SILU_MUL else H, generator=_g(H), device=DEV).to(BF16)
+    rows = torch.randint(0, 40, (M,), generator=_g(M), device=DEV, dtype=torch.int32)
+    rows[3], rows[5], rows[6], rows[11] = -1, 40, rows[7], 2 ** 31 - 1
+    there = (rows >= 0) & (rows < 40)
+    want_q, want_s = ops.quant_fp8(ctx, torch.where(there[:, None], x[rows.clamp(0, 39).long()], torch.zeros((), dtype=BF16, device=DEV)), act=act)
+    for used in (0, 1, M // 2, M - 1, M, M + 7, -3):
+        q, s = torch.full((M, H), 0x33, dtype=torch.uint8, device=DEV).view(E4M3), torch.full(want_s.shape, 7.0, device=DEV)
+        ops.quant_fp8(ctx, x, act=act, rows=rows, num_rows=torch.tensor([used], dtype=torch.int32, device=DEV), q=q, scale=s)
+        n = min(max(used, 0), M)
+        assert torch.equal(_bits(q)[:n], _bits(want_q)[:n]) and torch.equal(s[:n], want_s[:n]), used
+        assert torch.all(_bits(q)[n:] == 0x33) and torch.all(s[n:] == 7.0), used
+
+
+def test_calls_on_several_streams_at_once(ctx):
+    """Three streams with products of every kernel, norms and rows in flight together: nothing is shared between calls, the bits are those of one call after the other."""
+    sizes = [(3, 1056, 2048), (24, 800, 4096), (150, 1536, 1040), (300, 2080, 512), (1100, 1024, 1024), (2600, 3104, 640)]
+    work = []
+    for i, (M, N, K) in enumerate(sizes):
+        x, w = torch.randn(M, K, generator=_g(i), device=DEV).to(BF16), torch.ones(K, dtype=BF16, device=DEV)
+        work.append((x, w, ops.quant_fp8_weight(ctx, torch.randn(N, K, generator=_g(10 + i), device=DEV) * K ** -0.5)))
+
+    def step(x, w, weight):
+        q, s, _ = ops.add_rmsnorm_fp8(ctx, x, w, 1e-6)
+        y = ops.gemm_fp8(ctx, q, s, *weight)
+        return y, *ops.quant_fp8(ctx, y, act=ops.ACT_SILU_MUL)
+
+    want = [step(*t) for t in work]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(3)], []
+    for _ in range(4):
+        for i in range(len(work)):
+            for j, stream in enumerate(streams):
+                with torch.cuda.stream(stream):
+                    k = (i + 2 * j) % len(work)
+                    got.append((k, step(*work[k])))
+    torch.cuda.synchronize()
+    for k, out in got:
+        assert all(torch.equal(_bits(a), _bits(b)) for a, b in zip(out, want[k])), k
