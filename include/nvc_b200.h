@@ -737,7 +737,8 @@ int nvc_quant_fp8_rows(nvc_ctx* ctx, const void* x, int x_dtype, int ldx, int x_
 /* nvc_fused_add_rmsnorm with 8-bit rows behind it, from the fp32 result:
  *   s = x + residual_in (optional); residual_out = s (optional, may alias);  y = s * rsqrt(mean(s^2) + eps) * w;
  *   q, scale = the 8-bit form of y;  out = bf16(y) (optional: a router reads it).
- * x, w: bf16 or fp32; x, residuals, out contiguous.  H <= 16384. */
+ * x, w: bf16 or fp32; x, residuals, out contiguous.  H <= 16384.  Few and many rows take kernels that add in another order: a row's last bits may depend
+ * on how many come with it (so may a product's, which takes its kernel by the number of rows). */
 int nvc_add_rmsnorm_fp8(nvc_ctx* ctx, const void* x, int x_dtype, const float* residual_in, float* residual_out, const void* w, int w_dtype, float eps,
                         nvc_fp8* q, int ldq, float* scale, int lds, nvc_bf16* out, int N, int H, void* stream);
 /* Weights w [groups, N, K] (bf16 or fp32, contiguous) -> q [groups, N, K], scale [groups, ceil(N / 128), ceil(K / 128)]; blocks end with their group.

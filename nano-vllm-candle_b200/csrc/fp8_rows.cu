@@ -403,7 +403,7 @@ extern "C" int nvc_quant_fp8_rows(nvc_ctx* ctx, const void* x, int x_dtype, int 
   const bool flat = 40 * stretches > 11 * blocks && (int64_t)N * blocks < 0xfffffff0LL;
   const int64_t ctas = ((flat ? ((int64_t)N * blocks + 3) / 4 : (int64_t)N * stretches) + kRowsPerCta - 1) / kRowsPerCta;
   NVC_REQUIRE(ctx, ctas <= 0x7fffffffLL, NVC_ESHAPE, "too many rows");
-  // gated units of large inputs go on from stretch to stretch: 64 x 12 288 bf16 2.7 us for 3.5, 8 191 x 12 288 87 for 89; nothing to gain where nothing is computed (49 for 55)
+  // gated units of large inputs go on from stretch to stretch (with a lighter unit 64 x 12 288 bf16 2.7 us for 3.5, 8 191 x 12 288 87 for 89); nothing to gain where nothing is computed (49 for 55)
   const int64_t grid = gated && ctas > (int64_t)ctx->num_sms * 16 ? (int64_t)ctx->num_sms * 16 : ctas;
   DeviceGuard guard(ctx->device);
   NVC_DISPATCH_DT(x_dtype, T, {
@@ -433,7 +433,7 @@ extern "C" int nvc_add_rmsnorm_fp8(nvc_ctx* ctx, const void* x, int x_dtype, con
     const int stages = std::max(1, std::min(4, std::max(200 * 1024 / row / std::max(1024 / threads, 1), 200 * 1024 / row >= 2 ? 2 : 1)));
     const int per_sm = std::max(1, std::min({1024 / threads, 24, 200 * 1024 / (stages * row)}));
     const int64_t places = std::min<int64_t>((int64_t)ctx->num_sms * per_sm, N);
-    // a ring where SMs have several rows and half a million numbers to go through (a CTA per row / ring, us: 148 x 4 096 3.2 / 4.5, 300 5.7 / 5.2, 1 200 13.7 / 10.8; 300 x 1 024
+    // a ring where SMs have several rows and half a million numbers to go through (a CTA per row / ring, us: 148 x 4 096 3.2 / 4.5, 300 5.7 / 5.2, 1 200 13.7 / 10.5; 300 x 1 024
     // 2.8 / 3.3, 600 4.1 / 3.9; 1 800 x 256 4.25 / 4.06, 5 000 8.1 / 6.4)
     if (N < 2 * ctx->num_sms || (int64_t)N * H < (1 << 19)) {
       NVC_CUDA_CHECK(ctx, nvc_launch(ctx, one, dim3(N), dim3(threads), 0, nvc_stream(stream), xt, residual_in, residual_out, wt, eps, q, (int64_t)ldq, scale, (int64_t)lds, out, H));

@@ -3,7 +3,10 @@
 // The inner sums run on the tensor cores (e4m3 products are exact in fp32) in an accumulator of their own per k-block; the outer sums, whose factors differ
 // from block to block, in fp32 registers.
 //
-// What bounds them: the tensor pipe takes 512 cycles for a k-block of 128 x 256, and the epilogue has to read and scale every k-block's sums in the same time.
+// What bounds them: the tensor pipe takes 512 cycles for a k-block of 128 x 256, the epilogue has to read and scale every k-block's sums in the same time, and the operands have to come
+// from L2.  On CTA pairs (32 KB per k-block and SM) the epilogue holds them; tiles of one CTA are held by the operands' way (48 KB, and 32 for 128 x 128).  Numbers of zero, us, whole /
+// nothing read and summed / a quarter of the tensor instructions besides: 4 096 x 4 096 x 4 096 on pairs 55.5 / 46.8 / 42.7, tiles of 256 columns 61.0 / 57.7 / 48.1, of 128 64.5 / 57.8 /
+// 50.3; 72 blocks of rows by expert, 4 096 x 2 048, 75.2 / 69.6 / 60.5; 333 x 4 096 x 2 560 on tiles of 128 9.9 / 9.4 / 8.5.
 // 8 192 x 24 576 x 4 096 bf16: 660 to 680 us in short runs (2.4 PFLOP/s), 792 after seconds of them, which the power cap holds at 1.35 GHz; numbers of zero, which need
 // less power, 535 (3.1) and 595 at 1.77 GHz.  That is 790 to 805 cycles per k-block of a pair's 256 x 256.
 //
@@ -826,8 +829,8 @@ struct Route {
 
 // The kernel with the least time by a model of waves and k-blocks (us): a start, w waves, k-blocks per wave (those of a full chip take longer), the weights' way from
 // memory where a wave does not show it, the sums' way over the cluster.  Fitted to 3 229 timings of 301 products (17 weights of 0.4 to 100 MB, 1 to 4 096 rows): 6 to 10 % off
-// in the mean, and its choice is 1.3 % above the best of all kernels and shares, at most 19 %.  No one kernel does it all: 64 x 1 024 x 2 048 4.3 us on kFew32 with
-// eight shares, 6.5 on kRows128, 9.5 on kPair; 256 x 4 096 x 4 096 11.2 on kShared with two, 12.7, 17.0; 512 x 24 576 x 4 096 51 on kPair, 71 on kRows128.
+// in the mean; its choice is 1.4 % above the best of all kernels and shares in the mean, at most 21 % (profiles/fp8_product_routes.txt).  No one kernel does it all: 64 x 1 024 x 2 048
+// 4.4 us on kFew32 with five shares, 6.4 on kRows128, 9.0 on kPair; 256 x 4 096 x 4 096 11.1 on kShared with two, 12.4, 16.7; 512 x 24 576 x 4 096 49.6 on kPair, 69.7 on kRows128.
 Route choose_route(const nvc_ctx* ctx, int M, int N, int num_kb) {
   const double mb = (double)N * num_kb * BK * 1e-6;
   auto tiles = [&](int rows, int cols) { return (double)((M + rows - 1) / rows) * ((N + cols - 1) / cols); };
