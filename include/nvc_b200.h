@@ -754,6 +754,46 @@ int nvc_gemm_fp8(nvc_ctx* ctx, const nvc_fp8* A, int lda, const float* a_scale, 
 int nvc_gemm_fp8_grouped(nvc_ctx* ctx, const nvc_fp8* A, int lda, const float* a_scale, int lds, const nvc_fp8* W, const float* w_scale, void* C, int ldc,
                          int out_dtype, int M_cap, int Nout, int K, const int32_t* tile_group, int groups, int zero, void* stream);
 
+/* ---- a paged key-value cache in 4 bits, and the attention that reads it (serving only) ----
+ * A cached row of 128 numbers is 8 blocks of 16.  A block is 16 codes of 4 bits (e2m1: sign, then a magnitude of 0, 0.5, 1, 1.5, 2, 3, 4, 6) and a scale of 8 bits
+ * (5 of exponent, 3 of mantissa, no sign: the fp16 number with the bits b << 7); a number stands for code * scale:
+ *   scale = nearest(max|x| / 6), half way to the even mantissa, at most 10240;   code = nearest(x / scale), half way to the smaller magnitude, at most 6.
+ * 72 bytes a row in place of 256, and no scale to be calibrated.  Numbers beyond 61440 become +-61440, a block whose largest is below 2^-18 * 6 zeros; a block with
+ * an infinity or a NaN (scale byte 255) reads as NaN.
+ * Layout: k, v [num_blocks, kv, block_size, 64] (number 2i in the low half of byte i), k_scale, v_scale [num_blocks, kv, block_size, 8], each 16-byte aligned: a
+ * page's rows of one key head lie together.  block_size % 16 == 0, num_blocks * block_size < 2^31; the slot of a token is block * block_size + offset, as above.
+ * head_dim is 128.  These calls have no static operands (launch order, above): everything, tables and lengths too, is read behind the wait. */
+typedef struct nvc_fp4_cache {
+  uint8_t *k, *k_scale, *v, *v_scale;
+  int num_blocks, kv, block_size;
+} nvc_fp4_cache;
+/* nvc_qk_norm_rope_store with such a cache.  qkv: bf16 rows of (nh + 2 kv) * 128, stride ld.  q_out == NULL: q and k heads in place, as there; else the q heads go to
+ * q_out (rows of nh * 128, stride ldqo) and qkv is left as it is.  The k rows enter the cache from their bf16 form.  A slot that is negative or beyond the cache is passed
+ * over; no slot may come twice.  cos_sin: [max_pos, 128] (nvc_rope_table_init_sync); a position outside gives rows of NaN.  qw == kw == NULL: rotation alone.
+ * Strides are multiples of 8, pointers 16-byte aligned. */
+int nvc_qk_norm_rope_store_fp4(nvc_ctx* ctx, nvc_bf16* qkv, int ld, const nvc_bf16* qw, const nvc_bf16* kw, float eps, const float* cos_sin, int max_pos,
+                               const int32_t* positions, const int32_t* slot_mapping, const nvc_fp4_cache* cache, nvc_bf16* q_out, int ldqo, int N, int nh,
+                               void* stream);
+/* nvc_store_kvcache with such a cache: rows of kv * 128 numbers as they are, each side with its stride. */
+int nvc_store_kvcache_fp4(nvc_ctx* ctx, const nvc_bf16* k, int ldk, const nvc_bf16* v, int ldv, const nvc_fp4_cache* cache, const int32_t* slot_mapping, int N,
+                          void* stream);
+/* Rows back: k, v [N, kv, 128] the codes as e4m3 numbers, k_scale, v_scale [N, kv, 8] their scales in bf16 (both exact).  A slot that is not in the cache: zeros. */
+int nvc_read_kvcache_fp4(nvc_ctx* ctx, const nvc_fp4_cache* cache, const int32_t* slots, nvc_fp8* k, nvc_bf16* k_scale, nvc_fp8* v, nvc_bf16* v_scale, int N,
+                         void* stream);
+/* nvc_paged_decode_attn over such a cache.  q [B, nh * 128] stride ldq; block_tables [B, bt_stride]; out [B, nh * 128] stride ldo (multiples of 8).  A context of length 0 (or
+ * less) gives zeros; a length beyond the table's bt_stride * block_size counts as that; a block outside the pool reads as rows of zeros.  Rows past a context
+ * may hold anything.  The weights of a row's keys are rounded to fp16 for the second product (2^-11 of each).  workspace: nvc_attn_fp4_workspace_bytes, of this call alone
+ * while it runs; nothing in it has to be cleared.
+ * A row's sums are grouped by what the whole batch holds: a call repeats itself bit by bit, a sequence beside others may differ in rounding. */
+size_t nvc_attn_fp4_workspace_bytes(const nvc_ctx* ctx, int nh, int kv);
+int nvc_paged_decode_attn_fp4(nvc_ctx* ctx, const nvc_bf16* q, int ldq, const nvc_fp4_cache* cache, const int32_t* block_tables, int bt_stride,
+                              const int32_t* context_lens, int B, int nh, float scale, nvc_bf16* out, int ldo, void* workspace, size_t workspace_bytes, void* stream);
+/* nvc_prefill_attn_paged over such a cache: q row i of sequence b (rows cu_seqlens_q[b] .. cu_seqlens_q[b + 1], ascending from 0) is position context_lens[b] - q_len_b + i and
+ * sees the keys up to itself, none where that is negative (zeros).  max_seqlen_q: at least the longest q_len.  Rows behind cu_seqlens_q[B] are left as they are. */
+int nvc_prefill_attn_paged_fp4(nvc_ctx* ctx, const nvc_bf16* q, int ldq, const nvc_fp4_cache* cache, const int32_t* block_tables, int bt_stride,
+                               const int32_t* context_lens, const int32_t* cu_seqlens_q, int B, int total_q_tokens, int max_seqlen_q, int nh, float scale,
+                               nvc_bf16* out, int ldo, void* workspace, size_t workspace_bytes, void* stream);
+
 /* K8. Replaces Qwen3ModelRunner::argmax (src/engine/llm_engine.rs:135-142) on device:
  * idx[b] = LAST index of the maximum of logits[b, :] (Iterator::max_by tie rule);
  * val[b] = that maximum.  idx is offset by `index_offset` (TP vocab shard). */

@@ -155,6 +155,11 @@ def _declare(l: C.CDLL) -> None:
         "nvc_gemm_fp8": [_vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp],
         "nvc_gemm_fp8_ex": [_vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp],
         "nvc_gemm_fp8_grouped": [_vp, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _i, _i, _vp],
+        "nvc_qk_norm_rope_store_fp4": [_vp, _vp, _i, _vp, _vp, _f, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _vp],
+        "nvc_store_kvcache_fp4": [_vp, _vp, _i, _vp, _i, _vp, _vp, _i, _vp],
+        "nvc_read_kvcache_fp4": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp],
+        "nvc_paged_decode_attn_fp4": [_vp, _vp, _i, _vp, _vp, _i, _vp, _i, _i, _f, _vp, _i, _vp, _sz, _vp],
+        "nvc_prefill_attn_paged_fp4": [_vp, _vp, _i, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _f, _vp, _i, _vp, _sz, _vp],
         "nvc_debug_set": [_i, _i],
     }
     for name, args in sigs.items():
@@ -175,6 +180,8 @@ def _declare(l: C.CDLL) -> None:
     l.nvc_ctx_nvls_status.argtypes = [_vp]
     l.nvc_paged_decode_workspace_bytes.restype = _sz
     l.nvc_paged_decode_workspace_bytes.argtypes = [_i, _i, _i, _i]
+    l.nvc_attn_fp4_workspace_bytes.restype = _sz
+    l.nvc_attn_fp4_workspace_bytes.argtypes = [_vp, _i, _i]
     l.nvc_paged_decode_static_scratch_bytes.restype = _sz
     l.nvc_paged_decode_static_scratch_bytes.argtypes = []
     from . import _engine_sigs

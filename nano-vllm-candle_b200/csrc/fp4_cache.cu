@@ -1,0 +1,195 @@
+// Rows into the 4-bit cache, and back.  nvc_qk_norm_rope_store_fp4 is nvc_qk_norm_rope_store with a cache in 4 bits: q / k RMSNorm, RoPE and the scatter in
+// one pass over the QKV rows (src/models/qwen3.rs:206-234); nvc_store_kvcache_fp4 scatters rows that are ready; nvc_read_kvcache_fp4 gives rows back.
+#include "fp4.cuh"
+#include "internal.h"
+
+namespace {
+
+struct StoreArgs {
+  const nvc_bf16 *q, *k, *v;            // heads' rows: q may be absent (nh = 0)
+  int64_t ldq, ldk, ldv;
+  nvc_bf16 *q_out, *k_out;              // k_out may be null
+  int64_t ldqo, ldko;
+  uint8_t *kc, *ks, *vc, *vs;
+  int kv, block_size, slots;            // slots: of the cache
+  const float4* table;                  // null: rows are stored as they are
+  int max_pos;
+  const uint4 *qw, *kw;                 // null: no norm
+  const int32_t *positions, *slot_mapping;
+  float eps;
+  int N, nh;
+};
+
+// 8 lanes per (token, head): lane l owns the numbers [8l, 8l + 8) and [64 + 8l, 64 + 8l + 8), so that a rotation's pairs are one lane's and a block of 16 is two
+// neighbouring lanes'.  Memory-bound: per token (nh + 2 kv) * 256 bytes in, nh * 256 (and kv * 256 in place) + kv * 144 out.
+__global__ void __launch_bounds__(256) store_fp4_kernel(const StoreArgs p) {
+  pdl_trigger();
+  const int units = p.nh + 2 * p.kv;
+  const int64_t unit = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 3;
+  const int l = threadIdx.x & 7;
+  const unsigned mask = 0xffu << ((threadIdx.x & 31) & ~7);
+  pdl_wait();
+  if (unit >= (int64_t)p.N * units) return;
+  const int n = (int)(unit / units), u = (int)(unit - (int64_t)n * units);
+  const bool is_q = u < p.nh, is_v = u >= p.nh + p.kv;
+  const int h = is_q ? u : is_v ? u - p.nh - p.kv : u - p.nh;
+  const nvc_bf16* src = is_q ? p.q + n * p.ldq : is_v ? p.v + n * p.ldv : p.k + n * p.ldk;
+  const uint4* row = reinterpret_cast<const uint4*>(src + (int64_t)h * 128);
+  uint4 a = ld_once_u4(row + l), b = ld_once_u4(row + l + 8);
+  if (!is_v && p.table) {
+    const int pos = p.positions[n];
+    float4 c0, c1, s0, s1;
+    if ((unsigned)pos < (unsigned)p.max_pos) {
+      const float4* cs = p.table + (int64_t)pos * 32;                        // cos[64], sin[64]
+      c0 = cs[2 * l]; c1 = cs[2 * l + 1]; s0 = cs[16 + 2 * l]; s1 = cs[16 + 2 * l + 1];
+    } else {                                                                  // a position that the table does not have: rows of NaN
+      const float bad = __uint_as_float(0x7fffffffu);
+      c0 = c1 = s0 = s1 = make_float4(bad, bad, bad, bad);
+    }
+    const uint4* w = is_q ? p.qw : p.kw;
+    uint4 w_lo = make_uint4(0, 0, 0, 0), w_hi = w_lo;
+    if (w) { w_lo = w[l]; w_hi = w[l + 8]; }
+    uint4 o1, o2;
+    qk_norm_rope8(a, b, mask, w != nullptr, w_lo, w_hi, p.eps, c0, c1, s0, s1, o1, o2);
+    a = o1;
+    b = o2;
+    nvc_bf16* out = is_q ? p.q_out + n * p.ldqo : p.k_out ? p.k_out + n * p.ldko : nullptr;
+    if (out) {
+      uint4* o = reinterpret_cast<uint4*>(out + (int64_t)h * 128);
+      o[l] = a;
+      o[l + 8] = b;
+    }
+  }
+  if (is_q) return;
+  const int slot = p.slot_mapping[n];
+  uint32_t ma = fp4_amax8(a), mb = fp4_amax8(b);
+  ma = max(ma, __shfl_xor_sync(mask, ma, 1));
+  mb = max(mb, __shfl_xor_sync(mask, mb, 1));
+  if ((unsigned)slot >= (unsigned)p.slots) return;
+  const uint32_t sa = fp4_scale_byte(ma), sb = fp4_scale_byte(mb);
+  const int block = slot / p.block_size;
+  const int64_t at = ((int64_t)block * p.kv + h) * p.block_size + (slot - block * p.block_size);
+  uint32_t* codes = reinterpret_cast<uint32_t*>((is_v ? p.vc : p.kc) + at * kFp4Codes);
+  uint8_t* scales = (is_v ? p.vs : p.ks) + at * kFp4Scales;
+  codes[l] = sa == 255u ? 0u : fp4_codes8(a, fp4_inverse(sa));
+  codes[l + 8] = sb == 255u ? 0u : fp4_codes8(b, fp4_inverse(sb));
+  if (!(l & 1)) {
+    scales[l >> 1] = (uint8_t)sa;
+    scales[4 + (l >> 1)] = (uint8_t)sb;
+  }
+}
+
+// 8 lanes per (row, head, side), 16 numbers a lane
+__global__ void __launch_bounds__(256)
+read_fp4_kernel(const uint8_t* kc, const uint8_t* ks, const uint8_t* vc, const uint8_t* vs, int kv, int block_size, int slots, const int32_t* slot_list, uint4* k, nvc_bf16* k_scale,
+                uint4* v, nvc_bf16* v_scale, int N) {
+  pdl_trigger();
+  const int64_t unit = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 3;
+  const int l = threadIdx.x & 7;
+  pdl_wait();
+  if (unit >= (int64_t)N * 2 * kv) return;
+  const int n = (int)(unit / (2 * kv)), u = (int)(unit - (int64_t)n * 2 * kv);
+  const bool is_v = u >= kv;
+  const int h = is_v ? u - kv : u;
+  const int slot = slot_list[n];
+  uint2 codes = make_uint2(0, 0);
+  uint32_t byte = 0;
+  if ((unsigned)slot < (unsigned)slots) {
+    const int block = slot / block_size;
+    const int64_t at = ((int64_t)block * kv + h) * block_size + (slot - block * block_size);
+    codes = reinterpret_cast<const uint2*>((is_v ? vc : kc) + at * kFp4Codes)[l];
+    byte = ((is_v ? vs : ks) + at * kFp4Scales)[l];
+  }
+  // four codes -> four e4m3 bytes: the magnitudes 0, 0.5, 1, 1.5 and 2, 3, 4, 6 by their place, then the signs
+  auto e4m3 = [](uint32_t c) {
+    const uint32_t sign = c & 0x8888u;
+    const uint32_t s = ((sign & 0x8u) << 4) | ((sign & 0x80u) << 8) | ((sign & 0x800u) << 12) | ((sign & 0x8000u) << 16);
+    return __byte_perm(0x3c383000u, 0x4c484440u, c & 0x7777u) | s;
+  };
+  const int64_t to = (int64_t)n * kv + h;
+  (is_v ? v : k)[to * 8 + l] = make_uint4(e4m3(codes.x), e4m3(codes.x >> 16), e4m3(codes.y), e4m3(codes.y >> 16));
+  (is_v ? v_scale : k_scale)[to * 8 + l] = __bfloat16_as_ushort(__float2bfloat16_rn(fp4_scale(byte)));
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+int launch_store(nvc_ctx* ctx, const StoreArgs& p, void* stream) {
+  const int64_t blocks = ((int64_t)p.N * (p.nh + 2 * p.kv) * 8 + 255) / 256;
+  NVC_REQUIRE(ctx, blocks <= 0x7fffffffLL, NVC_ESHAPE, "too many rows");
+  DeviceGuard guard(ctx->device);
+  NVC_CUDA_CHECK(ctx, nvc_launch(ctx, store_fp4_kernel, dim3((unsigned)blocks), dim3(256), 0, nvc_stream(stream), p));
+  NVC_CUDA_CHECK(ctx, cudaGetLastError());
+  ctx->launches++;
+  return NVC_OK;
+}
+
+}  // namespace
+
+int nvc_fp4_cache_check(nvc_ctx* ctx, const nvc_fp4_cache* c) {
+  NVC_REQUIRE(ctx, ctx && c && c->k && c->k_scale && c->v && c->v_scale, NVC_EINVAL, "null pointer");
+  NVC_REQUIRE(ctx, c->num_blocks > 0 && c->kv > 0 && c->block_size > 0, NVC_EINVAL, "bad sizes of the cache");
+  NVC_REQUIRE(ctx, c->block_size % 16 == 0, NVC_ESHAPE, "block_size must be a multiple of 16");
+  NVC_REQUIRE(ctx, (int64_t)c->num_blocks * c->block_size <= 0x7fffffffLL, NVC_ESHAPE, "a cache has at most 2^31 - 1 slots");
+  NVC_REQUIRE(ctx, aligned16(c->k) && aligned16(c->k_scale) && aligned16(c->v) && aligned16(c->v_scale), NVC_EINVAL, "the cache's parts must be 16-byte aligned");
+  return NVC_OK;
+}
+
+extern "C" int nvc_qk_norm_rope_store_fp4(nvc_ctx* ctx, nvc_bf16* qkv, int ld, const nvc_bf16* qw, const nvc_bf16* kw, float eps, const float* cos_sin, int max_pos,
+                                          const int32_t* positions, const int32_t* slot_mapping, const nvc_fp4_cache* cache, nvc_bf16* q_out, int ldqo, int N, int nh, void* stream) {
+  if (const int rc = nvc_fp4_cache_check(ctx, cache)) return rc;
+  const int kv = cache->kv;
+  NVC_REQUIRE(ctx, qkv && cos_sin && positions && slot_mapping, NVC_EINVAL, "null pointer");
+  NVC_REQUIRE(ctx, (qw == nullptr) == (kw == nullptr), NVC_EINVAL, "q/k norm weights must both be given or both be NULL");
+  NVC_REQUIRE(ctx, N >= 0 && nh > 0 && max_pos > 0 && nh <= 0xffffff && kv <= 0xffffff, NVC_EINVAL, "bad sizes");
+  NVC_REQUIRE(ctx, ld >= ((int64_t)nh + 2 * kv) * 128 && ld % 8 == 0 && (!q_out || (ldqo >= (int64_t)nh * 128 && ldqo % 8 == 0)), NVC_ESHAPE,
+              "row strides must cover the heads and be multiples of 8");
+  NVC_REQUIRE(ctx, aligned16(qkv) && aligned16(qw) && aligned16(kw) && aligned16(cos_sin) && aligned16(q_out), NVC_EINVAL, "pointers must be 16-byte aligned");
+  if (N == 0) return NVC_OK;
+  StoreArgs p{};
+  p.q = qkv; p.k = qkv + (int64_t)nh * 128; p.v = qkv + ((int64_t)nh + kv) * 128;
+  p.ldq = p.ldk = p.ldv = ld;
+  p.q_out = q_out ? q_out : qkv;
+  p.ldqo = q_out ? ldqo : ld;
+  p.k_out = q_out ? nullptr : qkv + (int64_t)nh * 128;
+  p.ldko = ld;
+  p.kc = cache->k; p.ks = cache->k_scale; p.vc = cache->v; p.vs = cache->v_scale;
+  p.kv = kv; p.block_size = cache->block_size; p.slots = cache->num_blocks * cache->block_size;
+  p.table = reinterpret_cast<const float4*>(cos_sin); p.max_pos = max_pos;
+  p.qw = reinterpret_cast<const uint4*>(qw); p.kw = reinterpret_cast<const uint4*>(kw);
+  p.positions = positions; p.slot_mapping = slot_mapping; p.eps = eps; p.N = N; p.nh = nh;
+  return launch_store(ctx, p, stream);
+}
+
+extern "C" int nvc_store_kvcache_fp4(nvc_ctx* ctx, const nvc_bf16* k, int ldk, const nvc_bf16* v, int ldv, const nvc_fp4_cache* cache, const int32_t* slot_mapping, int N,
+                                     void* stream) {
+  if (const int rc = nvc_fp4_cache_check(ctx, cache)) return rc;
+  NVC_REQUIRE(ctx, k && v && slot_mapping, NVC_EINVAL, "null pointer");
+  NVC_REQUIRE(ctx, N >= 0 && cache->kv <= 0xffffff, NVC_EINVAL, "bad sizes");
+  NVC_REQUIRE(ctx, ldk >= (int64_t)cache->kv * 128 && ldv >= (int64_t)cache->kv * 128 && ldk % 8 == 0 && ldv % 8 == 0, NVC_ESHAPE,
+              "row strides must cover the heads and be multiples of 8");
+  NVC_REQUIRE(ctx, aligned16(k) && aligned16(v), NVC_EINVAL, "pointers must be 16-byte aligned");
+  if (N == 0) return NVC_OK;
+  StoreArgs p{};
+  p.k = k; p.v = v; p.ldk = ldk; p.ldv = ldv;
+  p.kc = cache->k; p.ks = cache->k_scale; p.vc = cache->v; p.vs = cache->v_scale;
+  p.kv = cache->kv; p.block_size = cache->block_size; p.slots = cache->num_blocks * cache->block_size;
+  p.slot_mapping = slot_mapping; p.N = N;
+  return launch_store(ctx, p, stream);
+}
+
+extern "C" int nvc_read_kvcache_fp4(nvc_ctx* ctx, const nvc_fp4_cache* cache, const int32_t* slots, nvc_fp8* k, nvc_bf16* k_scale, nvc_fp8* v, nvc_bf16* v_scale, int N,
+                                    void* stream) {
+  if (const int rc = nvc_fp4_cache_check(ctx, cache)) return rc;
+  NVC_REQUIRE(ctx, slots && k && k_scale && v && v_scale, NVC_EINVAL, "null pointer");
+  NVC_REQUIRE(ctx, N >= 0 && cache->kv <= 0xffffff, NVC_EINVAL, "bad sizes");
+  NVC_REQUIRE(ctx, aligned16(k) && aligned16(v), NVC_EINVAL, "pointers must be 16-byte aligned");
+  if (N == 0) return NVC_OK;
+  const int64_t blocks = ((int64_t)N * 2 * cache->kv * 8 + 255) / 256;
+  NVC_REQUIRE(ctx, blocks <= 0x7fffffffLL, NVC_ESHAPE, "too many rows");
+  DeviceGuard guard(ctx->device);
+  NVC_CUDA_CHECK(ctx, nvc_launch(ctx, read_fp4_kernel, dim3((unsigned)blocks), dim3(256), 0, nvc_stream(stream), cache->k, cache->k_scale, cache->v, cache->v_scale, cache->kv,
+                                 cache->block_size, cache->num_blocks * cache->block_size, slots, reinterpret_cast<uint4*>(k), k_scale, reinterpret_cast<uint4*>(v), v_scale, N));
+  NVC_CUDA_CHECK(ctx, cudaGetLastError());
+  ctx->launches++;
+  return NVC_OK;
+}

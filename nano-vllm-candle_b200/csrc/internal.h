@@ -41,6 +41,8 @@ int nvc_gemm_fp8_ex(nvc_ctx* ctx, const uint8_t* A, int lda, const float* a_scal
 int nvc_prefill_attn_init(nvc_ctx* ctx);
 int nvc_paged_decode_init(nvc_ctx* ctx);
 }
+// the pointers and sizes of a 4-bit cache
+int nvc_fp4_cache_check(nvc_ctx* ctx, const nvc_fp4_cache* cache);
 // nvc_attn_paged_wide with its tcgen05 route for prompt portions on or off (the switch of a model's body)
 int nvc_attn_paged_wide_on(nvc_ctx* ctx, const void* q, int ldq, const void* k_cache, int ldk, const void* v_cache, int ldv, const int32_t* block_tables, int bt_stride,
                            const int32_t* context_lens, const int32_t* cu_seqlens, int B, int rows, int max_qlen, int block_size, const nvc_attn_spec* spec, void* out,
