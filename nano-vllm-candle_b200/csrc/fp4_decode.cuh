@@ -7,42 +7,45 @@
 // bytes of a V row are 16 neighbouring dims of the result.  V's fragments pair two tokens in a register: their codes are put side by side before they are decoded (4 logical
 // instructions for 16 numbers).  P goes from accumulator to operand through movmatrix.
 //
-// A warp is alone with a ring of four tiles of 16 tokens in shared memory (cp.async, 2 304 bytes a tile).  The scales of rows behind the context, and of pages outside the pool, arrive as
-// zeros, so that whatever their codes are counts for nothing.
+// A warp is alone with a ring of two tiles of 32 tokens in shared memory, filled by bulk copies of a page's rows (4 608 bytes a tile).  The rows of a tile (of 16 tokens each time) are the
+// products' rows in an order in which neither the reads of K nor those of V meet in a bank more than twice.
 //
 // Work is cut by what the device finds in the lengths: all tiles of all (sequence, key head, columns) units, one behind another, in equal stretches, one for each warp of a grid that fills the
-// GPU once.  A unit inside a warp's stretch is written by it; the pieces of others are joined in shared memory where the warps are of one CTA, and by a second kernel (combine) where not.
-// Contexts of any mixture of lengths thus take the time of their sum.
+// GPU once; a unit counts as kUnitCost tiles more than it has, for its queries and its result.  A unit inside a warp's stretch is written by it; the pieces of others are joined in shared memory
+// where the warps are of one CTA, and by a second kernel (combine) where not.  Contexts of any mixture of lengths thus take the time of their sum.
 //
 // The exponentials are taken against a reference that follows a column's maximum only when that grew by more than 2^8 (a vote; nothing is exchanged otherwise), shifted by 2^7: weights lie
 // below 2^15, inside fp16, and those down to 2^-31 of the largest are kept.  Queries are brought to fp16 behind a power of two of their own, that the score's factor takes back.
 #pragma once
 #include "fp4.cuh"
+#include "ptx.cuh"
 
 namespace fp4d {
 
-constexpr int kTile = 16, kStages = 4, kWarps = 4;
-constexpr int kStageBytes = 2 * kTile * (kFp4Codes + kFp4Scales);      // K codes, V codes, K scales, V scales
+constexpr int kTile = 32, kHalf = 16, kStages = 2, kWarps = 4;
+constexpr int kAtV = kTile * kFp4Codes, kAtKs = 2 * kAtV, kAtVs = kAtKs + kTile * kFp4Scales;      // of a stage: K codes, V codes, K scales, V scales
+constexpr int kStageBytes = kAtVs + kTile * kFp4Scales;
 constexpr int kRingBytes = kStages * kStageBytes;
-constexpr float kFloor = -3.0e38f;                                     // reference of a column that has seen nothing
+constexpr float kFloor = -3.0e38f;                                     // a piece's reference for a column that saw nothing in it
 constexpr float kShift = 7.0f, kMost = 15.0f;
-constexpr int kMinTiles = 2;                                           // of a warp's stretch
+constexpr int kUnitCost = 2;
 
 struct Args {
   const nvc_bf16* q;
   nvc_bf16* out;
   int64_t ldq, ldo;
   const uint8_t *kc, *ks, *vc, *vs;
-  const int32_t *tables, *lens, *cu;                                   // cu null: one row of each sequence
+  const int32_t *block_tables, *context_lens, *cu_seqlens;             // cu_seqlens null: one row of each sequence
   int bt_stride, num_blocks, kv, block_size, B, group, rows;
   float scale_log2e;
+  int4* notes;                                                         // of each CTA, what begins there and ends in another: sequence (-1: nothing), unit, last CTA
   float* parts;                                                        // two records of each CTA
   int warps;                                                           // of the attention kernel's grid
 };
 
 template <int NT> constexpr int kCols = 8 * NT;
 template <int NT> constexpr int kRecord = kCols<NT> * 130;             // floats: O [cols][128], reference [cols], sum [cols]
-template <int NT> constexpr int kWarpBytes = kRingBytes + kRecord<NT> * 4;     // the last piece goes where the ring was
+template <int NT> constexpr int kWarpBytes = kRingBytes + kRecord<NT> * 4;     // a stretch's last piece goes where the ring was
 template <int NT> constexpr int kSmem = kWarps * kWarpBytes<NT>;
 static_assert(kRecord<2> * 4 <= kRingBytes, "a record fits where the ring was");
 
@@ -51,12 +54,9 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
 __device__ __forceinline__ void mma(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
@@ -93,6 +93,13 @@ __device__ __forceinline__ uint32_t lds8(uint32_t a) {
   asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(a));
   return v;
 }
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+// The copies that the barrier counts are of memory of this GPU, so that it always completes
+__device__ __forceinline__ void wait_bar(uint32_t bar, uint32_t parity) {
+  uint32_t spins = 0;
+  while (!ptx::mbar_try_wait(bar, parity))
+    if (++spins > (1u << 23)) __trap();
+}
 
 // A sequence's share of the work: `units` (key head, columns) units of `tiles` tiles.
 struct Seq { int len, qlen, tiles, units; };
@@ -100,172 +107,237 @@ template <int NT>
 __device__ __forceinline__ Seq seq_of(const Args& p, int b) {
   Seq s;
   const int64_t room = (int64_t)p.bt_stride * p.block_size;
-  s.len = (int)min((int64_t)max(p.lens[b], 0), room);
-  s.qlen = p.cu ? max(p.cu[b + 1] - p.cu[b], 0) : 1;
+  s.len = (int)min((int64_t)max(p.context_lens[b], 0), room);
+  s.qlen = p.cu_seqlens ? max(p.cu_seqlens[b + 1] - p.cu_seqlens[b], 0) : 1;
   s.tiles = s.len / kTile + (s.len % kTile != 0);
   s.units = p.kv * ((s.qlen * p.group + kCols<NT> - 1) / kCols<NT>);
   return s;
 }
-// All tiles, the same in every lane
+__device__ __forceinline__ int64_t weight(const Seq& s) { return s.tiles ? (int64_t)s.units * (s.tiles + kUnitCost) : 0; }
+
+// The list, summed: a lane has the sequences [lane * m, lane * m + m)
+struct List { int m; int64_t upto, total; };            // upto: this lane's last sequence included
 template <int NT>
-__device__ __forceinline__ int64_t total_tiles(const Args& p, int lane) {
-  int64_t sum = 0;
-  for (int b = lane; b < p.B; b += 32) {
-    const Seq s = seq_of<NT>(p, b);
-    sum += (int64_t)s.units * s.tiles;
+__device__ __forceinline__ List list_of(const Args& p, int lane) {
+  List x;
+  x.m = (p.B + 31) / 32;
+  x.upto = 0;
+  for (int i = 0; i < x.m; ++i) {
+    const int b = lane * x.m + i;
+    if (b < p.B) x.upto += weight(seq_of<NT>(p, b));
   }
 #pragma unroll
-  for (int w = 1; w < 32; w <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-  return sum;
-}
-__device__ __forceinline__ int64_t stretch(const Args& p, int64_t total) {
-  const int64_t per = (total + p.warps - 1) / p.warps;
-  return per < kMinTiles ? kMinTiles : per;
+  for (int w = 1; w < 32; w <<= 1) {
+    const int64_t up = __shfl_up_sync(0xffffffffu, x.upto, w);
+    if (lane >= w) x.upto += up;
+  }
+  x.total = __shfl_sync(0xffffffffu, x.upto, 31);
+  return x;
 }
 
-// A place in the list of tiles: tile t of unit u of sequence b
-struct Place {
-  int b, u, t;
+// A warp's pieces, one behind another: tiles [t, end) of unit u of sequence b.  `rest`: what the stretch still has behind the unit's begin.
+struct Piece {
+  int b, u, t, end;
+  int64_t rest;
   Seq s;
+  __device__ __forceinline__ bool cut(int64_t into) {   // the unit's tiles from weight `into` of it on, as far as the stretch goes; false: none
+    t = (int)max((int64_t)0, into - kUnitCost);
+    end = (int)min((int64_t)s.tiles, rest - kUnitCost);
+    return end > t;
+  }
 };
 template <int NT>
-__device__ __forceinline__ Place find(const Args& p, int64_t at, int lane) {      // at < all tiles
-  int64_t before = 0;
-  for (int b0 = 0;; b0 += 32) {
-    int64_t mine = 0;
-    if (b0 + lane < p.B) {
-      const Seq s = seq_of<NT>(p, b0 + lane);
-      mine = (int64_t)s.units * s.tiles;
-    }
-    int64_t up = mine;
-#pragma unroll
-    for (int w = 1; w < 32; w <<= 1) {
-      const int64_t x = __shfl_up_sync(0xffffffffu, up, w);
-      if (lane >= w) up += x;
-    }
-    const unsigned behind = __ballot_sync(0xffffffffu, before + up > at);
-    if (behind) {
-      const int f = __ffs(behind) - 1;
-      const int64_t start = before + __shfl_sync(0xffffffffu, up - mine, f);
-      Place x;
-      x.b = b0 + f;
-      x.s = seq_of<NT>(p, x.b);
-      x.u = (int)((at - start) / x.s.tiles);
-      x.t = (int)(at - start - (int64_t)x.u * x.s.tiles);
-      return x;
-    }
-    before += __shfl_sync(0xffffffffu, up, 31);
+__device__ __forceinline__ bool first_piece(const Args& p, const List& list, int64_t at, int64_t per, int lane, Piece& x) {
+  if (at >= list.total) return false;
+  const int f = __ffs(__ballot_sync(0xffffffffu, list.upto > at)) - 1;
+  const int64_t before = __shfl_sync(0xffffffffu, list.upto, max(f - 1, 0));
+  at -= f ? before : 0;
+  for (x.b = f * list.m;; ++x.b) {
+    x.s = seq_of<NT>(p, x.b);
+    const int64_t w = weight(x.s);
+    if (at < w) break;
+    at -= w;
   }
+  const int unit = x.s.tiles + kUnitCost;
+  x.u = (int)(at / unit);
+  at -= (int64_t)x.u * unit;
+  x.rest = at + per;
+  return x.cut(at);
 }
 template <int NT>
-__device__ __forceinline__ void next_unit(const Args& p, Place& x) {
-  x.t = 0;
-  if (++x.u < x.s.units) return;
-  x.u = 0;
-  do {
-    if (++x.b >= p.B) return;
-    x.s = seq_of<NT>(p, x.b);
-  } while (x.s.units == 0 || x.s.tiles == 0);
+__device__ __forceinline__ bool next_piece(const Args& p, Piece& x) {
+  x.rest -= x.s.tiles + kUnitCost;
+  if (x.rest <= kUnitCost) return false;
+  if (++x.u == x.s.units) {
+    x.u = 0;
+    do {
+      if (++x.b >= p.B) return false;
+      x.s = seq_of<NT>(p, x.b);
+    } while (x.s.units == 0 || x.s.tiles == 0);
+  }
+  return x.cut(0);
 }
 
 // Column c of a unit: which row, which head, and how many keys it sees; false: none
 template <int NT>
 __device__ __forceinline__ bool column(const Args& p, const Seq& s, int b, int u, int c, int& row, int& head, int& seen) {
-  const int chunks = s.units / p.kv, kvh = u / chunks, r = (u - kvh * chunks) * kCols<NT> + c;
-  const int i = r / p.group;
+  const int chunks = p.kv == s.units ? 1 : s.units / p.kv, kvh = chunks == 1 ? u : u / chunks, r = (u - kvh * chunks) * kCols<NT> + c;
+  int i = 0;
+  row = b;
+  if (p.cu_seqlens) {
+    i = r / p.group;
+    row = p.cu_seqlens[b] + i;
+  }
   head = kvh * p.group + (r - i * p.group);
-  row = p.cu ? p.cu[b] + i : b;
   seen = s.len - s.qlen + i + 1;
-  return i < s.qlen && (unsigned)row < (unsigned)p.rows;
+  return (p.cu_seqlens ? i < s.qlen : r < p.group) && (unsigned)row < (unsigned)p.rows;
 }
 
 template <int NT>
 __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 3) attn_kernel(const Args p) {
   pdl_trigger();
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int4 notes[kWarps][2];                   // of a piece: sequence (-1: no piece), unit, whether it begins and ends its unit
+  __shared__ __align__(8) uint64_t bars[kWarps][kStages];
+  __shared__ int4 pieces[kWarps][2];                  // sequence (-1: no piece), unit, first tile, tile behind the last
+  __shared__ int tiles_of[kWarps][2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  if (lane < 2) notes[warp][lane] = make_int4(-1, 0, 0, 0);
-  pdl_wait();
-  const int64_t total = total_tiles<NT>(p, lane), per = stretch(p, total);
-  const int64_t first = per * (blockIdx.x * kWarps + warp);
-  if (per * blockIdx.x * kWarps >= total) return;                             // the whole CTA
-  const int n = (int)max((int64_t)0, min(per, total - first));
+  if (lane < 2) pieces[warp][lane] = make_int4(-1, 0, 0, 0);
+  const uint32_t bar = smem_u32(&bars[warp][0]);
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) ptx::mbar_init(bar + 8 * i, 1);
+    ptx::fence_barrier_init();
+  }
+  __syncwarp();
+  const List list = list_of<NT>(p, lane);
+  const int64_t per = max((list.total + p.warps - 1) / p.warps, (int64_t)1 + kUnitCost);
   uint8_t* const mine = smem + warp * kWarpBytes<NT>;
   const uint32_t ring = smem_u32(mine);
+  Piece at;
+  bool any = first_piece<NT>(p, list, per * (blockIdx.x * kWarps + warp), per, lane, at);
 
-  if (n > 0) {
-    Place at = find<NT>(p, first, lane);
+  // ---- the reading side: a tile ahead.  Lane 0 copies; the others know which rows are not there
+  const int per_page = p.block_size / kHalf, last_page = p.bt_stride - 1;
+  const bool whole = (per_page & 1) == 0;             // a tile lies in one page
+  Piece rd = at;
+  bool rd_any = any;
+  int page = 0, in_page = 0, kvh = 0, blk = 0, next = 0;
+  auto enter = [&] {                                  // to a piece's first tile
+    const int chunks = p.kv == rd.s.units ? 1 : rd.s.units / p.kv;
+    kvh = chunks == 1 ? rd.u : rd.u / chunks;
+    const int32_t* table = p.block_tables + (int64_t)rd.b * p.bt_stride;
+    page = 2 * rd.t / per_page;
+    in_page = 2 * rd.t - page * per_page;
+    blk = table[page];
+    next = table[min(page + 1, last_page)];
+  };
+  if (rd_any) enter();
+  pdl_wait();
 
-    // ---- the reading side: a place of its own, kStages - 1 tiles ahead
-    Place rd = at;
-    int rd_left = n, page = -1, blk = -1;              // page: number whose block `blk` is
-    const int per_page = p.block_size / kTile;
-    int kvh, in_page;
-    auto enter = [&] {                                  // a unit's first tile of this stretch
-      const int chunks = rd.s.units / p.kv;
-      kvh = rd.u / chunks;
-      page = rd.t / per_page;
-      in_page = rd.t - page * per_page;
-      blk = p.tables[(int64_t)rd.b * p.bt_stride + page];
-    };
-    enter();
-    // lane c copies 16-byte chunks c and c + 32 of the 64 of a tile's codes: row c / 4; two rows share 128 bytes, whose eight chunks are permuted so that neither the
-    // reads of K (two rows at once) nor those of V (four rows, 32 bytes of each) meet in a bank
-    const uint32_t to = (uint32_t)((lane >> 3) * 128 + ((((lane >> 2) & 1) * 4 + (lane & 3)) ^ (2 * ((lane >> 3) & 3))) * 16);
-    auto issue = [&](int stage) {
-      if (rd_left > 0) {
-        const bool there = (unsigned)blk < (unsigned)p.num_blocks;
-        const int64_t row = ((int64_t)(there ? blk : 0) * p.kv + kvh) * p.block_size + in_page * kTile;
-        const uint32_t st = ring + stage * kStageBytes;
-        const uint8_t *k = p.kc + row * kFp4Codes + lane * 16, *v = p.vc + row * kFp4Codes + lane * 16;
-        copy16(st + to, k, 16);
-        copy16(st + to + 512, k + 512, 16);
-        copy16(st + 1024 + to, v, 16);
-        copy16(st + 1024 + to + 512, v + 512, 16);
-        if (lane < 16) {                                // two rows' scales; zeros for the ones that are not there
-          const int live = there ? (rd.s.len - rd.t * kTile - 2 * (lane & 7)) * kFp4Scales : 0;
-          copy16(st + 2048 + lane * 16, (lane < 8 ? p.ks : p.vs) + row * kFp4Scales + (lane & 7) * 16, (uint32_t)min(max(live, 0), 16));
-        }
-        --rd_left;
-        if (rd_left > 0) {
-          if (++rd.t == rd.s.tiles) {
-            next_unit<NT>(p, rd);
-            enter();
-          } else if (++in_page == per_page) {
-            in_page = 0;
-            blk = p.tables[(int64_t)rd.b * p.bt_stride + ++page];
-          }
-        }
+  // sequences without a context: zeros
+  for (int b = blockIdx.x * kWarps + warp; b < p.B; b += p.warps) {
+    const Seq s = seq_of<NT>(p, b);
+    if (s.tiles == 0)
+      for (int i = 0; i < s.qlen; ++i) {
+        const int row = p.cu_seqlens ? p.cu_seqlens[b] + i : b;
+        if ((unsigned)row < (unsigned)p.rows)
+          for (int c = lane; c < p.kv * p.group * 16; c += 32) reinterpret_cast<uint4*>(p.out + row * p.ldo)[c] = make_uint4(0, 0, 0, 0);
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) issue(i);
+  }
+  if (per * blockIdx.x * kWarps >= list.total) {      // the whole CTA
+    if (threadIdx.x == 0) p.notes[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    return;
+  }
 
+  // half a tile, or all of it (rows: 16 or 32), of the page that the place is in
+  auto copy = [&](uint32_t st, uint32_t stage_bar, int half, int rows) {
+    const int64_t row = ((int64_t)blk * p.kv + kvh) * p.block_size + in_page * kHalf;
+    ptx::mbar_arrive_expect_tx(stage_bar, rows * 2 * (kFp4Codes + kFp4Scales));
+    ptx::bulk_load(st + half * kHalf * kFp4Codes, p.kc + row * kFp4Codes, rows * kFp4Codes, stage_bar);
+    ptx::bulk_load(st + kAtKs + half * kHalf * kFp4Scales, p.ks + row * kFp4Scales, rows * kFp4Scales, stage_bar);
+    ptx::bulk_load(st + kAtV + half * kHalf * kFp4Codes, p.vc + row * kFp4Codes, rows * kFp4Codes, stage_bar);
+    ptx::bulk_load(st + kAtVs + half * kHalf * kFp4Scales, p.vs + row * kFp4Scales, rows * kFp4Scales, stage_bar);
+  };
+  auto turn = [&] {
+    in_page = 0;
+    ++page;
+    blk = next;
+    next = p.block_tables[(int64_t)rd.b * p.bt_stride + min(page + 1, last_page)];
+  };
+  uint32_t absent = 0;                                // bit 2 * stage + h: half h was not copied
+  auto issue = [&](int stage) {
+    if (!rd_any) return;
+    const uint32_t st = ring + stage * kStageBytes, stage_bar = bar + 8 * stage;
+    uint32_t gone = 0;
+    if (whole) {
+      if (in_page == per_page) turn();
+      if ((unsigned)blk < (unsigned)p.num_blocks) {
+        if (lane == 0) copy(st, stage_bar, 0, kTile);
+      } else {
+        gone = 3;
+        if (lane == 0) ptx::mbar_arrive(stage_bar);
+      }
+      in_page += 2;
+    } else {                                          // a barrier phase takes one arrival: the first half's is without it
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
+        const bool there = rd.t * kTile + h * kHalf < rd.s.len;
+        if (there && in_page == per_page) turn();
+        if (!there || (unsigned)blk >= (unsigned)p.num_blocks) gone |= 1u << h;
+        else if (lane == 0) {
+          const int64_t row = ((int64_t)blk * p.kv + kvh) * p.block_size + in_page * kHalf;
+          asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(stage_bar), "r"(kHalf * 2 * (kFp4Codes + kFp4Scales)) : "memory");
+          ptx::bulk_load(st + h * kHalf * kFp4Codes, p.kc + row * kFp4Codes, kHalf * kFp4Codes, stage_bar);
+          ptx::bulk_load(st + kAtKs + h * kHalf * kFp4Scales, p.ks + row * kFp4Scales, kHalf * kFp4Scales, stage_bar);
+          ptx::bulk_load(st + kAtV + h * kHalf * kFp4Codes, p.vc + row * kFp4Codes, kHalf * kFp4Codes, stage_bar);
+          ptx::bulk_load(st + kAtVs + h * kHalf * kFp4Scales, p.vs + row * kFp4Scales, kHalf * kFp4Scales, stage_bar);
+        }
+        if (there) ++in_page;
+      }
+      if (lane == 0) ptx::mbar_arrive(stage_bar);
+    }
+    absent = (absent & ~(3u << (2 * stage))) | gone << (2 * stage);
+    if (++rd.t == rd.end) {
+      rd_any = next_piece<NT>(p, rd);
+      if (rd_any) {
+        enter();
+        int row, head, seen;                          // its queries, on their way to L2
+        if (!(t & 1) && column<NT>(p, rd.s, rd.b, rd.u, g, row, head, seen)) prefetch_l2(p.q + row * p.ldq + (int64_t)head * 128 + 32 * t);
+      }
+    }
+  };
+
+  if (any) {
     // ---- the computing side
+    uint4 qw[NT][4];
     uint32_t qf[NT][16];
     float o[NT][8][4], ref[NT][2], sum[NT][2], factor[NT][2];
-    int lim[NT][2], least = 0;                          // keys that this thread's columns see, and the unit's column that sees least
-    int begun = 0;                                      // first tile of this piece
-    bool head_piece = true;                             // the stretch's first
+    int lim[NT][2], least = 0;                        // keys that this thread's columns see, and the unit's column that sees least
+    int begun = 0;                                    // first tile of this piece
+    bool head_piece = true;                           // the stretch's first
+    bool fresh = true;                                // no tile of the piece has been looked at: the references are 0, and take the first maximum
+    int limit[NT];                                    // of column g
 
-    auto begin = [&] {
-      begun = at.t;
-      least = 0x7fffffff;
+    auto load_q = [&] {
 #pragma unroll
       for (int x = 0; x < NT; ++x) {
         int row, head, seen;
         const bool real = column<NT>(p, at.s, at.b, at.u, 8 * x + g, row, head, seen);
-        uint4 w[4] = {};
-        if (real) {
-          const uint4* src = reinterpret_cast<const uint4*>(p.q + row * p.ldq + (int64_t)head * 128) + 4 * t;
+        const uint4* src = reinterpret_cast<const uint4*>(p.q + (real ? row * p.ldq + (int64_t)head * 128 : 0)) + 4 * t;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = src[i];
-        }
+        for (int i = 0; i < 4; ++i) qw[x][i] = real ? src[i] : make_uint4(0, 0, 0, 0);
+        limit[x] = real ? seen : 0x7fffffff;
+      }
+    };
+    auto begin = [&] {
+      begun = at.t;
+      fresh = true;
+      least = at.s.len;
+#pragma unroll
+      for (int x = 0; x < NT; ++x) {
         uint32_t top = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) top = max(top, fp4_amax8(w[i]));
+        for (int i = 0; i < 4; ++i) top = max(top, fp4_amax8(qw[x][i]));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
         // 2^-e brings the largest number to [1, 2); a row with an infinity or a NaN, or of zeros, stays as it is.  (2^-e and 2^e are floats for -126 <= e <= 126;
@@ -275,28 +347,27 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 3) attn_kernel(cons
         const float down = __uint_as_float((uint32_t)(127 - e) << 23), back = __uint_as_float((uint32_t)(127 + e) << 23);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint32_t f[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+          const uint32_t f[4] = {qw[x][i].x, qw[x][i].y, qw[x][i].z, qw[x][i].w};
 #pragma unroll
           for (int j = 0; j < 4; ++j) qf[x][4 * i + j] = halves(bf16_lo(f[j]) * down, bf16_hi(f[j]) * down);
         }
-        const int limit = real ? seen : 0x7fffffff;
+        least = min(least, limit[x]);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {                   // columns 2t, 2t + 1 are lanes 8t, 8t + 4's
+        for (int c = 0; c < 2; ++c) {                 // columns 2t, 2t + 1 are lanes 8t, 8t + 4's
           factor[x][c] = __shfl_sync(0xffffffffu, back, 8 * t + 4 * c) * p.scale_log2e;
-          lim[x][c] = __shfl_sync(0xffffffffu, limit, 8 * t + 4 * c);
-          least = min(least, lim[x][c]);
-          ref[x][c] = kFloor;
+          lim[x][c] = min(__shfl_sync(0xffffffffu, limit[x], 8 * t + 4 * c), at.s.len);
+          ref[x][c] = 0.f;
           sum[x][c] = 0.f;
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) o[x][j][0] = o[x][j][1] = o[x][j][2] = o[x][j][3] = 0.f;
       }
-      least = __reduce_min_sync(0xffffffffu, min(least, at.s.len));
+      least = __reduce_min_sync(0xffffffffu, least);
     };
 
     // a unit, or this warp's piece of it, is complete
-    auto end = [&](int ends_at) {
-      const bool begins = begun == 0, ends = ends_at == at.s.tiles;
+    auto end = [&] {
+      const bool begins = begun == 0, ends = at.end == at.s.tiles;
 #pragma unroll
       for (int x = 0; x < NT; ++x)
 #pragma unroll
@@ -319,12 +390,9 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 3) attn_kernel(cons
             dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
           }
       } else {
-        // the stretch's first piece has a place of its own; its last, with nothing left to read, the ring's
-        if (!head_piece) {
-          asm volatile("cp.async.wait_group 0;" ::: "memory");
-          __syncwarp();
-        }
+        // the stretch's first piece has a place of its own; its last, with nothing on its way any more, the ring's
         float* rec = reinterpret_cast<float*>(mine + (head_piece ? kRingBytes : 0));
+        __syncwarp();
 #pragma unroll
         for (int x = 0; x < NT; ++x)
 #pragma unroll
@@ -334,30 +402,52 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 3) attn_kernel(cons
             for (int j = 0; j < 4; ++j)
               reinterpret_cast<float4*>(to)[j] = make_float4(o[x][2 * j][c], o[x][2 * j][c + 2], o[x][2 * j + 1][c], o[x][2 * j + 1][c + 2]);
             if (g == 0) {
-              rec[kCols<NT> * 128 + 8 * x + 2 * t + c] = ref[x][c];
+              rec[kCols<NT> * 128 + 8 * x + 2 * t + c] = sum[x][c] == 0.f ? kFloor : ref[x][c];
               rec[kCols<NT> * 129 + 8 * x + 2 * t + c] = sum[x][c];
             }
           }
-        if (lane == 0) notes[warp][head_piece ? 0 : 1] = make_int4(at.b, at.u, begins, ends);
+        if (lane == 0) {
+          pieces[warp][head_piece ? 0 : 1] = make_int4(at.b, at.u, begun, at.end);
+          tiles_of[warp][head_piece ? 0 : 1] = at.s.tiles;
+        }
       }
       head_piece = false;
     };
 
+    // row r of the products is token r, the two of every second pair exchanged: K's reads (rows g) take both 64-byte halves of 128 at once, and V's (rows 2t) two of each
+    const int rk = g ^ ((g >> 1) & 1), rv = 2 * t + (t & 1);                 // tokens of rows g and 2t; of row 2t + 1: rv ^ 1
+    const uint32_t at_k = (uint32_t)(rk * kFp4Codes + t * 16), at_ks = (uint32_t)(kAtKs + rk * kFp4Scales + 2 * t);
+    const uint32_t at_v = (uint32_t)(kAtV + rv * kFp4Codes + g * 8), at_v1 = (uint32_t)(kAtV + (rv ^ 1) * kFp4Codes + g * 8);
+    const uint32_t at_vs = (uint32_t)(kAtVs + rv * kFp4Scales + g), at_vs1 = (uint32_t)(kAtVs + (rv ^ 1) * kFp4Scales + g);
+    load_q();
+    issue(0);
     begin();
-    for (int i = 0; i < n; ++i) {
-      __syncwarp();                                     // everyone is done with the stage that is filled now
-      issue((i + kStages - 1) % kStages);
-      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
-      __syncwarp();
-      const uint32_t st = ring + (i % kStages) * kStageBytes;
-      // ---- S^T = K Q^T: rows g and g + 8
-      float s[NT][4];
+#pragma unroll 1
+    for (int i = 0;; ++i) {
+      __syncwarp();                                   // everyone is done with the stage that is filled now
+      issue((i + 1) & 1);
+      const uint32_t st = ring + (i & 1) * kStageBytes;
+      wait_bar(bar + 8 * (i & 1), (i >> 1) & 1);
+      const uint32_t gone = (absent >> (2 * (i & 1))) & 3u;
+      if (gone || (at.t + 1) * kTile > at.s.len) {    // rows that are not there: scales of 0, whatever their codes are
+        if ((gone >> (lane >> 4)) & 1 || at.t * kTile + lane >= at.s.len) {
+          asm volatile("st.shared.v2.u32 [%0], {%1, %1};" ::"r"(st + kAtKs + lane * kFp4Scales), "r"(0) : "memory");
+          asm volatile("st.shared.v2.u32 [%0], {%1, %1};" ::"r"(st + kAtVs + lane * kFp4Scales), "r"(0) : "memory");
+        }
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+      }
+      // ---- S^T = K Q^T: of each half, rows g and g + 8
+      float s[NT][2][4];
 #pragma unroll
-      for (int x = 0; x < NT; ++x) s[x][0] = s[x][1] = s[x][2] = s[x][3] = 0.f;
-      {
-        const uint32_t a = st + (g >> 1) * 128 + ((((g & 1) * 4 + t) ^ (2 * ((g >> 1) & 3))) << 4);
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) s[x][h][0] = s[x][h][1] = s[x][h][2] = s[x][h][3] = 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t a = st + h * 1024 + at_k, b = st + h * 128 + at_ks;
         const uint4 lo = lds128(a), hi = lds128(a + 512);
-        const uint32_t slo = lds16(st + 2048 + g * 8 + 2 * t), shi = lds16(st + 2048 + 64 + g * 8 + 2 * t);
+        const uint32_t slo = lds16(b), shi = lds16(b + 64);
         const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
@@ -367,68 +457,76 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 3) attn_kernel(cons
           const uint32_t a1 = mul2(b4.x, fh), a3 = mul2(b4.y, fh), c1 = mul2(b4.z, fh), c3 = mul2(b4.w, fh);
 #pragma unroll
           for (int x = 0; x < NT; ++x) {
-            mma(s[x], a0, a1, a2, a3, qf[x][4 * w], qf[x][4 * w + 1]);
-            mma(s[x], c0, c1, c2, c3, qf[x][4 * w + 2], qf[x][4 * w + 3]);
+            mma(s[x][h], a0, a1, a2, a3, qf[x][4 * w], qf[x][4 * w + 1]);
+            mma(s[x][h], c0, c1, c2, c3, qf[x][4 * w + 2], qf[x][4 * w + 3]);
           }
         }
       }
-      // ---- weights: token g (0, 1) and g + 8 (2, 3), columns 2t and 2t + 1
-      const int tok = at.t * kTile + g;
-      if ((at.t + 1) * kTile > least) {                 // some column does not see the whole tile
-#pragma unroll
-        for (int x = 0; x < NT; ++x)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const int l = min(lim[x][c], at.s.len);
-            // a factor that turns a masked score's sign, or is 0, leaves it masked: the masked score is what comes out of it
-            s[x][c] = tok < l ? s[x][c] * factor[x][c] : -INFINITY;
-            s[x][c + 2] = tok + 8 < l ? s[x][c + 2] * factor[x][c] : -INFINITY;
-          }
-      } else {
-#pragma unroll
-        for (int x = 0; x < NT; ++x)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) s[x][c] *= factor[x][c & 1];
-      }
-      bool grew = false;
+      // ---- exponents: of half h, rows g (0, 1) and g + 8 (2, 3), columns 2t and 2t + 1
 #pragma unroll
       for (int x = 0; x < NT; ++x)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) grew |= s[x][c] - ref[x][c & 1] > kMost;
-      if (__any_sync(0xffffffffu, grew)) {
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) s[x][h][c] = fmaf(s[x][h][c], factor[x][c & 1], -ref[x][c & 1]);
+      if ((at.t + 1) * kTile > least) {               // some column does not see the whole tile
+        const int tok = at.t * kTile + rk;
+#pragma unroll
+        for (int x = 0; x < NT; ++x)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) s[x][h][c] = tok + 16 * h + 4 * (c & 2) < lim[x][c & 1] ? s[x][h][c] : -INFINITY;
+      }
+      float top[NT][2], most = -INFINITY;
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          top[x][c] = fmaxf(fmaxf(s[x][0][c], s[x][0][c + 2]), fmaxf(s[x][1][c], s[x][1][c + 2]));
+          most = fmaxf(most, top[x][c]);
+        }
+      if (fresh || __any_sync(0xffffffffu, most > kMost)) {
 #pragma unroll
         for (int x = 0; x < NT; ++x)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            float top = fmaxf(s[x][c], s[x][c + 2]);
 #pragma unroll
-            for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-            const float now = fmaxf(ref[x][c], top - kShift), a = ex2(ref[x][c] - now);
-            ref[x][c] = now;
+            for (int w = 4; w < 32; w <<= 1) top[x][c] = fmaxf(top[x][c], __shfl_xor_sync(0xffffffffu, top[x][c], w));
+            const float over = top[x][c] - kShift;
+            const float up = fresh ? (over == -INFINITY ? 0.f : over) : fmaxf(0.f, over), a = fresh ? 0.f : ex2(-up);
+            ref[x][c] += up;
             sum[x][c] *= a;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              s[x][h][c] -= up;
+              s[x][h][c + 2] -= up;
+            }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               o[x][j][c] *= a;
               o[x][j][c + 2] *= a;
             }
           }
+        fresh = false;
       }
-      uint32_t pb[NT][2];
+      uint32_t pb[NT][2][2];
 #pragma unroll
-      for (int x = 0; x < NT; ++x) {
-        const float p0 = ex2(s[x][0] - ref[x][0]), p1 = ex2(s[x][1] - ref[x][1]), p2 = ex2(s[x][2] - ref[x][0]), p3 = ex2(s[x][3] - ref[x][1]);
-        sum[x][0] += p0 + p2;
-        sum[x][1] += p1 + p3;
-        pb[x][0] = transpose8(halves(p0, p1));
-        pb[x][1] = transpose8(halves(p2, p3));
-      }
-      // ---- O^T += V^T P^T: dims 16g + 2j (row g) and 16g + 2j + 1 (row g + 8), tokens 2t, 2t + 1, 2t + 8, 2t + 9
-      {
-        const uint32_t base = st + 1024 + t * 128 + (g & 1) * 8, sw = 2 * t;
-        const uint2 ra = lds64(base + (((g >> 1) ^ sw) << 4)), rb = lds64(base + (((4 + (g >> 1)) ^ sw) << 4));
-        const uint2 rc = lds64(base + 512 + (((g >> 1) ^ sw) << 4)), re = lds64(base + 512 + (((4 + (g >> 1)) ^ sw) << 4));
-        const uint32_t sc = st + 2048 + 128 + t * 16 + g;
-        const uint32_t f0 = (lds8(sc) << 7) | (lds8(sc + 8) << 23), f1 = (lds8(sc + 64) << 7) | (lds8(sc + 72) << 23);
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float p0 = ex2(s[x][h][0]), p1 = ex2(s[x][h][1]), p2 = ex2(s[x][h][2]), p3 = ex2(s[x][h][3]);
+          sum[x][0] += p0 + p2;
+          sum[x][1] += p1 + p3;
+          pb[x][h][0] = transpose8(halves(p0, p1));
+          pb[x][h][1] = transpose8(halves(p2, p3));
+        }
+      // ---- O^T += V^T P^T: dims 16g + 2j (row g) and 16g + 2j + 1 (row g + 8); of each half the tokens of rows 2t, 2t + 1, 2t + 8, 2t + 9
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t vb = st + h * 1024, sb = st + h * 128;
+        const uint2 ra = lds64(vb + at_v), rb = lds64(vb + at_v1), rc = lds64(vb + at_v + 512), re = lds64(vb + at_v1 + 512);
+        const uint32_t f0 = (lds8(sb + at_vs) << 7) | (lds8(sb + at_vs1) << 23), f1 = (lds8(sb + at_vs + 64) << 7) | (lds8(sb + at_vs1 + 64) << 23);
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
           const uint32_t xa = w ? ra.y : ra.x, xb = w ? rb.y : rb.x, xc = w ? rc.y : rc.x, xd = w ? re.y : re.x;
@@ -439,62 +537,81 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 3) attn_kernel(cons
           for (int j = 0; j < 4; ++j) {
             const uint32_t m0 = mul2(v0[j], f0), m1 = mul2(v1[j], f0), m2 = mul2(v2[j], f1), m3 = mul2(v3[j], f1);
 #pragma unroll
-            for (int x = 0; x < NT; ++x) mma(o[x][4 * w + j], m0, m1, m2, m3, pb[x][0], pb[x][1]);
+            for (int x = 0; x < NT; ++x) mma(o[x][4 * w + j], m0, m1, m2, m3, pb[x][h][0], pb[x][h][1]);
           }
         }
       }
-      ++at.t;
-      if (at.t == at.s.tiles || i + 1 == n) {
-        end(at.t);
-        if (i + 1 < n) {
-          next_unit<NT>(p, at);
-          begin();
-        }
+      if (++at.t == at.end) {
+        Piece now = at;
+        const bool more = next_piece<NT>(p, now);
+        end();
+        if (!more) break;
+        at = now;
+        load_q();
+        begin();
       }
     }
   }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
 
-  // ---- pieces of one unit, in the CTA's order of tiles: to the result where that is all of it, else to one of the CTA's two records
+  // ---- pieces of one unit, in the CTA's order of tiles: to the result where that is all of it, else to one of the CTA's two records.  16 threads a column, 8 numbers each
   auto record = [&](int i) { return reinterpret_cast<const float*>(smem + (i >> 1) * kWarpBytes<NT> + (i & 1 ? 0 : kRingBytes)); };
-  const int4* note = &notes[0][0];
+  const int4* piece = &pieces[0][0];
+  int4 note = make_int4(-1, 0, 0, 0);
+#pragma unroll 1
   for (int i = 0; i < 2 * kWarps;) {
-    if (note[i].x < 0) {
+    const int4 head_of = piece[i];
+    if (head_of.x < 0) {
       ++i;
       continue;
     }
-    int last = i;
-    for (int j = i + 1; j < 2 * kWarps; ++j)
-      if (note[j].x >= 0) {
-        if (note[j].x != note[i].x || note[j].y != note[i].y) break;
+    int last = i, behind = head_of.w;
+    uint32_t in = 1u << i;
+    for (int j = i + 1; j < 2 * kWarps; ++j) {
+      const int4 x = piece[j];
+      if (x.x >= 0) {
+        if (x.x != head_of.x || x.y != head_of.y) break;
         last = j;
+        behind = x.w;
+        in |= 1u << j;
       }
-    const bool begins = note[i].z, ends = note[last].w;
-    const int b = note[i].x, u = note[i].y;
+    }
+    const int tiles = (&tiles_of[0][0])[i];
+    const bool begins = head_of.z == 0, ends = behind == tiles;
+    if (begins && !ends)                              // it ends in a later CTA: that many stretches of four warps behind this one's end
+      note = make_int4(head_of.x, head_of.y, (int)blockIdx.x + 1 + (int)((tiles - 1 - behind) / (per * kWarps)), 0);
     float* part = p.parts + ((int64_t)blockIdx.x * 2 + (begins ? 1 : 0)) * kRecord<NT>;
-    const Seq s = seq_of<NT>(p, b);
-    for (int c = warp; c < kCols<NT>; c += kWarps) {
-      int row, head, seen;
-      const bool real = column<NT>(p, s, b, u, c, row, head, seen);
+    const int d = (threadIdx.x & 15) * 8;
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+      const int c = 8 * x + (threadIdx.x >> 4);
       float top = kFloor;
-      for (int j = i; j <= last; ++j)
-        if (note[j].x >= 0) top = fmaxf(top, record(j)[kCols<NT> * 128 + c]);
+#pragma unroll
+      for (int j = 0; j < 2 * kWarps; ++j)
+        if (in >> j & 1) top = fmaxf(top, record(j)[kCols<NT> * 128 + c]);
       float l = 0.f;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int j = i; j <= last; ++j)
-        if (note[j].x >= 0) {
-          const float w = ex2(record(j)[kCols<NT> * 128 + c] - top);
-          const float4 x = *reinterpret_cast<const float4*>(record(j) + c * 128 + 4 * lane);
-          l += record(j)[kCols<NT> * 129 + c] * w;
-          v.x += x.x * w; v.y += x.y * w; v.z += x.z * w; v.w += x.w * w;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f), w = v;
+#pragma unroll
+      for (int j = 0; j < 2 * kWarps; ++j)
+        if (in >> j & 1) {
+          const float* r = record(j);
+          const float f = ex2(r[kCols<NT> * 128 + c] - top);
+          const float4 y = *reinterpret_cast<const float4*>(r + c * 128 + d), z = *reinterpret_cast<const float4*>(r + c * 128 + d + 4);
+          l += r[kCols<NT> * 129 + c] * f;
+          v.x += y.x * f; v.y += y.y * f; v.z += y.z * f; v.w += y.w * f;
+          w.x += z.x * f; w.y += z.y * f; w.z += z.z * f; w.w += z.w * f;
         }
       if (begins && ends) {
-        const float inv = l == 0.f ? 0.f : 1.0f / l;
-        if (real) reinterpret_cast<uint2*>(p.out + row * p.ldo + (int64_t)head * 128)[lane] = make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
+        int row, head, seen;
+        if (column<NT>(p, seq_of<NT>(p, head_of.x), head_of.x, head_of.y, c, row, head, seen)) {
+          const float inv = l == 0.f ? 0.f : 1.0f / l;
+          *reinterpret_cast<uint4*>(p.out + row * p.ldo + (int64_t)head * 128 + d) =
+              make_uint4(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv), pack_bf16(w.x * inv, w.y * inv), pack_bf16(w.z * inv, w.w * inv));
+        }
       } else {
-        __stcg(reinterpret_cast<float4*>(part + c * 128) + lane, v);
-        if (lane == 0) {
+        __stcg(reinterpret_cast<float4*>(part + c * 128 + d), v);
+        __stcg(reinterpret_cast<float4*>(part + c * 128 + d + 4), w);
+        if (d == 0) {
           __stcg(part + kCols<NT> * 128 + c, top);
           __stcg(part + kCols<NT> * 129 + c, l);
         }
@@ -502,62 +619,53 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 3) attn_kernel(cons
     }
     i = last + 1;
   }
+  if (threadIdx.x == 0) p.notes[blockIdx.x] = note;
 }
 
-// Units that lie in several CTAs, and those without a tile (zeros).  One CTA per (unit of a sequence, sequence), a warp per column.
+// Units that lie in several CTAs, by the CTA in which they begin; a warp per column.
 template <int NT>
-__global__ void __launch_bounds__(32 * kCols<NT>) combine_kernel(const Args p, int most_units) {
+__global__ void __launch_bounds__(32 * kCols<NT>) combine_kernel(const Args p) {
   pdl_trigger();
-  const int b = blockIdx.x / most_units, u = blockIdx.x - b * most_units, c = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int c0 = blockIdx.x, c = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
-  const Seq s = seq_of<NT>(p, b);
-  if (u >= s.units) return;
-  int row, head, seen;
-  if (!column<NT>(p, s, b, u, c, row, head, seen)) return;
-  uint2* dst = reinterpret_cast<uint2*>(p.out + row * p.ldo + (int64_t)head * 128) + lane;
-  if (s.tiles == 0) {
-    *dst = make_uint2(0, 0);
-    return;
-  }
-  int64_t before = 0, total = 0;
-  for (int i = lane; i < p.B; i += 32) {
-    const Seq x = seq_of<NT>(p, i);
-    const int64_t w = (int64_t)x.units * x.tiles;
-    total += w;
-    if (i < b) before += w;
-  }
-#pragma unroll
-  for (int w = 1; w < 32; w <<= 1) {
-    before += __shfl_xor_sync(0xffffffffu, before, w);
-    total += __shfl_xor_sync(0xffffffffu, total, w);
-  }
-  const int64_t per = stretch(p, total) * kWarps, start = before + (int64_t)u * s.tiles;
-  const int c0 = (int)(start / per), c1 = (int)((start + s.tiles - 1) / per);
-  if (c0 == c1) return;
+  const int4 note = __ldcg(p.notes + c0);
+  if (note.x < 0) return;
+  const int c1 = note.z;
   const float* parts = p.parts;
   auto record = [&](int i) { return parts + ((int64_t)i * 2 + (i == c0 ? 1 : 0)) * kRecord<NT>; };
+  // weights of the first 32 pieces and numbers of the first 8 on their way together
+  constexpr int kAhead = 8;
+  float4 x[kAhead];
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) x[j] = __ldcg(reinterpret_cast<const float4*>(record(min(i0 + j, c1)) + c * 128) + lane);
+  };
+  load(c0);
   float top = kFloor;
   for (int i = c0 + lane; i <= c1; i += 32) top = fmaxf(top, __ldcg(record(i) + kCols<NT> * 128 + c));
   top = warp_max(top);
-  float l = 0.f;
+  float l = 0.f, w = 0.f;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = c0; i0 <= c1; i0 += 32) {
-    float w = 0.f;
-    if (i0 + lane <= c1) {
-      w = ex2(__ldcg(record(i0 + lane) + kCols<NT> * 128 + c) - top);
-      l += w * __ldcg(record(i0 + lane) + kCols<NT> * 129 + c);
+  for (int i = 0; i <= c1 - c0; i += kAhead) {
+    if ((i & 31) == 0) {
+      w = 0.f;
+      if (c0 + i + lane <= c1) {
+        w = ex2(__ldcg(record(c0 + i + lane) + kCols<NT> * 128 + c) - top);
+        l += w * __ldcg(record(c0 + i + lane) + kCols<NT> * 129 + c);
+      }
     }
-    const int m = min(32, c1 - i0 + 1);
-#pragma unroll 4
-    for (int j = 0; j < m; ++j) {
-      const float f = __shfl_sync(0xffffffffu, w, j);
-      const float4 x = __ldcg(reinterpret_cast<const float4*>(record(i0 + j) + c * 128) + lane);
-      v.x += x.x * f; v.y += x.y * f; v.z += x.z * f; v.w += x.w * f;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const float f = __shfl_sync(0xffffffffu, w, (i + j) & 31);
+      if (c0 + i + j <= c1) { v.x += x[j].x * f; v.y += x[j].y * f; v.z += x[j].z * f; v.w += x[j].w * f; }
     }
+    if (i + kAhead <= c1 - c0) load(c0 + i + kAhead);
   }
   l = warp_sum(l);
+  int row, head, seen;
+  if (!column<NT>(p, seq_of<NT>(p, note.x), note.x, note.y, c, row, head, seen)) return;
   const float inv = l == 0.f ? 0.f : 1.0f / l;
-  *dst = make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
+  reinterpret_cast<uint2*>(p.out + row * p.ldo + (int64_t)head * 128)[lane] = make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
 }
 
 }  // namespace fp4d
