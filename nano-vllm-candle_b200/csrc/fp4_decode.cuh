@@ -73,24 +73,25 @@ __device__ __forceinline__ uint32_t halves(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
   return d;
 }
+// (not volatile: they may be moved, but not in front of where their stage's address becomes known, behind the wait)
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
   uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  asm("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
   return v;
 }
 __device__ __forceinline__ uint2 lds64(uint32_t a) {
   uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  asm("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
   return v;
 }
 __device__ __forceinline__ uint32_t lds16(uint32_t a) {
   uint16_t v;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
+  asm("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
   return v;
 }
 __device__ __forceinline__ uint32_t lds8(uint32_t a) {
   uint32_t v;
-  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(a));
+  asm("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(a));
   return v;
 }
 __device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
@@ -114,6 +115,10 @@ __device__ __forceinline__ Seq seq_of(const Args& p, int b) {
   return s;
 }
 __device__ __forceinline__ int64_t weight(const Seq& s) { return s.tiles ? (int64_t)s.units * (s.tiles + kUnitCost) : 0; }
+// n / d; the short division where the numbers allow it
+__device__ __forceinline__ int64_t divide(int64_t n, int64_t d) {
+  return (uint64_t)(n | d) >> 32 ? n / d : (int64_t)((uint32_t)n / (uint32_t)d);
+}
 
 // The list, summed: a lane has the sequences [lane * m, lane * m + m)
 struct List { int m; int64_t upto, total; };            // upto: this lane's last sequence included
@@ -122,9 +127,11 @@ __device__ __forceinline__ List list_of(const Args& p, int lane) {
   List x;
   x.m = (p.B + 31) / 32;
   x.upto = 0;
+#pragma unroll 4
   for (int i = 0; i < x.m; ++i) {
     const int b = lane * x.m + i;
-    if (b < p.B) x.upto += weight(seq_of<NT>(p, b));
+    const Seq s = seq_of<NT>(p, min(b, p.B - 1));
+    x.upto += b < p.B ? weight(s) : 0;
   }
 #pragma unroll
   for (int w = 1; w < 32; w <<= 1) {
@@ -137,17 +144,16 @@ __device__ __forceinline__ List list_of(const Args& p, int lane) {
 
 // A warp's pieces, one behind another: tiles [t, end) of unit u of sequence b.  `rest`: what the stretch still has behind the unit's begin.
 struct Piece {
-  int b, u, t, end;
-  int64_t rest;
+  int b, u, t, end, rest;
   Seq s;
-  __device__ __forceinline__ bool cut(int64_t into) {   // the unit's tiles from weight `into` of it on, as far as the stretch goes; false: none
-    t = (int)max((int64_t)0, into - kUnitCost);
-    end = (int)min((int64_t)s.tiles, rest - kUnitCost);
+  __device__ __forceinline__ bool cut(int into) {       // the unit's tiles from weight `into` of it on, as far as the stretch goes; false: none
+    t = max(0, into - kUnitCost);
+    end = min(s.tiles, rest - kUnitCost);
     return end > t;
   }
 };
 template <int NT>
-__device__ __forceinline__ bool first_piece(const Args& p, const List& list, int64_t at, int64_t per, int lane, Piece& x) {
+__device__ __forceinline__ bool first_piece(const Args& p, const List& list, int64_t at, int per, int lane, Piece& x) {
   if (at >= list.total) return false;
   const int f = __ffs(__ballot_sync(0xffffffffu, list.upto > at)) - 1;
   const int64_t before = __shfl_sync(0xffffffffu, list.upto, max(f - 1, 0));
@@ -159,10 +165,10 @@ __device__ __forceinline__ bool first_piece(const Args& p, const List& list, int
     at -= w;
   }
   const int unit = x.s.tiles + kUnitCost;
-  x.u = (int)(at / unit);
-  at -= (int64_t)x.u * unit;
-  x.rest = at + per;
-  return x.cut(at);
+  x.u = (int)divide(at, unit);
+  const int into = (int)(at - (int64_t)x.u * unit);
+  x.rest = into + per;
+  return x.cut(into);
 }
 template <int NT>
 __device__ __forceinline__ bool next_piece(const Args& p, Piece& x) {
@@ -210,26 +216,31 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 3) attn_kernel(cons
   }
   __syncwarp();
   const List list = list_of<NT>(p, lane);
-  const int64_t per = max((list.total + p.warps - 1) / p.warps, (int64_t)1 + kUnitCost);
+  const int per = max((int)divide(list.total + p.warps - 1, p.warps), 1 + kUnitCost);          // (a stretch of 2^31 tiles would be 10 TB of cache)
   uint8_t* const mine = smem + warp * kWarpBytes<NT>;
   const uint32_t ring = smem_u32(mine);
   Piece at;
-  bool any = first_piece<NT>(p, list, per * (blockIdx.x * kWarps + warp), per, lane, at);
+  bool any = first_piece<NT>(p, list, (int64_t)per * (blockIdx.x * kWarps + warp), per, lane, at);
 
   // ---- the reading side: a tile ahead.  Lane 0 copies; the others know which rows are not there
   const int per_page = p.block_size / kHalf, last_page = p.bt_stride - 1;
   const bool whole = (per_page & 1) == 0;             // a tile lies in one page
   Piece rd = at;
   bool rd_any = any;
-  int page = 0, in_page = 0, kvh = 0, blk = 0, next = 0;
+  int page = 0, page_left = 0, kvh = 0, next = 0;     // halves that the page still has; the next page's block
+  uint32_t half_at = 0;                               // the place's half, counted through the cache
+  bool there = false;                                 // the pool has the page
+  auto turn = [&](int blk, int in_page) {
+    there = (unsigned)blk < (unsigned)p.num_blocks;
+    half_at = ((uint32_t)blk * p.kv + kvh) * per_page + in_page;
+    page_left = per_page - in_page;
+    next = p.block_tables[(int64_t)rd.b * p.bt_stride + min(page + 1, last_page)];
+  };
   auto enter = [&] {                                  // to a piece's first tile
     const int chunks = p.kv == rd.s.units ? 1 : rd.s.units / p.kv;
     kvh = chunks == 1 ? rd.u : rd.u / chunks;
-    const int32_t* table = p.block_tables + (int64_t)rd.b * p.bt_stride;
     page = 2 * rd.t / per_page;
-    in_page = 2 * rd.t - page * per_page;
-    blk = table[page];
-    next = table[min(page + 1, last_page)];
+    turn(p.block_tables[(int64_t)rd.b * p.bt_stride + page], 2 * rd.t - page * per_page);
   };
   if (rd_any) enter();
   pdl_wait();
@@ -244,25 +255,17 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 3) attn_kernel(cons
           for (int c = lane; c < p.kv * p.group * 16; c += 32) reinterpret_cast<uint4*>(p.out + row * p.ldo)[c] = make_uint4(0, 0, 0, 0);
       }
   }
-  if (per * blockIdx.x * kWarps >= list.total) {      // the whole CTA
+  if ((int64_t)per * (blockIdx.x * kWarps) >= list.total) {      // the whole CTA
     if (threadIdx.x == 0) p.notes[blockIdx.x] = make_int4(-1, 0, 0, 0);
     return;
   }
 
-  // half a tile, or all of it (rows: 16 or 32), of the page that the place is in
-  auto copy = [&](uint32_t st, uint32_t stage_bar, int half, int rows) {
-    const int64_t row = ((int64_t)blk * p.kv + kvh) * p.block_size + in_page * kHalf;
-    ptx::mbar_arrive_expect_tx(stage_bar, rows * 2 * (kFp4Codes + kFp4Scales));
-    ptx::bulk_load(st + half * kHalf * kFp4Codes, p.kc + row * kFp4Codes, rows * kFp4Codes, stage_bar);
-    ptx::bulk_load(st + kAtKs + half * kHalf * kFp4Scales, p.ks + row * kFp4Scales, rows * kFp4Scales, stage_bar);
-    ptx::bulk_load(st + kAtV + half * kHalf * kFp4Codes, p.vc + row * kFp4Codes, rows * kFp4Codes, stage_bar);
-    ptx::bulk_load(st + kAtVs + half * kHalf * kFp4Scales, p.vs + row * kFp4Scales, rows * kFp4Scales, stage_bar);
-  };
-  auto turn = [&] {
-    in_page = 0;
-    ++page;
-    blk = next;
-    next = p.block_tables[(int64_t)rd.b * p.bt_stride + min(page + 1, last_page)];
+  // half a tile, or all of it (rows: 16 or 32)
+  auto copy = [&](uint32_t to, uint32_t to_scales, uint32_t stage_bar, int rows) {
+    ptx::bulk_load(to, p.kc + (uint64_t)half_at * (kHalf * kFp4Codes), rows * kFp4Codes, stage_bar);
+    ptx::bulk_load(to + kAtV, p.vc + (uint64_t)half_at * (kHalf * kFp4Codes), rows * kFp4Codes, stage_bar);
+    ptx::bulk_load(to_scales + kAtKs, p.ks + (uint64_t)half_at * (kHalf * kFp4Scales), rows * kFp4Scales, stage_bar);
+    ptx::bulk_load(to_scales + kAtVs, p.vs + (uint64_t)half_at * (kHalf * kFp4Scales), rows * kFp4Scales, stage_bar);
   };
   uint32_t absent = 0;                                // bit 2 * stage + h: half h was not copied
   auto issue = [&](int stage) {
@@ -270,29 +273,42 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 3) attn_kernel(cons
     const uint32_t st = ring + stage * kStageBytes, stage_bar = bar + 8 * stage;
     uint32_t gone = 0;
     if (whole) {
-      if (in_page == per_page) turn();
-      if ((unsigned)blk < (unsigned)p.num_blocks) {
-        if (lane == 0) copy(st, stage_bar, 0, kTile);
+      if (page_left == 0) {
+        ++page;
+        turn(next, 0);
+      }
+      if (there) {
+        if (ptx::elect_one()) {
+          ptx::mbar_arrive_expect_tx(stage_bar, kStageBytes);
+          copy(st, st, stage_bar, kTile);
+        }
       } else {
         gone = 3;
         if (lane == 0) ptx::mbar_arrive(stage_bar);
       }
-      in_page += 2;
-    } else {                                          // a barrier phase takes one arrival: the first half's is without it
-#pragma unroll 1
+      page_left -= 2;
+      half_at += 2;
+    } else {                                          // a barrier phase takes one arrival: behind both halves
+#pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const bool there = rd.t * kTile + h * kHalf < rd.s.len;
-        if (there && in_page == per_page) turn();
-        if (!there || (unsigned)blk >= (unsigned)p.num_blocks) gone |= 1u << h;
-        else if (lane == 0) {
-          const int64_t row = ((int64_t)blk * p.kv + kvh) * p.block_size + in_page * kHalf;
-          asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(stage_bar), "r"(kHalf * 2 * (kFp4Codes + kFp4Scales)) : "memory");
-          ptx::bulk_load(st + h * kHalf * kFp4Codes, p.kc + row * kFp4Codes, kHalf * kFp4Codes, stage_bar);
-          ptx::bulk_load(st + kAtKs + h * kHalf * kFp4Scales, p.ks + row * kFp4Scales, kHalf * kFp4Scales, stage_bar);
-          ptx::bulk_load(st + kAtV + h * kHalf * kFp4Codes, p.vc + row * kFp4Codes, kHalf * kFp4Codes, stage_bar);
-          ptx::bulk_load(st + kAtVs + h * kHalf * kFp4Scales, p.vs + row * kFp4Scales, kHalf * kFp4Scales, stage_bar);
+        if (rd.t * kTile + h * kHalf < rd.s.len) {
+          if (page_left == 0) {
+            ++page;
+            turn(next, 0);
+          }
+          if (there) {
+            if (ptx::elect_one()) {
+              asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(stage_bar), "r"(kStageBytes / 2) : "memory");
+              copy(st + h * kHalf * kFp4Codes, st + h * kHalf * kFp4Scales, stage_bar, kHalf);
+            }
+          } else {
+            gone |= 1u << h;
+          }
+          --page_left;
+          ++half_at;
+        } else {
+          gone |= 1u << h;
         }
-        if (there) ++in_page;
       }
       if (lane == 0) ptx::mbar_arrive(stage_bar);
     }
@@ -426,7 +442,7 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 3) attn_kernel(cons
     for (int i = 0;; ++i) {
       __syncwarp();                                   // everyone is done with the stage that is filled now
       issue((i + 1) & 1);
-      const uint32_t st = ring + (i & 1) * kStageBytes;
+      uint32_t st = ring + (i & 1) * kStageBytes;
       wait_bar(bar + 8 * (i & 1), (i >> 1) & 1);
       const uint32_t gone = (absent >> (2 * (i & 1))) & 3u;
       if (gone || (at.t + 1) * kTile > at.s.len) {    // rows that are not there: scales of 0, whatever their codes are
@@ -437,6 +453,7 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 3) attn_kernel(cons
         ptx::fence_proxy_async_smem();
         __syncwarp();
       }
+      asm volatile("" : "+r"(st)::"memory");
       // ---- S^T = K Q^T: of each half, rows g and g + 8
       float s[NT][2][4];
 #pragma unroll
@@ -579,7 +596,7 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 3) attn_kernel(cons
     const int tiles = (&tiles_of[0][0])[i];
     const bool begins = head_of.z == 0, ends = behind == tiles;
     if (begins && !ends)                              // it ends in a later CTA: that many stretches of four warps behind this one's end
-      note = make_int4(head_of.x, head_of.y, (int)blockIdx.x + 1 + (int)((tiles - 1 - behind) / (per * kWarps)), 0);
+      note = make_int4(head_of.x, head_of.y, (int)blockIdx.x + 1 + (int)((tiles - 1 - behind) / ((int64_t)per * kWarps)), 0);
     float* part = p.parts + ((int64_t)blockIdx.x * 2 + (begins ? 1 : 0)) * kRecord<NT>;
     const int d = (threadIdx.x & 15) * 8;
 #pragma unroll
