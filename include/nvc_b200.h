@@ -762,7 +762,8 @@ int nvc_gemm_fp8_grouped(nvc_ctx* ctx, const nvc_fp8* A, int lda, const float* a
  * an infinity or a NaN (scale byte 255) reads as NaN.
  * Layout: k, v [num_blocks, kv, block_size, 64] (number 2i in the low half of byte i), k_scale, v_scale [num_blocks, kv, block_size, 8], each 16-byte aligned: a
  * page's rows of one key head lie together.  block_size % 16 == 0, num_blocks * block_size < 2^31; the slot of a token is block * block_size + offset, as above.
- * head_dim is 128.  These calls have no static operands (launch order, above): everything, tables and lengths too, is read behind the wait. */
+ * head_dim is 128.  Static operands (launch order, above) of the attention calls are block_tables, context_lens and cu_seqlens_q; those that store and read rows have none, and
+ * queries and cached rows may come from any earlier work of the stream. */
 typedef struct nvc_fp4_cache {
   uint8_t *k, *k_scale, *v, *v_scale;
   int num_blocks, kv, block_size;
@@ -782,14 +783,15 @@ int nvc_read_kvcache_fp4(nvc_ctx* ctx, const nvc_fp4_cache* cache, const int32_t
                          void* stream);
 /* nvc_paged_decode_attn over such a cache.  q [B, nh * 128] stride ldq; block_tables [B, bt_stride]; out [B, nh * 128] stride ldo (multiples of 8).  A context of length 0 (or
  * less) gives zeros; a length beyond the table's bt_stride * block_size counts as that; a block outside the pool reads as rows of zeros.  Rows past a context
- * may hold anything.  The weights of a row's keys are rounded to fp16 for the second product (2^-11 of each).  workspace: nvc_attn_fp4_workspace_bytes, of this call alone
- * while it runs; nothing in it has to be cleared.
+ * may hold anything.  The weights of a row's keys are rounded to fp16 for the second product (2^-11 of each).  workspace: nvc_attn_fp4_workspace_bytes with max_seqlen_q = 1, 16-byte
+ * aligned, of this call alone while it runs; nothing in it has to be cleared.
  * A row's sums are grouped by what the whole batch holds: a call repeats itself bit by bit, a sequence beside others may differ in rounding. */
-size_t nvc_attn_fp4_workspace_bytes(const nvc_ctx* ctx, int nh, int kv);
+size_t nvc_attn_fp4_workspace_bytes(const nvc_ctx* ctx, int nh, int kv, int max_seqlen_q);
 int nvc_paged_decode_attn_fp4(nvc_ctx* ctx, const nvc_bf16* q, int ldq, const nvc_fp4_cache* cache, const int32_t* block_tables, int bt_stride,
                               const int32_t* context_lens, int B, int nh, float scale, nvc_bf16* out, int ldo, void* workspace, size_t workspace_bytes, void* stream);
 /* nvc_prefill_attn_paged over such a cache: q row i of sequence b (rows cu_seqlens_q[b] .. cu_seqlens_q[b + 1], ascending from 0) is position context_lens[b] - q_len_b + i and
- * sees the keys up to itself, none where that is negative (zeros).  max_seqlen_q: at least the longest q_len.  Rows behind cu_seqlens_q[B] are left as they are. */
+ * sees the keys up to itself, none where that is negative (zeros).  max_seqlen_q: at least the longest q_len; workspace: for the smaller of it
+ * and total_q_tokens.  Rows behind cu_seqlens_q[B] are left as they are. */
 int nvc_prefill_attn_paged_fp4(nvc_ctx* ctx, const nvc_bf16* q, int ldq, const nvc_fp4_cache* cache, const int32_t* block_tables, int bt_stride,
                                const int32_t* context_lens, const int32_t* cu_seqlens_q, int B, int total_q_tokens, int max_seqlen_q, int nh, float scale,
                                nvc_bf16* out, int ldo, void* workspace, size_t workspace_bytes, void* stream);

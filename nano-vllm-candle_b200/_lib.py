@@ -181,7 +181,7 @@ def _declare(l: C.CDLL) -> None:
     l.nvc_paged_decode_workspace_bytes.restype = _sz
     l.nvc_paged_decode_workspace_bytes.argtypes = [_i, _i, _i, _i]
     l.nvc_attn_fp4_workspace_bytes.restype = _sz
-    l.nvc_attn_fp4_workspace_bytes.argtypes = [_vp, _i, _i]
+    l.nvc_attn_fp4_workspace_bytes.argtypes = [_vp, _i, _i, _i]
     l.nvc_paged_decode_static_scratch_bytes.restype = _sz
     l.nvc_paged_decode_static_scratch_bytes.argtypes = []
     from . import _engine_sigs

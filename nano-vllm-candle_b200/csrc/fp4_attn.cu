@@ -1,6 +1,7 @@
 // Attention over the 4-bit paged cache: decode (one new row of each sequence) and prompt portions (the last rows of each context, causal).
 // FLOPs: 4 * 128 for every (query head, visible key); bytes: 144 for every (key head, cached token), 512 for every query head's row and its result.
 #include "fp4_decode.cuh"
+#include "fp4_prefill.cuh"
 #include "internal.h"
 
 #include <algorithm>
@@ -31,6 +32,23 @@ int launch_few(nvc_ctx* ctx, fp4d::Args& p, int64_t most_rows, cudaStream_t stre
   return NVC_OK;
 }
 
+constexpr int kFewRows = 64;          // of a key head: up to here the kernel for few rows
+int64_t most_rows_of(int rows, int max_qlen, int group) { return std::min(rows, max_qlen) * (int64_t)group; }
+size_t many_bytes(const nvc_ctx* ctx) { return (size_t)ctx->num_sms * (16 + 2 * fp4p::kRecord * 4); }
+
+int launch_many(nvc_ctx* ctx, const fp4d::Args& f, float scale, cudaStream_t stream, size_t workspace_bytes) {
+  NVC_REQUIRE(ctx, f.notes && ((uintptr_t)f.notes & 15) == 0 && workspace_bytes >= many_bytes(ctx), NVC_ENOMEM, "workspace too small");
+  const int grid = ctx->num_sms;
+  const fp4p::Args p{f.q, f.out, f.ldq, f.ldo, f.kc, f.ks, f.vc, f.vs, f.block_tables, f.context_lens, f.cu_seqlens, f.bt_stride, f.num_blocks, f.kv, f.block_size, f.B, f.group,
+                     f.rows, fp4p::make_div(f.group), fp4p::make_div(f.block_size), scale > 0.f ? 1.f : scale < 0.f ? -1.f : 0.f,
+                     scale == 0.f ? 1.f : std::fabs(scale) * 1.4426950408889634f, f.notes, reinterpret_cast<float*>(f.notes + grid)};
+  NVC_CUDA_CHECK(ctx, nvc_launch(ctx, fp4p::attn_kernel, dim3(grid), dim3(fp4p::kThreads), (size_t)fp4p::kSmemBytes, stream, p));
+  NVC_CUDA_CHECK(ctx, nvc_launch(ctx, fp4p::combine_kernel, dim3(grid * 8), dim3(256), 0, stream, p));
+  NVC_CUDA_CHECK(ctx, cudaGetLastError());
+  ctx->launches += 2;
+  return NVC_OK;
+}
+
 int attn_fp4(nvc_ctx* ctx, const nvc_bf16* q, int ldq, const nvc_fp4_cache* cache, const int32_t* block_tables, int bt_stride, const int32_t* context_lens,
              const int32_t* cu_seqlens_q, int B, int rows, int max_qlen, int nh, float scale, nvc_bf16* out, int ldo, void* workspace, size_t workspace_bytes, void* stream) {
   if (const int rc = nvc_fp4_cache_check(ctx, cache)) return rc;
@@ -42,11 +60,12 @@ int attn_fp4(nvc_ctx* ctx, const nvc_bf16* q, int ldq, const nvc_fp4_cache* cach
   NVC_REQUIRE(ctx, std::isfinite(scale), NVC_EINVAL, "the scale must be finite");
   if (B == 0 || rows == 0 || max_qlen == 0) return NVC_OK;
   const int group = nh / cache->kv;
-  const int64_t most_rows = std::min(rows, max_qlen) * (int64_t)group;             // of one key head, columns of its units
+  const int64_t most_rows = most_rows_of(rows, max_qlen, group);             // of a sequence and key head
   NVC_REQUIRE(ctx, most_rows <= 0x7ffffff0LL, NVC_ESHAPE, "too many rows");
   fp4d::Args p{q, out, ldq, ldo, cache->k, cache->k_scale, cache->v, cache->v_scale, block_tables, context_lens, cu_seqlens_q, bt_stride, cache->num_blocks, cache->kv,
                cache->block_size, B, group, rows, scale * 1.4426950408889634f, static_cast<int4*>(workspace), nullptr, 0};
   DeviceGuard guard(ctx->device);
+  if (most_rows > kFewRows) return launch_many(ctx, p, scale, nvc_stream(stream), workspace_bytes);
   return most_rows <= 8 ? launch_few<1>(ctx, p, most_rows, nvc_stream(stream), workspace_bytes) : launch_few<2>(ctx, p, most_rows, nvc_stream(stream), workspace_bytes);
 }
 
@@ -55,11 +74,14 @@ int attn_fp4(nvc_ctx* ctx, const nvc_bf16* q, int ldq, const nvc_fp4_cache* cach
 extern "C" int nvc_fp4_attn_init(nvc_ctx* ctx) {
   NVC_CUDA_CHECK(ctx, cudaFuncSetAttribute(fp4d::attn_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, fp4d::kSmem<1>));
   NVC_CUDA_CHECK(ctx, cudaFuncSetAttribute(fp4d::attn_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, fp4d::kSmem<2>));
+  NVC_CUDA_CHECK(ctx, cudaFuncSetAttribute(fp4p::attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, fp4p::kSmemBytes));
   return NVC_OK;
 }
 
-extern "C" size_t nvc_attn_fp4_workspace_bytes(const nvc_ctx* ctx, int nh, int kv) {
-  return ctx ? (size_t)std::max(parts_bytes<1>(ctx), parts_bytes<2>(ctx)) : 0;
+extern "C" size_t nvc_attn_fp4_workspace_bytes(const nvc_ctx* ctx, int nh, int kv, int max_seqlen_q) {
+  if (!ctx || nh <= 0 || kv <= 0 || max_seqlen_q <= 0) return 0;
+  const int64_t rows = most_rows_of(max_seqlen_q, max_seqlen_q, (nh + kv - 1) / kv);
+  return rows > kFewRows ? many_bytes(ctx) : (size_t)(rows <= 8 ? parts_bytes<1>(ctx) : parts_bytes<2>(ctx));
 }
 
 extern "C" int nvc_paged_decode_attn_fp4(nvc_ctx* ctx, const nvc_bf16* q, int ldq, const nvc_fp4_cache* cache, const int32_t* block_tables, int bt_stride,

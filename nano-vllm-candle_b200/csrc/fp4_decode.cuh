@@ -109,7 +109,7 @@ __device__ __forceinline__ Seq seq_of(const Args& p, int b) {
   Seq s;
   const int64_t room = (int64_t)p.bt_stride * p.block_size;
   s.len = (int)min((int64_t)max(p.context_lens[b], 0), room);
-  s.qlen = p.cu_seqlens ? max(p.cu_seqlens[b + 1] - p.cu_seqlens[b], 0) : 1;
+  s.qlen = p.cu_seqlens ? min(max(p.cu_seqlens[b + 1] - p.cu_seqlens[b], 0), p.rows) : 1;
   s.tiles = s.len / kTile + (s.len % kTile != 0);
   s.units = p.kv * ((s.qlen * p.group + kCols<NT> - 1) / kCols<NT>);
   return s;

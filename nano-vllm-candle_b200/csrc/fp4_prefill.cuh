@@ -1,0 +1,593 @@
+// Causal attention of prompt portions over the 4-bit paged cache on tcgen05 (fp16 operands, fp32 sums in tensor memory).
+//
+// One CTA per SM, 256 query rows - the rows of all the query heads of a key head, head by head within a token - as two tiles of 128 against key tiles of 128 tokens:
+//   * 4 warps decode the cache's rows into fp16 tiles in shared memory (K and V, two of each), once for 256 rows: half a percent of what decoding for each head would cost.  A thread
+//     has a token's row: 64 bytes of codes and 8 of scales, requested two tiles ahead;
+//   * 1 warp issues the products, S_w = Q_w K^T and O_w += P_w V, tile 0's and tile 1's in turn, so that the tensor cores work on one while the other's softmax runs;
+//   * 4 warps for each tile: a thread owns a row.  P goes back into tensor memory over the S it came from (fp16 pairs) and is the A operand there.  The reference of the exponentials
+//     follows the row's maximum when that grew by more than 2^8, shifted by 2^7, as in the kernel for few rows; only then O is rescaled.
+// Queries are brought to fp16 behind a power of two of their own row, that the score's factor takes back.  The sign of the scale goes with them, so that a row's maximum may be taken in front of
+// the factor.
+//
+// Work is cut as in the kernel for few rows: the key tiles of all (sequence, 256 rows, key head) units in one list, an equal stretch for each CTA; units that lie in several CTAs are joined by
+// combine_kernel from records in the workspace.
+#pragma once
+#include "fp4.cuh"
+#include "ptx.cuh"
+
+namespace fp4p {
+
+constexpr int kKT = 128, kRows = 256, kThreads = 512;
+constexpr int kTileBytes = 128 * 128 * 2;                  // fp16, two halves of 64 dims: [128 rows][128 bytes], 16-byte chunks permuted by the row
+constexpr int kHalf = kTileBytes / 2;
+constexpr int kOffQ = 0, kOffK = 2 * kTileBytes, kOffV = kOffK + 2 * kTileBytes, kOffFactor = kOffV + 2 * kTileBytes, kOffBar = kOffFactor + kRows * 4;
+constexpr int kNumBars = 18;
+constexpr int kSmemBytes = kOffBar + kNumBars * 8 + 16 + 1024;          // and room to begin at a multiple of 1024
+constexpr int kUnitCost = 2;                               // a unit's queries and result, in tiles
+constexpr float kFloor = -1.0e30f, kShift = 7.0f, kGrow = 8.0f;
+constexpr int kRecord = kRows * 130;                       // floats: O [32 groups of 4 dims][256 rows][4], reference [256], sum [256]
+constexpr int kChunk = 2048;                               // sequences whose weights are looked at together (in shared memory)
+
+// n / d for n < 2^31 and a d of the host's: d's inverse, rounded up, with as many bits as that takes
+struct Div {
+  unsigned long long mul;
+  int shift;
+  __device__ __forceinline__ int operator()(int n) const { return (int)((unsigned long long)(unsigned)n * mul >> shift); }
+};
+inline Div make_div(int d) {
+  int s = 0;
+  while ((1ll << s) < d) ++s;
+  return Div{((1ull << (32 + s)) + (unsigned long long)d - 1) / (unsigned long long)d, 32 + s};
+}
+
+struct Args {
+  const nvc_bf16* q;
+  nvc_bf16* out;
+  int64_t ldq, ldo;
+  const uint8_t *kc, *ks, *vc, *vs;
+  const int32_t *block_tables, *context_lens, *cu_seqlens;
+  int bt_stride, num_blocks, kv, block_size, B, group, rows;
+  Div by_group, by_block;
+  float q_sign, factor;                                    // -1, 0 or 1; what scores are multiplied with (positive)
+  int4* notes;                                             // of each CTA, the unit that begins there and ends in another: sequence (-1: none), 256 rows' number, key head, last CTA
+  float* parts;                                            // two records of each CTA
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t halves(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+// instruction descriptor: fp16 x fp16 -> fp32 (formats 0), M = N = 128
+__host__ __device__ constexpr uint32_t idesc(int b_mn_major) { return (1u << 4) | ((uint32_t)b_mn_major << 16) | (128u >> 3 << 17) | (128u >> 4 << 24); }
+
+struct Seq { int len, qlen, begin, blocks; };              // begin: its first row; blocks: units of 256 rows
+__device__ __forceinline__ Seq seq_of(const Args& p, int b) {
+  Seq s;
+  s.len = (int)min((int64_t)max(p.context_lens[b], 0), (int64_t)p.bt_stride * p.block_size);
+  s.begin = p.cu_seqlens[b];
+  s.qlen = min(max(p.cu_seqlens[b + 1] - s.begin, 0), p.rows);
+  s.blocks = (int)(((int64_t)s.qlen * p.group + kRows - 1) / kRows);
+  return s;
+}
+// key tiles of a unit: up to its last row's last key; one where there is none
+__device__ __forceinline__ int tiles_of(const Args& p, const Seq& s, int j) {
+  const int last = min(s.qlen - 1, p.by_group(kRows * j + kRows - 1));
+  return max(1, (max(s.len - s.qlen + last + 1, 0) + kKT - 1) / kKT);
+}
+
+// A CTA's pieces: tiles [t, end) of unit (b, j, h)
+struct Piece {
+  int b, j, h, t, end, tiles, rest;                        // rest: what the stretch still has behind the unit's begin
+  Seq s;
+  __device__ __forceinline__ bool cut(int into) {
+    t = max(0, into - kUnitCost);
+    end = min(tiles, rest - kUnitCost);
+    return end > t;
+  }
+};
+__device__ __forceinline__ bool next_piece(const Args& p, Piece& x) {
+  x.rest -= x.tiles + kUnitCost;
+  if (x.rest <= kUnitCost) return false;
+  if (++x.h == p.kv) {
+    x.h = 0;
+    if (++x.j == x.s.blocks) {
+      x.j = 0;
+      do {
+        if (++x.b >= p.B) return false;
+        x.s = seq_of(p, x.b);
+      } while (x.s.blocks == 0);
+    }
+    x.tiles = tiles_of(p, x.s, x.j);
+  }
+  return x.cut(0);
+}
+__device__ __forceinline__ int64_t sum64(int64_t x) {
+#pragma unroll
+  for (int w = 1; w < 32; w <<= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
+  return x;
+}
+// Where the CTA's stretch begins, found by all its warps (16) together.  weights: shared memory for kChunk numbers; every thread gets the result.  per: a stretch's length.
+__device__ __forceinline__ bool plan(const Args& p, int64_t* weights, int warp, int lane, Piece& x, int& per, int64_t& total) {
+  constexpr int kW = kThreads / 32;
+  __shared__ int64_t sums[kW];
+  auto weigh = [&](int b) {                                // a sequence's weight, of a whole warp
+    const Seq s = seq_of(p, b);
+    int64_t mine = 0;
+    for (int j = lane; j < s.blocks; j += 32) mine += tiles_of(p, s, j) + kUnitCost;
+    return sum64(mine) * p.kv;
+  };
+  int64_t mine = 0;
+  for (int b = warp; b < p.B; b += kW) {
+    const int64_t w = weigh(b);
+    if (b < kChunk && lane == 0) weights[b] = w;           // the first of them stay for the second look
+    mine += w;
+  }
+  if (lane == 0) sums[warp] = mine;
+  __syncthreads();
+  total = 0;
+#pragma unroll
+  for (int i = 0; i < kW; ++i) total += sums[i];
+  per = max((int)((total + gridDim.x - 1) / gridDim.x), 4 + kUnitCost);
+  int64_t at = (int64_t)per * blockIdx.x;
+  if (at >= total) return false;
+  int b0 = 0;
+  for (;;) {                                               // by chunks of sequences
+    const int n = min(kChunk, p.B - b0);
+    // every warp alike: lanes take runs of m sequences
+    const int m = (n + 31) / 32;
+    int64_t upto = 0;
+    for (int i = 0; i < m; ++i)
+      if (lane * m + i < n) upto += weights[lane * m + i];
+#pragma unroll
+    for (int w = 1; w < 32; w <<= 1) {
+      const int64_t up = __shfl_up_sync(0xffffffffu, upto, w);
+      if (lane >= w) upto += up;
+    }
+    const unsigned behind = __ballot_sync(0xffffffffu, upto > at);
+    if (behind) {
+      const int f = __ffs(behind) - 1;
+      const int64_t before = __shfl_sync(0xffffffffu, upto, max(f - 1, 0));
+      at -= f ? before : 0;
+      int i = f * m;
+      while (at >= weights[i]) at -= weights[i++];
+      x.b = b0 + i;
+      break;
+    }
+    at -= __shfl_sync(0xffffffffu, upto, 31);
+    b0 += kChunk;
+    __syncthreads();
+    for (int b = b0 + warp; b < min(p.B, b0 + kChunk); b += kW) {
+      const int64_t w = weigh(b);
+      if (lane == 0) weights[b - b0] = w;
+    }
+    __syncthreads();
+  }
+  x.s = seq_of(p, x.b);
+  for (int j0 = 0;; j0 += 32) {                            // within the sequence: 256 rows after 256 rows
+    const int64_t w = j0 + lane < x.s.blocks ? (int64_t)(tiles_of(p, x.s, j0 + lane) + kUnitCost) * p.kv : 0;
+    int64_t upto = w;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t up = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += up;
+    }
+    const unsigned behind = __ballot_sync(0xffffffffu, upto > at);
+    if (behind) {
+      const int f = __ffs(behind) - 1;
+      at -= __shfl_sync(0xffffffffu, upto - w, f);
+      x.j = j0 + f;
+      break;
+    }
+    at -= __shfl_sync(0xffffffffu, upto, 31);
+  }
+  x.tiles = tiles_of(p, x.s, x.j);
+  const int unit = x.tiles + kUnitCost;
+  x.h = (int)((uint32_t)at / (uint32_t)unit);              // a unit's heads: below 2^32 in all
+  const int into = (int)at - x.h * unit;
+  x.rest = into + per;
+  return x.cut(into);
+}
+
+__global__ void __launch_bounds__(kThreads, 1) attn_kernel(const Args p) {
+  pdl_trigger();
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* const gen = smem_raw + (base - smem_u32(smem_raw));
+  const uint32_t bar0 = base + kOffBar;
+  auto q_full = [&](int w) { return bar0 + 8u * w; };
+  auto k_full = [&](uint32_t s) { return bar0 + 8u * (2 + s); };
+  auto k_empty = [&](uint32_t s) { return bar0 + 8u * (4 + s); };
+  auto v_full = [&](uint32_t s) { return bar0 + 8u * (6 + s); };
+  auto v_empty = [&](uint32_t s) { return bar0 + 8u * (8 + s); };
+  auto s_full = [&](int w) { return bar0 + 8u * (10 + w); };
+  auto p_full = [&](int w) { return bar0 + 8u * (12 + w); };
+  auto o_done = [&](int w) { return bar0 + 8u * (14 + w); };
+  const uint32_t tmem_slot = bar0 + 8u * kNumBars;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      for (int i = 0; i < 2; ++i) {
+        ptx::mbar_init(q_full(i), 128);
+        ptx::mbar_init(k_full(i), 128);
+        ptx::mbar_init(k_empty(i), 1);
+        ptx::mbar_init(v_full(i), 128);
+        ptx::mbar_init(v_empty(i), 1);
+        ptx::mbar_init(s_full(i), 1);
+        ptx::mbar_init(p_full(i), 128);
+        ptx::mbar_init(o_done(i), 1);
+      }
+      ptx::fence_barrier_init();
+    }
+    __syncwarp();
+  } else if (warp == 12) {
+    ptx::tmem_alloc(tmem_slot, 512);
+    ptx::tmem_relinquish();
+  }
+  Piece at;
+  int per;
+  int64_t total;
+  const bool any = plan(p, reinterpret_cast<int64_t*>(gen + kOffK), warp, lane, at, per, total);
+  ptx::tcgen05_fence_before();
+  __syncthreads();
+  ptx::tcgen05_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(gen + kOffBar + kNumBars * 8);
+  auto tmem_s = [&](int w) { return tmem + 128u * w; };
+  auto tmem_o = [&](int w) { return tmem + 256u + 128u * w; };
+  pdl_wait();
+
+  if (!any) {
+    if (threadIdx.x == 0) p.notes[blockIdx.x] = make_int4(-1, 0, 0, 0);
+  } else if (warp >= 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    // ------------------------------------------------------------ the products (one warp of the four)
+    if (warp == 12) {
+      constexpr uint32_t hi = ptx::umma_desc_hi_sw128(1024);
+      auto issue_s = [&](int w, uint32_t g) {
+        if (ptx::elect_one()) {
+          const uint32_t q_lo = ptx::umma_desc_lo(base + kOffQ + w * kTileBytes, 16), k_lo = ptx::umma_desc_lo(base + kOffK + (g & 1) * kTileBytes, 16);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const uint32_t off = ((k >> 2) * kHalf + (k & 3) * 32) >> 4;
+            ptx::umma_bf16_ss(tmem_s(w), ptx::umma_desc(q_lo + off, hi), ptx::umma_desc(k_lo + off, hi), idesc(0), k != 0);
+          }
+          ptx::umma_commit(s_full(w));
+          if (w == 1) ptx::umma_commit(k_empty(g & 1));
+        }
+        __syncwarp();
+      };
+      uint32_t g = 0, done = 0;
+      bool more = true;
+      while (more) {
+        const int n = at.end - at.t;
+        ptx::mbar_wait(k_full(g & 1), (g >> 1) & 1);
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          ptx::mbar_wait(q_full(w), done & 1);
+          ptx::tcgen05_fence_after();
+          issue_s(w, g);
+        }
+        for (int j = 0; j < n; ++j, ++g) {
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            ptx::mbar_wait(p_full(w), g & 1);              // P is there, O rescaled (or, in a piece's first tile, read out)
+            if (w == 0) ptx::mbar_wait(v_full(g & 1), (g >> 1) & 1);
+            ptx::tcgen05_fence_after();
+            if (ptx::elect_one()) {
+              const uint32_t v_lo = ptx::umma_desc_lo(base + kOffV + (g & 1) * kTileBytes, (uint32_t)kHalf);       // dims are its rows: 16 tokens a step
+#pragma unroll
+              for (int k = 0; k < 8; ++k) ptx::umma_bf16_ts(tmem_o(w), tmem_s(w) + k * 8, ptx::umma_desc(v_lo + k * (2048 >> 4), hi), idesc(1), (j | k) != 0);
+              ptx::umma_commit(o_done(w));
+              if (w == 1) ptx::umma_commit(v_empty(g & 1));
+            }
+            __syncwarp();
+            if (j + 1 < n) {
+              if (w == 0) {
+                ptx::mbar_wait(k_full((g + 1) & 1), ((g + 1) >> 1) & 1);
+                ptx::tcgen05_fence_after();
+              }
+              issue_s(w, g + 1);
+            }
+          }
+        }
+        ++done;
+        more = next_piece(p, at);
+      }
+    }
+  } else if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    // ------------------------------------------------------------ the cache's rows, decoded: a thread has a token of the tile
+    const int r = threadIdx.x - 256;
+    struct Raw { uint4 c[4]; uint2 s; };
+    const int last_page = p.bt_stride - 1;
+    auto block_of = [&](const Piece& x, int tile) {        // of this thread's token; -1 where it has none
+      const int tok = tile * kKT + r;
+      if (tok >= x.s.len) return -1;
+      return p.block_tables[(int64_t)x.b * p.bt_stride + min(p.by_block(tok), last_page)];
+    };
+    auto load = [&](const Piece& x, int tile, int blk, const uint8_t* codes, const uint8_t* scales) {
+      Raw w;
+      const int tok = tile * kKT + r;
+      if (tok < x.s.len && (unsigned)blk < (unsigned)p.num_blocks) {
+        const int64_t row = ((int64_t)blk * p.kv + x.h) * p.block_size + (tok - p.by_block(tok) * p.block_size);
+        const uint4* c = reinterpret_cast<const uint4*>(codes + row * kFp4Codes);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w.c[i] = c[i];
+        w.s = *reinterpret_cast<const uint2*>(scales + row * kFp4Scales);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w.c[i] = make_uint4(0, 0, 0, 0);
+        w.s = make_uint2(0, 0);
+      }
+      return w;
+    };
+    auto write = [&](const Raw& w, uint32_t tile_at, uint32_t bar) {
+      const uint32_t row = tile_at + r * 128;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t c[4] = {w.c[i].x, w.c[i].y, w.c[i].z, w.c[i].w};
+        const uint32_t two = (i < 2 ? w.s.x : w.s.y) >> (16 * (i & 1));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {                      // 8 dims: chunk 4i + k of 16 bytes
+          const uint32_t f = (k < 2 ? two & 0xffu : (two >> 8) & 0xffu) * 0x00800080u;
+          const uint4 x = fp4_halves8(c[k]);
+          const uint32_t chunk = 4 * (i & 1) + k;
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + (i >> 1) * kHalf + ((chunk ^ (r & 7)) << 4)), "r"(mul2(x.x, f)), "r"(mul2(x.y, f)),
+                       "r"(mul2(x.z, f)), "r"(mul2(x.w, f)) : "memory");
+        }
+      }
+      ptx::fence_proxy_async_smem();
+      ptx::mbar_arrive(bar);
+    };
+    uint32_t g = 0;
+    bool more = true;
+    Raw rk, rv;
+    int b1 = block_of(at, at.t), b2 = at.t + 1 < at.end ? block_of(at, at.t + 1) : -1, b3;
+    rk = load(at, at.t, b1, p.kc, p.ks);
+    rv = load(at, at.t, b1, p.vc, p.vs);
+    while (more) {
+      const Piece x = at;
+      more = next_piece(p, at);
+      ptx::mbar_wait(k_empty(g & 1), ((g >> 1) & 1) ^ 1u);
+      write(rk, base + kOffK + (g & 1) * kTileBytes, k_full(g & 1));
+      if (x.t + 1 < x.end) rk = load(x, x.t + 1, b2, p.kc, p.ks);
+      else if (more) rk = load(at, at.t, block_of(at, at.t), p.kc, p.ks);
+      for (int j = x.t; j < x.end; ++j, ++g) {
+        // b2: the next tile's block; K runs a tile ahead of V
+        b3 = j + 2 < x.end ? block_of(x, j + 2) : -1;
+        if (j + 1 < x.end) {
+          ptx::mbar_wait(k_empty((g + 1) & 1), (((g + 1) >> 1) & 1) ^ 1u);
+          write(rk, base + kOffK + ((g + 1) & 1) * kTileBytes, k_full((g + 1) & 1));
+          if (j + 2 < x.end) rk = load(x, j + 2, b3, p.kc, p.ks);
+          else if (more) rk = load(at, at.t, block_of(at, at.t), p.kc, p.ks);
+        }
+        ptx::mbar_wait(v_empty(g & 1), ((g >> 1) & 1) ^ 1u);
+        write(rv, base + kOffV + (g & 1) * kTileBytes, v_full(g & 1));
+        if (j + 1 < x.end) rv = load(x, j + 1, b2, p.vc, p.vs);
+        b2 = b3;
+      }
+      if (more) {
+        rv = load(at, at.t, block_of(at, at.t), p.vc, p.vs);
+        b2 = at.t + 1 < at.end ? block_of(at, at.t + 1) : -1;
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    // ------------------------------------------------------------ softmax, a thread for a row; queries in front of a piece, the result behind it
+    const int w = warp >> 2, quad = warp & 3, r = quad * 32 + lane;
+    const uint32_t lane_at = (uint32_t)(quad * 32) << 16;
+    float* const factors = reinterpret_cast<float*>(gen + kOffFactor) + w * 128;
+    uint8_t* const q_tile = gen + kOffQ + w * kTileBytes;
+    uint32_t g = 0;
+    bool more = true;
+    int4 note = make_int4(-1, 0, 0, 0);
+    while (more) {
+      const Piece x = at;
+      const int first = kRows * x.j + 128 * w;             // packed row of the tile's first
+      const int real = x.s.qlen * p.group;                 // (at most 2^31: the host's check)
+      // ---- this warp's 32 rows of Q: 16 lanes a row
+#pragma unroll 1
+      for (int i0 = 0; i0 < 16; i0 += 8) {
+        uint4 y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int row = first + quad * 32 + 2 * (i0 + i) + (lane >> 4), tok = p.by_group(row);
+          const int at_row = x.s.begin + tok;
+          y[i] = make_uint4(0, 0, 0, 0);
+          if (row < real && (unsigned)at_row < (unsigned)p.rows)
+            y[i] = reinterpret_cast<const uint4*>(p.q + at_row * p.ldq + (int64_t)(x.h * p.group + row - tok * p.group) * 128)[lane & 15];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint32_t top = fp4_amax8(y[i]);
+#pragma unroll
+          for (int d = 1; d < 16; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+          int e = top >= 0x7f80u || top == 0 ? 0 : (int)(top >> 7) - 127;
+          e = min(max(e, -126), 126);
+          const float down = __uint_as_float((uint32_t)(127 - e) << 23) * p.q_sign;
+          const int row = quad * 32 + 2 * (i0 + i) + (lane >> 4), c = lane & 15;
+          *reinterpret_cast<uint4*>(q_tile + (c >> 3) * kHalf + row * 128 + (((c & 7) ^ (row & 7)) << 4)) =
+              make_uint4(halves(bf16_lo(y[i].x) * down, bf16_hi(y[i].x) * down), halves(bf16_lo(y[i].y) * down, bf16_hi(y[i].y) * down),
+                         halves(bf16_lo(y[i].z) * down, bf16_hi(y[i].z) * down), halves(bf16_lo(y[i].w) * down, bf16_hi(y[i].w) * down));
+          if (c == 0) factors[row] = fmaxf(__uint_as_float((uint32_t)(127 + e) << 23) * p.factor, 1.2e-38f);        // 0 would turn a masked score into a NaN
+        }
+      }
+      ptx::fence_proxy_async_smem();
+      ptx::mbar_arrive(q_full(w));
+      __syncwarp();
+      const float factor = factors[r];
+      const int tok = p.by_group(first + r);
+      const int lim = x.s.len - x.s.qlen + min(tok, x.s.qlen - 1);          // the last key that the row sees
+      const int least = x.s.len - x.s.qlen + p.by_group(first + quad * 32);   // of the warp's rows
+      float ref = kFloor, sum = 0.f;
+      const int n = x.end - x.t;
+      for (int j = 0; j < n; ++j, ++g) {
+        const uint32_t s_at = tmem_s(w) + lane_at;
+        ptx::mbar_wait(s_full(w), g & 1);
+        ptx::tcgen05_fence_after();
+        uint32_t sv[128];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) ptx::tmem_ld_32x32b_x32(s_at + 32 * c, sv + 32 * c);
+        ptx::tmem_ld_wait();
+        const int t0 = (x.t + j) * kKT;
+        if (t0 + kKT - 1 > least) {
+          const int l = lim - t0;
+#pragma unroll
+          for (int i = 0; i < 128; ++i)
+            if (i > l) sv[i] = 0xff800000u;
+        }
+        float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 128; i += 4) {
+          m0 = fmaxf(m0, __uint_as_float(sv[i]));
+          m1 = fmaxf(m1, __uint_as_float(sv[i + 1]));
+          m2 = fmaxf(m2, __uint_as_float(sv[i + 2]));
+          m3 = fmaxf(m3, __uint_as_float(sv[i + 3]));
+        }
+        const float top = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * factor - kShift;
+        const bool move = __any_sync(0xffffffffu, top > ref + kGrow);
+        float alpha = 1.0f;
+        if (move) {
+          const float now = fmaxf(ref, top);
+          alpha = ex2(ref - now);
+          ref = now;
+        }
+        float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+#pragma unroll
+        for (int i = 0; i < 128; i += 4) {
+          const float p0 = ex2(fmaf(__uint_as_float(sv[i]), factor, -ref)), p1 = ex2(fmaf(__uint_as_float(sv[i + 1]), factor, -ref));
+          const float p2 = ex2(fmaf(__uint_as_float(sv[i + 2]), factor, -ref)), p3 = ex2(fmaf(__uint_as_float(sv[i + 3]), factor, -ref));
+          s0 += p0;
+          s1 += p1;
+          s2 += p2;
+          s3 += p3;
+          sv[i >> 1] = halves(p0, p1);
+          sv[(i >> 1) + 1] = halves(p2, p3);
+        }
+        sum = sum * alpha + ((s0 + s1) + (s2 + s3));
+        if (j > 0) {
+          // the product of the tile before has been added to O.  Looked at in every tile, so that no phase of the barrier is missed
+          ptx::mbar_wait(o_done(w), (g - 1) & 1);
+          if (move) {
+            ptx::tcgen05_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              uint32_t v[32];
+              ptx::tmem_ld_32x32b_x32(tmem_o(w) + lane_at + 32 * c, v);
+              ptx::tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
+              ptx::tmem_st_32x32b_x32(tmem_o(w) + lane_at + 32 * c, v);
+            }
+          }
+        }
+        ptx::tmem_st_32x32b_x32(s_at, sv);
+        ptx::tmem_st_32x32b_x32(s_at + 32, sv + 32);
+        ptx::tmem_st_wait();
+        ptx::tcgen05_fence_before();
+        ptx::mbar_arrive(p_full(w));
+      }
+      // ---- the result, or this CTA's part of it
+      more = next_piece(p, at);
+      ptx::mbar_wait(o_done(w), (g - 1) & 1);
+      ptx::tcgen05_fence_after();
+      const bool begins = x.t == 0, ends = x.end == x.tiles;
+      if (begins && ends) {
+        const float inv = sum == 0.f ? 0.f : 1.0f / sum;   // seen nothing: zeros
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {                      // through the tile's Q, which every product has read
+          uint32_t v[32];
+          ptx::tmem_ld_32x32b_x32(tmem_o(w) + lane_at + 32 * c, v);
+          ptx::tmem_ld_wait();
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint4 y;
+            y.x = pack_bf16(__uint_as_float(v[8 * k]) * inv, __uint_as_float(v[8 * k + 1]) * inv);
+            y.y = pack_bf16(__uint_as_float(v[8 * k + 2]) * inv, __uint_as_float(v[8 * k + 3]) * inv);
+            y.z = pack_bf16(__uint_as_float(v[8 * k + 4]) * inv, __uint_as_float(v[8 * k + 5]) * inv);
+            y.w = pack_bf16(__uint_as_float(v[8 * k + 6]) * inv, __uint_as_float(v[8 * k + 7]) * inv);
+            *reinterpret_cast<uint4*>(q_tile + (c >> 1) * kHalf + r * 128 + (((4 * (c & 1) + k) ^ (r & 7)) << 4)) = y;
+          }
+        }
+        __syncwarp();
+#pragma unroll 4
+        for (int i = 0; i < 16; ++i) {
+          const int in_tile = quad * 32 + 2 * i + (lane >> 4), row = first + in_tile, tk = p.by_group(row), at_row = x.s.begin + tk, c = lane & 15;
+          const uint4 y = *reinterpret_cast<const uint4*>(q_tile + (c >> 3) * kHalf + in_tile * 128 + (((c & 7) ^ (in_tile & 7)) << 4));
+          if (row < real && (unsigned)at_row < (unsigned)p.rows)
+            reinterpret_cast<uint4*>(p.out + at_row * p.ldo + (int64_t)(x.h * p.group + row - tk * p.group) * 128)[c] = y;
+        }
+        __syncwarp();
+      } else {
+        if (begins) note = make_int4(x.b, x.j, x.h, (int)blockIdx.x + 1 + (x.tiles - 1 - x.end) / per);
+        float* part = p.parts + ((int64_t)blockIdx.x * 2 + (begins ? 1 : 0)) * kRecord;
+        const int row = 128 * w + r;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t v[32];
+          ptx::tmem_ld_32x32b_x32(tmem_o(w) + lane_at + 32 * c, v);
+          ptx::tmem_ld_wait();
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            __stcg(reinterpret_cast<float4*>(part) + (8 * c + k) * kRows + row, make_float4(__uint_as_float(v[4 * k]), __uint_as_float(v[4 * k + 1]), __uint_as_float(v[4 * k + 2]), __uint_as_float(v[4 * k + 3])));
+        }
+        __stcg(part + kRows * 128 + row, sum == 0.f ? kFloor : ref);
+        __stcg(part + kRows * 129 + row, sum);
+      }
+      ptx::tcgen05_fence_before();                         // O has been read: the next P V may write it (p_full)
+    }
+    if (threadIdx.x == 0) p.notes[blockIdx.x] = note;
+  }
+  ptx::tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    ptx::tcgen05_fence_after();
+    ptx::tmem_dealloc(tmem, 512);
+  }
+}
+
+// Units that lie in several CTAs, by the CTA in which they begin: 32 rows of it a CTA (8 of them a unit), a thread for a row and four dims at a time.
+__global__ void __launch_bounds__(256) combine_kernel(const Args p) {
+  pdl_trigger();
+  const int c0 = blockIdx.x >> 3, lane = threadIdx.x & 31, row = (blockIdx.x & 7) * 32 + lane, d0 = threadIdx.x >> 5;
+  pdl_wait();
+  const int4 note = __ldcg(p.notes + c0);
+  if (note.x < 0) return;
+  const int c1 = note.w;
+  auto record = [&](int i) { return p.parts + ((int64_t)i * 2 + (i == c0 ? 1 : 0)) * kRecord; };
+  float top = kFloor, l = 0.f;
+  for (int i = c0; i <= c1; ++i) top = fmaxf(top, __ldcg(record(i) + kRows * 128 + row));
+  float4 v[4] = {};
+  for (int i = c0; i <= c1; ++i) {
+    const float* rec = record(i);
+    const float f = ex2(__ldcg(rec + kRows * 128 + row) - top);
+    l += __ldcg(rec + kRows * 129 + row) * f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {                          // dims 16 d0 + 4 k ..
+      const float4 y = __ldcg(reinterpret_cast<const float4*>(rec) + (4 * d0 + k) * kRows + row);
+      v[k].x += y.x * f; v[k].y += y.y * f; v[k].z += y.z * f; v[k].w += y.w * f;
+    }
+  }
+  const Seq s = seq_of(p, note.x);
+  const int packed = kRows * note.y + row, tok = p.by_group(packed), at_row = s.begin + tok;
+  if (packed >= s.qlen * p.group || (unsigned)at_row >= (unsigned)p.rows) return;
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  uint4* dst = reinterpret_cast<uint4*>(p.out + at_row * p.ldo + (int64_t)(note.z * p.group + packed - tok * p.group) * 128) + 2 * d0;
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    dst[k] = make_uint4(pack_bf16(v[2 * k].x * inv, v[2 * k].y * inv), pack_bf16(v[2 * k].z * inv, v[2 * k].w * inv), pack_bf16(v[2 * k + 1].x * inv, v[2 * k + 1].y * inv),
+                        pack_bf16(v[2 * k + 1].z * inv, v[2 * k + 1].w * inv));
+}
+
+}  // namespace fp4p

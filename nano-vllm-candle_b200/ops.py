@@ -1237,7 +1237,7 @@ def read_kvcache_fp4(ctx, cache: Fp4Cache, slots):
     return k, ks, v, vs
 
 
-def _attn_fp4(ctx, q, cache, block_tables, context_lens, nh, out, B):
+def _attn_fp4(ctx, q, cache, block_tables, context_lens, nh, out, B, most: int):
     """Checks of both attentions: (addresses and strides of q, tables, lengths and the result, the result, the workspace)."""
     width, rows = nh * 128, q.shape[0] if q.dim() else 0
     ldq = _rows_stride(ctx, "q", q, rows, width)
@@ -1250,7 +1250,7 @@ def _attn_fp4(ctx, q, cache, block_tables, context_lens, nh, out, B):
         ldo = _rows_stride(ctx, "out", out, rows, width)
     if (rows | B | nh | ldq | ldo | block_tables.shape[1]) >> 31:
         raise ValueError(_TOO_FAR)
-    need = ctx.l.nvc_attn_fp4_workspace_bytes(ctx.h, nh, cache.kv)
+    need = ctx.l.nvc_attn_fp4_workspace_bytes(ctx.h, nh, cache.kv, min(most, rows))
     ws = q.new_empty(need, dtype=torch.uint8)          # of this call alone: other streams and captured graphs have their own
     return rows, ldq, lens, out, ldo, ws, need
 
@@ -1258,7 +1258,7 @@ def _attn_fp4(ctx, q, cache, block_tables, context_lens, nh, out, B):
 def paged_decode_attn_fp4(ctx, q, cache: Fp4Cache, block_tables, context_lens, nh: int, scale: float, out=None) -> torch.Tensor:
     """paged_decode_attn over a cache in 4 bits.  q: bf16 [B, nh * 128] (rows of any stride that is a multiple of 8), block_tables int32 [B, max_blocks], context_lens int32 [B] (0: zeros)."""
     at, B = _fp4_cache_given(ctx, cache), q.shape[0] if q.dim() else 0
-    _, ldq, lens, out, ldo, ws, need = _attn_fp4(ctx, q, cache, block_tables, context_lens, nh, out, B)
+    _, ldq, lens, out, ldo, ws, need = _attn_fp4(ctx, q, cache, block_tables, context_lens, nh, out, B, 1)
     if B:
         st = ctx.l.nvc_paged_decode_attn_fp4(ctx.h, q.data_ptr(), ldq, at, block_tables.data_ptr(), block_tables.shape[1], lens, B, nh, scale, out.data_ptr(), ldo, ws.data_ptr(), need,
                                              torch._C._cuda_getCurrentRawStream(ctx.device))
@@ -1273,10 +1273,10 @@ def prefill_attn_paged_fp4(ctx, q, cache: Fp4Cache, block_tables, context_lens, 
     at, B = _fp4_cache_given(ctx, cache), cu_seqlens_q.numel() - 1
     if B < 0:
         raise ValueError("cu_seqlens_q must have B + 1 entries")
-    rows, ldq, lens, out, ldo, ws, need = _attn_fp4(ctx, q, cache, block_tables, context_lens, nh, out, B)
-    cu = _numbers(ctx, "cu_seqlens_q", cu_seqlens_q, B + 1)
     if max_seqlen_q >> 31:
         raise ValueError(_TOO_FAR)
+    cu = _numbers(ctx, "cu_seqlens_q", cu_seqlens_q, B + 1)
+    rows, ldq, lens, out, ldo, ws, need = _attn_fp4(ctx, q, cache, block_tables, context_lens, nh, out, B, max_seqlen_q)
     if rows and B:
         st = ctx.l.nvc_prefill_attn_paged_fp4(ctx.h, q.data_ptr(), ldq, at, block_tables.data_ptr(), block_tables.shape[1], lens, cu, B, rows, max_seqlen_q, nh, scale, out.data_ptr(), ldo,
                                               ws.data_ptr(), need, torch._C._cuda_getCurrentRawStream(ctx.device))
