@@ -68,8 +68,42 @@ __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
+// two fp32 numbers in a register pair, and operations on both at once
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ float lo_of(uint64_t x) { return __uint_as_float((uint32_t)x); }
+__device__ __forceinline__ float hi_of(uint64_t x) { return __uint_as_float((uint32_t)(x >> 32)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, uint32_t b, uint32_t c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(__uint_as_float(b)), "f"(__uint_as_float(c)));
+  return d;
+}
+__device__ __forceinline__ void tmem_st_x16(uint32_t at, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+               "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
 // instruction descriptor: fp16 x fp16 -> fp32 (formats 0), M = N = 128
 __host__ __device__ constexpr uint32_t idesc(int b_mn_major) { return (1u << 4) | ((uint32_t)b_mn_major << 16) | (128u >> 3 << 17) | (128u >> 4 << 24); }
+
+// (without the message of ptx::mbar_wait: a call takes registers from the code around it)
+__device__ __forceinline__ void wait_bar(uint32_t bar, uint32_t parity) {
+  uint32_t spins = 0;
+  while (!ptx::mbar_try_wait(bar, parity))
+    if (++spins > NVC_MBAR_SPIN_LIMIT) __trap();
+}
 
 struct Seq { int len, qlen, begin, blocks; };              // begin: its first row; blocks: units of 256 rows
 __device__ __forceinline__ Seq seq_of(const Args& p, int b) {
@@ -213,6 +247,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const Args p) {
   auto s_full = [&](int w) { return bar0 + 8u * (10 + w); };
   auto p_full = [&](int w) { return bar0 + 8u * (12 + w); };
   auto o_done = [&](int w) { return bar0 + 8u * (14 + w); };
+  auto s_read = [&](int w) { return bar0 + 8u * (16 + w); };
   const uint32_t tmem_slot = bar0 + 8u * kNumBars;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -221,12 +256,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const Args p) {
       for (int i = 0; i < 2; ++i) {
         ptx::mbar_init(q_full(i), 128);
         ptx::mbar_init(k_full(i), 128);
-        ptx::mbar_init(k_empty(i), 1);
+        ptx::mbar_init(k_empty(i), 2);
         ptx::mbar_init(v_full(i), 128);
-        ptx::mbar_init(v_empty(i), 1);
+        ptx::mbar_init(v_empty(i), 2);
         ptx::mbar_init(s_full(i), 1);
         ptx::mbar_init(p_full(i), 128);
         ptx::mbar_init(o_done(i), 1);
+        ptx::mbar_init(s_read(i), 128);
       }
       ptx::fence_barrier_init();
     }
@@ -243,7 +279,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const Args p) {
   __syncthreads();
   ptx::tcgen05_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(gen + kOffBar + kNumBars * 8);
-  auto tmem_s = [&](int w) { return tmem + 128u * w; };
+  // S of one tile at a time; its reader takes all of it into registers at once.  P of each tile, O of each tile
+  const uint32_t tmem_s = tmem;
+  auto tmem_p = [&](int w) { return tmem + 128u + 64u * w; };
   auto tmem_o = [&](int w) { return tmem + 256u + 128u * w; };
   pdl_wait();
 
@@ -251,56 +289,54 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const Args p) {
     if (threadIdx.x == 0) p.notes[blockIdx.x] = make_int4(-1, 0, 0, 0);
   } else if (warp >= 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-    // ------------------------------------------------------------ the products (one warp of the four)
-    if (warp == 12) {
+    // ------------------------------------------------------------ the products: a warp for each tile (two of the four).  A product is taken in only when the ones before it are
+    // nearly through, so that one warp's waits would leave the tensor cores without work
+    if (warp < 14) {
       constexpr uint32_t hi = ptx::umma_desc_hi_sw128(1024);
-      auto issue_s = [&](int w, uint32_t g) {
-        if (ptx::elect_one()) {
-          const uint32_t q_lo = ptx::umma_desc_lo(base + kOffQ + w * kTileBytes, 16), k_lo = ptx::umma_desc_lo(base + kOffK + (g & 1) * kTileBytes, 16);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const uint32_t off = ((k >> 2) * kHalf + (k & 3) * 32) >> 4;
-            ptx::umma_bf16_ss(tmem_s(w), ptx::umma_desc(q_lo + off, hi), ptx::umma_desc(k_lo + off, hi), idesc(0), k != 0);
-          }
-          ptx::umma_commit(s_full(w));
-          if (w == 1) ptx::umma_commit(k_empty(g & 1));
-        }
-        __syncwarp();
-      };
+      const int w = warp - 12;
       uint32_t g = 0, done = 0;
       bool more = true;
       while (more) {
         const int n = at.end - at.t;
-        ptx::mbar_wait(k_full(g & 1), (g >> 1) & 1);
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          ptx::mbar_wait(q_full(w), done & 1);
-          ptx::tcgen05_fence_after();
-          issue_s(w, g);
-        }
-        for (int j = 0; j < n; ++j, ++g) {
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            ptx::mbar_wait(p_full(w), g & 1);              // P is there, O rescaled (or, in a piece's first tile, read out)
-            if (w == 0) ptx::mbar_wait(v_full(g & 1), (g >> 1) & 1);
+        wait_bar(q_full(w), done & 1);
+        // S_w(j), then P_w(j - 1) V: the tile's softmax finds its next S when it is through with one
+        for (int j = 0; j <= n; ++j) {
+          // (operands' addresses are hidden from the compiler: it would keep all of them for all stages)
+          if (j < n) {
+            const uint32_t k = g + j;
+            uint32_t q_lo = ptx::umma_desc_lo(base + kOffQ + w * kTileBytes, 16), k_lo = ptx::umma_desc_lo(base + kOffK + (k & 1) * kTileBytes, 16);
+            asm volatile("" : "+r"(q_lo), "+r"(k_lo));
+            wait_bar(k_full(k & 1), (k >> 1) & 1);
+            wait_bar(s_read(w ^ 1), (k & 1) ^ (w ^ 1));    // the S before this one, of the other tile, has been read: tile 0's waits for tile 1's of k - 1
             ptx::tcgen05_fence_after();
             if (ptx::elect_one()) {
-              const uint32_t v_lo = ptx::umma_desc_lo(base + kOffV + (g & 1) * kTileBytes, (uint32_t)kHalf);       // dims are its rows: 16 tokens a step
 #pragma unroll
-              for (int k = 0; k < 8; ++k) ptx::umma_bf16_ts(tmem_o(w), tmem_s(w) + k * 8, ptx::umma_desc(v_lo + k * (2048 >> 4), hi), idesc(1), (j | k) != 0);
-              ptx::umma_commit(o_done(w));
-              if (w == 1) ptx::umma_commit(v_empty(g & 1));
+              for (int i = 0; i < 8; ++i) {
+                const uint32_t off = ((i >> 2) * kHalf + (i & 3) * 32) >> 4;
+                ptx::umma_bf16_ss(tmem_s, ptx::umma_desc(q_lo + off, hi), ptx::umma_desc(k_lo + off, hi), idesc(0), i != 0);
+              }
+              ptx::umma_commit(s_full(w));
+              ptx::umma_commit(k_empty(k & 1));
             }
             __syncwarp();
-            if (j + 1 < n) {
-              if (w == 0) {
-                ptx::mbar_wait(k_full((g + 1) & 1), ((g + 1) >> 1) & 1);
-                ptx::tcgen05_fence_after();
-              }
-              issue_s(w, g + 1);
+          }
+          if (j > 0) {
+            const uint32_t k = g + j - 1;
+            uint32_t v_lo = ptx::umma_desc_lo(base + kOffV + (k & 1) * kTileBytes, (uint32_t)kHalf), from = tmem_p(w), to = tmem_o(w);       // dims are V's rows: 16 tokens a step
+            asm volatile("" : "+r"(v_lo), "+r"(from), "+r"(to));
+            wait_bar(v_full(k & 1), (k >> 1) & 1);
+            wait_bar(p_full(w), k & 1);                    // P is there, O rescaled (or, in a piece's first tile, read out)
+            ptx::tcgen05_fence_after();
+            if (ptx::elect_one()) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) ptx::umma_bf16_ts(to, from + i * 8, ptx::umma_desc(v_lo + i * (2048 >> 4), hi), idesc(1), j > 1 || i != 0);
+              ptx::umma_commit(o_done(w));
+              ptx::umma_commit(v_empty(k & 1));
             }
+            __syncwarp();
           }
         }
+        g += n;
         ++done;
         more = next_piece(p, at);
       }
@@ -359,7 +395,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const Args p) {
     while (more) {
       const Piece x = at;
       more = next_piece(p, at);
-      ptx::mbar_wait(k_empty(g & 1), ((g >> 1) & 1) ^ 1u);
+      wait_bar(k_empty(g & 1), ((g >> 1) & 1) ^ 1u);
       write(rk, base + kOffK + (g & 1) * kTileBytes, k_full(g & 1));
       if (x.t + 1 < x.end) rk = load(x, x.t + 1, b2, p.kc, p.ks);
       else if (more) rk = load(at, at.t, block_of(at, at.t), p.kc, p.ks);
@@ -367,12 +403,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const Args p) {
         // b2: the next tile's block; K runs a tile ahead of V
         b3 = j + 2 < x.end ? block_of(x, j + 2) : -1;
         if (j + 1 < x.end) {
-          ptx::mbar_wait(k_empty((g + 1) & 1), (((g + 1) >> 1) & 1) ^ 1u);
+          wait_bar(k_empty((g + 1) & 1), (((g + 1) >> 1) & 1) ^ 1u);
           write(rk, base + kOffK + ((g + 1) & 1) * kTileBytes, k_full((g + 1) & 1));
           if (j + 2 < x.end) rk = load(x, j + 2, b3, p.kc, p.ks);
           else if (more) rk = load(at, at.t, block_of(at, at.t), p.kc, p.ks);
         }
-        ptx::mbar_wait(v_empty(g & 1), ((g >> 1) & 1) ^ 1u);
+        wait_bar(v_empty(g & 1), ((g >> 1) & 1) ^ 1u);
         write(rv, base + kOffV + (g & 1) * kTileBytes, v_full(g & 1));
         if (j + 1 < x.end) rv = load(x, j + 1, b2, p.vc, p.vs);
         b2 = b3;
@@ -433,28 +469,34 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const Args p) {
       float ref = kFloor, sum = 0.f;
       const int n = x.end - x.t;
       for (int j = 0; j < n; ++j, ++g) {
-        const uint32_t s_at = tmem_s(w) + lane_at;
-        ptx::mbar_wait(s_full(w), g & 1);
+        wait_bar(s_full(w), g & 1);
         ptx::tcgen05_fence_after();
-        uint32_t sv[128];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) ptx::tmem_ld_32x32b_x32(s_at + 32 * c, sv + 32 * c);
-        ptx::tmem_ld_wait();
         const int t0 = (x.t + j) * kKT;
-        if (t0 + kKT - 1 > least) {
-          const int l = lim - t0;
-#pragma unroll
-          for (int i = 0; i < 128; ++i)
-            if (i > l) sv[i] = 0xff800000u;
-        }
+        const bool cut = t0 + kKT - 1 > least;
+        const int l = lim - t0;
+        uint32_t sv[128];
         float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
+        ptx::tmem_ld_32x32b_x32(tmem_s + lane_at, sv);
+        ptx::tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 128; i += 4) {
-          m0 = fmaxf(m0, __uint_as_float(sv[i]));
-          m1 = fmaxf(m1, __uint_as_float(sv[i + 1]));
-          m2 = fmaxf(m2, __uint_as_float(sv[i + 2]));
-          m3 = fmaxf(m3, __uint_as_float(sv[i + 3]));
+        for (int c = 0; c < 4; ++c) {                        // the next columns are on their way while these are looked at
+          if (c < 3) ptx::tmem_ld_32x32b_x32(tmem_s + lane_at + 32 * (c + 1), sv + 32 * (c + 1));
+          if (cut) {
+#pragma unroll
+            for (int i = 32 * c; i < 32 * c + 32; ++i)
+              if (i > l) sv[i] = 0xff800000u;
+          }
+#pragma unroll
+          for (int i = 32 * c; i < 32 * c + 32; i += 8) {
+            m0 = max3(m0, sv[i], sv[i + 1]);
+            m1 = max3(m1, sv[i + 2], sv[i + 3]);
+            m2 = max3(m2, sv[i + 4], sv[i + 5]);
+            m3 = max3(m3, sv[i + 6], sv[i + 7]);
+          }
+          if (c < 3) ptx::tmem_ld_wait();
         }
+        ptx::tcgen05_fence_before();
+        ptx::mbar_arrive(s_read(w));
         const float top = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * factor - kShift;
         const bool move = __any_sync(0xffffffffu, top > ref + kGrow);
         float alpha = 1.0f;
@@ -463,44 +505,48 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const Args p) {
           alpha = ex2(ref - now);
           ref = now;
         }
-        float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+        uint64_t s0 = 0, s1 = 0;                           // two sums each
+        const uint64_t by = pair(factor, factor), less = pair(-ref, -ref);
+        auto weights = [&](int from) {                     // of 64 columns
 #pragma unroll
-        for (int i = 0; i < 128; i += 4) {
-          const float p0 = ex2(fmaf(__uint_as_float(sv[i]), factor, -ref)), p1 = ex2(fmaf(__uint_as_float(sv[i + 1]), factor, -ref));
-          const float p2 = ex2(fmaf(__uint_as_float(sv[i + 2]), factor, -ref)), p3 = ex2(fmaf(__uint_as_float(sv[i + 3]), factor, -ref));
-          s0 += p0;
-          s1 += p1;
-          s2 += p2;
-          s3 += p3;
-          sv[i >> 1] = halves(p0, p1);
-          sv[(i >> 1) + 1] = halves(p2, p3);
-        }
-        sum = sum * alpha + ((s0 + s1) + (s2 + s3));
+          for (int i = from; i < from + 64; i += 4) {
+            const uint64_t y = fma2(pair(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])), by, less), z = fma2(pair(__uint_as_float(sv[i + 2]), __uint_as_float(sv[i + 3])), by, less);
+            const float p0 = ex2(lo_of(y)), p1 = ex2(hi_of(y)), p2 = ex2(lo_of(z)), p3 = ex2(hi_of(z));
+            s0 = add2(s0, pair(p0, p1));
+            s1 = add2(s1, pair(p2, p3));
+            sv[i >> 1] = halves(p0, p1);
+            sv[(i >> 1) + 1] = halves(p2, p3);
+          }
+        };
+        weights(0);
         if (j > 0) {
           // the product of the tile before has been added to O.  Looked at in every tile, so that no phase of the barrier is missed
-          ptx::mbar_wait(o_done(w), (g - 1) & 1);
+          wait_bar(o_done(w), (g - 1) & 1);
           if (move) {
             ptx::tcgen05_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              uint32_t v[32];
-              ptx::tmem_ld_32x32b_x32(tmem_o(w) + lane_at + 32 * c, v);
+            for (int c = 0; c < 8; ++c) {
+              uint32_t v[16];
+              ptx::tmem_ld_32x32b_x16(tmem_o(w) + lane_at + 16 * c, v);
               ptx::tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
-              ptx::tmem_st_32x32b_x32(tmem_o(w) + lane_at + 32 * c, v);
+              for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
+              tmem_st_x16(tmem_o(w) + lane_at + 16 * c, v);
             }
           }
         }
-        ptx::tmem_st_32x32b_x32(s_at, sv);
-        ptx::tmem_st_32x32b_x32(s_at + 32, sv + 32);
+        ptx::tmem_st_32x32b_x32(tmem_p(w) + lane_at, sv);
+        weights(64);
+        s0 = add2(s0, s1);
+        sum = sum * alpha + (lo_of(s0) + hi_of(s0));
+        ptx::tmem_st_32x32b_x32(tmem_p(w) + lane_at + 32, sv + 32);
         ptx::tmem_st_wait();
         ptx::tcgen05_fence_before();
         ptx::mbar_arrive(p_full(w));
       }
       // ---- the result, or this CTA's part of it
       more = next_piece(p, at);
-      ptx::mbar_wait(o_done(w), (g - 1) & 1);
+      wait_bar(o_done(w), (g - 1) & 1);
       ptx::tcgen05_fence_after();
       const bool begins = x.t == 0, ends = x.end == x.tiles;
       if (begins && ends) {
