@@ -23,7 +23,7 @@ constexpr int kHalf = kTileBytes / 2;
 constexpr int kOffQ = 0, kOffK = 2 * kTileBytes, kOffV = kOffK + 2 * kTileBytes, kOffFactor = kOffV + 2 * kTileBytes, kOffBar = kOffFactor + kRows * 4;
 constexpr int kNumBars = 18;
 constexpr int kSmemBytes = kOffBar + kNumBars * 8 + 16 + 1024;          // and room to begin at a multiple of 1024
-constexpr int kUnitCost = 2;                               // a unit's queries and result, in tiles
+constexpr int kUnitCost = 4;                               // a unit's queries and result, in tiles (a prompt of 8 191: 2 635 us, 3 534, 4 517, 6 530)
 constexpr float kFloor = -1.0e30f, kShift = 7.0f, kGrow = 8.0f;
 constexpr int kRecord = kRows * 130;                       // floats: O [32 groups of 4 dims][256 rows][4], reference [256], sum [256]
 constexpr int kChunk = 2048;                               // sequences whose weights are looked at together (in shared memory)
@@ -172,7 +172,7 @@ __device__ __forceinline__ bool plan(const Args& p, int64_t* weights, int warp, 
   total = 0;
 #pragma unroll
   for (int i = 0; i < kW; ++i) total += sums[i];
-  per = max((int)((total + gridDim.x - 1) / gridDim.x), 4 + kUnitCost);
+  per = max((int)((total + gridDim.x - 1) / gridDim.x), 2 + kUnitCost);
   int64_t at = (int64_t)per * blockIdx.x;
   if (at >= total) return false;
   int b0 = 0;
@@ -395,10 +395,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const Args p) {
     while (more) {
       const Piece x = at;
       more = next_piece(p, at);
+      const int nb = more ? block_of(at, at.t) : -1;
       wait_bar(k_empty(g & 1), ((g >> 1) & 1) ^ 1u);
       write(rk, base + kOffK + (g & 1) * kTileBytes, k_full(g & 1));
       if (x.t + 1 < x.end) rk = load(x, x.t + 1, b2, p.kc, p.ks);
-      else if (more) rk = load(at, at.t, block_of(at, at.t), p.kc, p.ks);
+      else if (more) rk = load(at, at.t, nb, p.kc, p.ks);
       for (int j = x.t; j < x.end; ++j, ++g) {
         // b2: the next tile's block; K runs a tile ahead of V
         b3 = j + 2 < x.end ? block_of(x, j + 2) : -1;
@@ -406,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const Args p) {
           wait_bar(k_empty((g + 1) & 1), (((g + 1) >> 1) & 1) ^ 1u);
           write(rk, base + kOffK + ((g + 1) & 1) * kTileBytes, k_full((g + 1) & 1));
           if (j + 2 < x.end) rk = load(x, j + 2, b3, p.kc, p.ks);
-          else if (more) rk = load(at, at.t, block_of(at, at.t), p.kc, p.ks);
+          else if (more) rk = load(at, at.t, nb, p.kc, p.ks);
         }
         wait_bar(v_empty(g & 1), ((g >> 1) & 1) ^ 1u);
         write(rv, base + kOffV + (g & 1) * kTileBytes, v_full(g & 1));
@@ -414,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const Args p) {
         b2 = b3;
       }
       if (more) {
-        rv = load(at, at.t, block_of(at, at.t), p.vc, p.vs);
+        rv = load(at, at.t, nb, p.vc, p.vs);
         b2 = at.t + 1 < at.end ? block_of(at, at.t + 1) : -1;
       }
     }
@@ -428,44 +429,56 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const Args p) {
     uint32_t g = 0;
     bool more = true;
     int4 note = make_int4(-1, 0, 0, 0);
-    while (more) {
-      const Piece x = at;
-      const int first = kRows * x.j + 128 * w;             // packed row of the tile's first
-      const int real = x.s.qlen * p.group;                 // (at most 2^31: the host's check)
-      // ---- this warp's 32 rows of Q: 16 lanes a row
-#pragma unroll 1
-      for (int i0 = 0; i0 < 16; i0 += 8) {
-        uint4 y[8];
+    // This warp's 32 rows of a piece's Q, 16 lanes a row: all of it on its way, then to shared memory (that every product of the piece before has read: its last S has been seen)
+    uint4 y[16];
+    auto fetch = [&](const Piece& x) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int row = first + quad * 32 + 2 * (i0 + i) + (lane >> 4), tok = p.by_group(row);
-          const int at_row = x.s.begin + tok;
-          y[i] = make_uint4(0, 0, 0, 0);
-          if (row < real && (unsigned)at_row < (unsigned)p.rows)
-            y[i] = reinterpret_cast<const uint4*>(p.q + at_row * p.ldq + (int64_t)(x.h * p.group + row - tok * p.group) * 128)[lane & 15];
-        }
+      for (int i = 0; i < 16; ++i) {
+        const int row = kRows * x.j + 128 * w + quad * 32 + 2 * i + (lane >> 4), tok = p.by_group(row), at_row = x.s.begin + tok;
+        y[i] = make_uint4(0, 0, 0, 0);
+        if (row < x.s.qlen * p.group && (unsigned)at_row < (unsigned)p.rows)
+          y[i] = reinterpret_cast<const uint4*>(p.q + at_row * p.ldq + (int64_t)(x.h * p.group + row - tok * p.group) * 128)[lane & 15];
+      }
+    };
+    auto place = [&] {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          uint32_t top = fp4_amax8(y[i]);
+      for (int i = 0; i < 16; ++i) {
+        uint32_t top = fp4_amax8(y[i]);
 #pragma unroll
-          for (int d = 1; d < 16; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
-          int e = top >= 0x7f80u || top == 0 ? 0 : (int)(top >> 7) - 127;
-          e = min(max(e, -126), 126);
-          const float down = __uint_as_float((uint32_t)(127 - e) << 23) * p.q_sign;
-          const int row = quad * 32 + 2 * (i0 + i) + (lane >> 4), c = lane & 15;
-          *reinterpret_cast<uint4*>(q_tile + (c >> 3) * kHalf + row * 128 + (((c & 7) ^ (row & 7)) << 4)) =
-              make_uint4(halves(bf16_lo(y[i].x) * down, bf16_hi(y[i].x) * down), halves(bf16_lo(y[i].y) * down, bf16_hi(y[i].y) * down),
-                         halves(bf16_lo(y[i].z) * down, bf16_hi(y[i].z) * down), halves(bf16_lo(y[i].w) * down, bf16_hi(y[i].w) * down));
-          if (c == 0) factors[row] = fmaxf(__uint_as_float((uint32_t)(127 + e) << 23) * p.factor, 1.2e-38f);        // 0 would turn a masked score into a NaN
-        }
+        for (int d = 1; d < 16; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+        int e = top >= 0x7f80u || top == 0 ? 0 : (int)(top >> 7) - 127;
+        e = min(max(e, -126), 126);
+        const float down = __uint_as_float((uint32_t)(127 - e) << 23) * p.q_sign;
+        const int row = quad * 32 + 2 * i + (lane >> 4), c = lane & 15;
+        *reinterpret_cast<uint4*>(q_tile + (c >> 3) * kHalf + row * 128 + (((c & 7) ^ (row & 7)) << 4)) =
+            make_uint4(halves(bf16_lo(y[i].x) * down, bf16_hi(y[i].x) * down), halves(bf16_lo(y[i].y) * down, bf16_hi(y[i].y) * down),
+                       halves(bf16_lo(y[i].z) * down, bf16_hi(y[i].z) * down), halves(bf16_lo(y[i].w) * down, bf16_hi(y[i].w) * down));
+        if (c == 0) factors[row] = fmaxf(__uint_as_float((uint32_t)(127 + e) << 23) * p.factor, 1.2e-38f);        // 0 would turn a masked score into a NaN
       }
       ptx::fence_proxy_async_smem();
       ptx::mbar_arrive(q_full(w));
+    };
+    auto ahead = [&](const Piece& x) {                      // to L2: 32 rows of two lines
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = kRows * x.j + 128 * w + quad * 32 + 16 * i + (lane >> 1), tok = p.by_group(row), at_row = x.s.begin + tok;
+        if (row < x.s.qlen * p.group && (unsigned)at_row < (unsigned)p.rows)
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(p.q + at_row * p.ldq + (int64_t)(x.h * p.group + row - tok * p.group) * 128 + 64 * (lane & 1)));
+      }
+    };
+    fetch(at);
+    place();
+    while (more) {
+      const Piece x = at;
+      more = next_piece(p, at);                            // (its lengths are on their way meanwhile)
+      const int first = kRows * x.j + 128 * w;             // packed row of the tile's first
+      const int real = x.s.qlen * p.group;                 // (at most 2^31: the host's check)
       __syncwarp();
       const float factor = factors[r];
       const int tok = p.by_group(first + r);
       const int lim = x.s.len - x.s.qlen + min(tok, x.s.qlen - 1);          // the last key that the row sees
       const int least = x.s.len - x.s.qlen + p.by_group(first + quad * 32);   // of the warp's rows
+      if (more) ahead(at);
       float ref = kFloor, sum = 0.f;
       const int n = x.end - x.t;
       for (int j = 0; j < n; ++j, ++g) {
@@ -545,36 +558,30 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const Args p) {
         ptx::mbar_arrive(p_full(w));
       }
       // ---- the result, or this CTA's part of it
-      more = next_piece(p, at);
+      if (more) {                                          // the next one's queries first: its S is made while this one's O is written
+        fetch(at);
+        place();
+      }
       wait_bar(o_done(w), (g - 1) & 1);
       ptx::tcgen05_fence_after();
       const bool begins = x.t == 0, ends = x.end == x.tiles;
       if (begins && ends) {
         const float inv = sum == 0.f ? 0.f : 1.0f / sum;   // seen nothing: zeros
+        const int at_row = x.s.begin + tok;
+        const bool there = first + r < real && (unsigned)at_row < (unsigned)p.rows;
+        uint4* dst = reinterpret_cast<uint4*>(p.out + at_row * p.ldo + (int64_t)(x.h * p.group + first + r - tok * p.group) * 128);
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {                      // through the tile's Q, which every product has read
+        for (int c = 0; c < 4; ++c) {
           uint32_t v[32];
           ptx::tmem_ld_32x32b_x32(tmem_o(w) + lane_at + 32 * c, v);
           ptx::tmem_ld_wait();
+          if (there) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            uint4 y;
-            y.x = pack_bf16(__uint_as_float(v[8 * k]) * inv, __uint_as_float(v[8 * k + 1]) * inv);
-            y.y = pack_bf16(__uint_as_float(v[8 * k + 2]) * inv, __uint_as_float(v[8 * k + 3]) * inv);
-            y.z = pack_bf16(__uint_as_float(v[8 * k + 4]) * inv, __uint_as_float(v[8 * k + 5]) * inv);
-            y.w = pack_bf16(__uint_as_float(v[8 * k + 6]) * inv, __uint_as_float(v[8 * k + 7]) * inv);
-            *reinterpret_cast<uint4*>(q_tile + (c >> 1) * kHalf + r * 128 + (((4 * (c & 1) + k) ^ (r & 7)) << 4)) = y;
+            for (int k = 0; k < 4; ++k)
+              dst[4 * c + k] = make_uint4(pack_bf16(__uint_as_float(v[8 * k]) * inv, __uint_as_float(v[8 * k + 1]) * inv), pack_bf16(__uint_as_float(v[8 * k + 2]) * inv, __uint_as_float(v[8 * k + 3]) * inv),
+                                          pack_bf16(__uint_as_float(v[8 * k + 4]) * inv, __uint_as_float(v[8 * k + 5]) * inv), pack_bf16(__uint_as_float(v[8 * k + 6]) * inv, __uint_as_float(v[8 * k + 7]) * inv));
           }
         }
-        __syncwarp();
-#pragma unroll 4
-        for (int i = 0; i < 16; ++i) {
-          const int in_tile = quad * 32 + 2 * i + (lane >> 4), row = first + in_tile, tk = p.by_group(row), at_row = x.s.begin + tk, c = lane & 15;
-          const uint4 y = *reinterpret_cast<const uint4*>(q_tile + (c >> 3) * kHalf + in_tile * 128 + (((c & 7) ^ (in_tile & 7)) << 4));
-          if (row < real && (unsigned)at_row < (unsigned)p.rows)
-            reinterpret_cast<uint4*>(p.out + at_row * p.ldo + (int64_t)(x.h * p.group + row - tk * p.group) * 128)[c] = y;
-        }
-        __syncwarp();
       } else {
         if (begins) note = make_int4(x.b, x.j, x.h, (int)blockIdx.x + 1 + (x.tiles - 1 - x.end) / per);
         float* part = p.parts + ((int64_t)blockIdx.x * 2 + (begins ? 1 : 0)) * kRecord;
@@ -612,18 +619,29 @@ __global__ void __launch_bounds__(256) combine_kernel(const Args p) {
   if (note.x < 0) return;
   const int c1 = note.w;
   auto record = [&](int i) { return p.parts + ((int64_t)i * 2 + (i == c0 ? 1 : 0)) * kRecord; };
+  // two records (most units lie in two CTAs) on their way at once, the sums against the larger reference so far
   float top = kFloor, l = 0.f;
-  for (int i = c0; i <= c1; ++i) top = fmaxf(top, __ldcg(record(i) + kRows * 128 + row));
   float4 v[4] = {};
-  for (int i = c0; i <= c1; ++i) {
-    const float* rec = record(i);
-    const float f = ex2(__ldcg(rec + kRows * 128 + row) - top);
-    l += __ldcg(rec + kRows * 129 + row) * f;
+  for (int i = c0; i <= c1; i += 2) {
+    const float *a = record(i), *b = record(min(i + 1, c1));
+    float4 x[4], y[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {                          // dims 16 d0 + 4 k ..
-      const float4 y = __ldcg(reinterpret_cast<const float4*>(rec) + (4 * d0 + k) * kRows + row);
-      v[k].x += y.x * f; v[k].y += y.y * f; v[k].z += y.z * f; v[k].w += y.w * f;
+      x[k] = __ldcg(reinterpret_cast<const float4*>(a) + (4 * d0 + k) * kRows + row);
+      y[k] = __ldcg(reinterpret_cast<const float4*>(b) + (4 * d0 + k) * kRows + row);
     }
+    const float ra = __ldcg(a + kRows * 128 + row), rb = i < c1 ? __ldcg(b + kRows * 128 + row) : kFloor;
+    const float la = __ldcg(a + kRows * 129 + row), lb = i < c1 ? __ldcg(b + kRows * 129 + row) : 0.f;
+    const float now = fmaxf(top, fmaxf(ra, rb)), f = ex2(top - now), fa = ex2(ra - now), fb = i < c1 ? ex2(rb - now) : 0.f;
+    l = l * f + la * fa + lb * fb;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      v[k].x = v[k].x * f + x[k].x * fa + y[k].x * fb;
+      v[k].y = v[k].y * f + x[k].y * fa + y[k].y * fb;
+      v[k].z = v[k].z * f + x[k].z * fa + y[k].z * fb;
+      v[k].w = v[k].w * f + x[k].w * fa + y[k].w * fb;
+    }
+    top = now;
   }
   const Seq s = seq_of(p, note.x);
   const int packed = kRows * note.y + row, tok = p.by_group(packed), at_row = s.begin + tok;
