@@ -3,6 +3,8 @@
 #include "fp4.cuh"
 #include "internal.h"
 
+#include <algorithm>
+
 namespace {
 
 struct StoreArgs {
@@ -21,24 +23,46 @@ struct StoreArgs {
 };
 
 // 8 lanes per (token, head): lane l owns the numbers [8l, 8l + 8) and [64 + 8l, 64 + 8l + 8), so that a rotation's pairs are one lane's and a block of 16 is two
-// neighbouring lanes'.  Memory-bound: per token (nh + 2 kv) * 256 bytes in, nh * 256 (and kv * 256 in place) + kv * 144 out.
-__global__ void __launch_bounds__(256) store_fp4_kernel(const StoreArgs p) {
+// neighbouring lanes'.  A warp takes `span` fours of one token's heads, so that the token's angles, slot and the norms' weights are read once for them, two fours ahead of their use.
+// Memory-bound: per token (nh + 2 kv) * 256 bytes in, nh * 256 (and kv * 256 in place) + kv * 144 out.
+__global__ void __launch_bounds__(128) store_fp4_kernel(const StoreArgs p, int span, int warps_per_token) {
   pdl_trigger();
   const int units = p.nh + 2 * p.kv;
-  const int64_t unit = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 3;
-  const int l = threadIdx.x & 7;
-  const unsigned mask = 0xffu << ((threadIdx.x & 31) & ~7);
+  const int64_t warp = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, l = lane & 7;
+  const unsigned mask = 0xffu << (lane & ~7);
+  const int n = (int)(warp / warps_per_token), first = (int)(warp - (int64_t)n * warps_per_token) * span;
   pdl_wait();
-  if (unit >= (int64_t)p.N * units) return;
-  const int n = (int)(unit / units), u = (int)(unit - (int64_t)n * units);
-  const bool is_q = u < p.nh, is_v = u >= p.nh + p.kv;
-  const int h = is_q ? u : is_v ? u - p.nh - p.kv : u - p.nh;
-  const nvc_bf16* src = is_q ? p.q + n * p.ldq : is_v ? p.v + n * p.ldv : p.k + n * p.ldk;
-  const uint4* row = reinterpret_cast<const uint4*>(src + (int64_t)h * 128);
-  uint4 a = ld_once_u4(row + l), b = ld_once_u4(row + l + 8);
-  if (!is_v && p.table) {
+  if (n >= p.N) return;
+  auto source = [&](int u) {
+    const nvc_bf16* src = u < p.nh ? p.q + n * p.ldq : u < p.nh + p.kv ? p.k + n * p.ldk : p.v + n * p.ldv;
+    const int h = u < p.nh ? u : u < p.nh + p.kv ? u - p.nh : u - p.nh - p.kv;
+    return reinterpret_cast<const uint4*>(src + (int64_t)h * 128);
+  };
+  constexpr int kAhead = 2;
+  uint4 a[kAhead], b[kAhead];
+  auto load = [&](int i, uint4& x, uint4& y) {
+    const int u = 4 * (first + i) + (lane >> 3);
+    if (i < span && u < units) {
+      const uint4* row = source(u);
+      x = ld_once_u4(row + l);
+      y = ld_once_u4(row + l + 8);
+    } else {
+      x = y = make_uint4(0, 0, 0, 0);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) load(i, a[i], b[i]);
+  const int slot = p.slot_mapping[n];
+  float4 c0, c1, s0, s1;
+  uint4 wq0 = make_uint4(0, 0, 0, 0), wq1 = wq0, wk0 = wq0, wk1 = wq0;
+  c0 = c1 = s0 = s1 = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (p.table) {
     const int pos = p.positions[n];
-    float4 c0, c1, s0, s1;
+    if (p.qw) {
+      wq0 = p.qw[l]; wq1 = p.qw[l + 8];
+      wk0 = p.kw[l]; wk1 = p.kw[l + 8];
+    }
     if ((unsigned)pos < (unsigned)p.max_pos) {
       const float4* cs = p.table + (int64_t)pos * 32;                        // cos[64], sin[64]
       c0 = cs[2 * l]; c1 = cs[2 * l + 1]; s0 = cs[16 + 2 * l]; s1 = cs[16 + 2 * l + 1];
@@ -46,36 +70,48 @@ __global__ void __launch_bounds__(256) store_fp4_kernel(const StoreArgs p) {
       const float bad = __uint_as_float(0x7fffffffu);
       c0 = c1 = s0 = s1 = make_float4(bad, bad, bad, bad);
     }
-    const uint4* w = is_q ? p.qw : p.kw;
-    uint4 w_lo = make_uint4(0, 0, 0, 0), w_hi = w_lo;
-    if (w) { w_lo = w[l]; w_hi = w[l + 8]; }
-    uint4 o1, o2;
-    qk_norm_rope8(a, b, mask, w != nullptr, w_lo, w_hi, p.eps, c0, c1, s0, s1, o1, o2);
-    a = o1;
-    b = o2;
-    nvc_bf16* out = is_q ? p.q_out + n * p.ldqo : p.k_out ? p.k_out + n * p.ldko : nullptr;
-    if (out) {
-      uint4* o = reinterpret_cast<uint4*>(out + (int64_t)h * 128);
-      o[l] = a;
-      o[l + 8] = b;
-    }
   }
-  if (is_q) return;
-  const int slot = p.slot_mapping[n];
-  uint32_t ma = fp4_amax8(a), mb = fp4_amax8(b);
-  ma = max(ma, __shfl_xor_sync(mask, ma, 1));
-  mb = max(mb, __shfl_xor_sync(mask, mb, 1));
-  if ((unsigned)slot >= (unsigned)p.slots) return;
-  const uint32_t sa = fp4_scale_byte(ma), sb = fp4_scale_byte(mb);
-  const int block = slot / p.block_size;
-  const int64_t at = ((int64_t)block * p.kv + h) * p.block_size + (slot - block * p.block_size);
-  uint32_t* codes = reinterpret_cast<uint32_t*>((is_v ? p.vc : p.kc) + at * kFp4Codes);
-  uint8_t* scales = (is_v ? p.vs : p.ks) + at * kFp4Scales;
-  codes[l] = sa == 255u ? 0u : fp4_codes8(a, fp4_inverse(sa));
-  codes[l + 8] = sb == 255u ? 0u : fp4_codes8(b, fp4_inverse(sb));
-  if (!(l & 1)) {
-    scales[l >> 1] = (uint8_t)sa;
-    scales[4 + (l >> 1)] = (uint8_t)sb;
+  const bool stored = (unsigned)slot < (unsigned)p.slots;
+  const int block = stored ? slot / p.block_size : 0;
+  const int64_t page_row = (int64_t)block * p.kv * p.block_size + (stored ? slot - block * p.block_size : 0);
+#pragma unroll 1
+  for (int i0 = 0; i0 < span; i0 += kAhead) {
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      uint4 x = a[j], y = b[j];
+      load(i0 + j + kAhead, a[j], b[j]);
+      const int u = 4 * (first + i0 + j) + (lane >> 3);
+      if (i0 + j >= span || u >= units) continue;                            // (a unit's eight lanes alike)
+      const bool is_q = u < p.nh, is_v = u >= p.nh + p.kv;
+      const int h = is_q ? u : is_v ? u - p.nh - p.kv : u - p.nh;
+      if (!is_v && p.table) {
+        uint4 o1, o2;
+        qk_norm_rope8(x, y, mask, p.qw != nullptr, is_q ? wq0 : wk0, is_q ? wq1 : wk1, p.eps, c0, c1, s0, s1, o1, o2);
+        x = o1;
+        y = o2;
+        nvc_bf16* out = is_q ? p.q_out + n * p.ldqo : p.k_out ? p.k_out + n * p.ldko : nullptr;
+        if (out) {
+          uint4* o = reinterpret_cast<uint4*>(out + (int64_t)h * 128);
+          o[l] = x;
+          o[l + 8] = y;
+        }
+      }
+      if (is_q) continue;
+      uint32_t ma = fp4_amax8(x), mb = fp4_amax8(y);
+      ma = max(ma, __shfl_xor_sync(mask, ma, 1));
+      mb = max(mb, __shfl_xor_sync(mask, mb, 1));
+      if (!stored) continue;
+      const uint32_t sa = fp4_scale_byte(ma), sb = fp4_scale_byte(mb);
+      const int64_t at = page_row + (int64_t)h * p.block_size;
+      uint32_t* codes = reinterpret_cast<uint32_t*>((is_v ? p.vc : p.kc) + at * kFp4Codes);
+      uint8_t* scales = (is_v ? p.vs : p.ks) + at * kFp4Scales;
+      codes[l] = sa == 255u ? 0u : fp4_codes8(x, fp4_inverse(sa));
+      codes[l + 8] = sb == 255u ? 0u : fp4_codes8(y, fp4_inverse(sb));
+      if (!(l & 1)) {
+        scales[l >> 1] = (uint8_t)sa;
+        scales[4 + (l >> 1)] = (uint8_t)sb;
+      }
+    }
   }
 }
 
@@ -114,10 +150,14 @@ read_fp4_kernel(const uint8_t* kc, const uint8_t* ks, const uint8_t* vc, const u
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 int launch_store(nvc_ctx* ctx, const StoreArgs& p, void* stream) {
-  const int64_t blocks = ((int64_t)p.N * (p.nh + 2 * p.kv) * 8 + 255) / 256;
+  // few tokens: their heads over many warps; many: all heads of a token in one
+  const int fours = (p.nh + 2 * p.kv + 3) / 4;
+  const int64_t room = (int64_t)ctx->num_sms * 32;
+  const int span = (int)std::min<int64_t>(fours, std::max<int64_t>(1, (int64_t)p.N * fours / room)), per_token = (fours + span - 1) / span;
+  const int64_t blocks = ((int64_t)p.N * per_token + 3) / 4;
   NVC_REQUIRE(ctx, blocks <= 0x7fffffffLL, NVC_ESHAPE, "too many rows");
   DeviceGuard guard(ctx->device);
-  NVC_CUDA_CHECK(ctx, nvc_launch(ctx, store_fp4_kernel, dim3((unsigned)blocks), dim3(256), 0, nvc_stream(stream), p));
+  NVC_CUDA_CHECK(ctx, nvc_launch(ctx, store_fp4_kernel, dim3((unsigned)blocks), dim3(128), 0, nvc_stream(stream), p, span, per_token));
   NVC_CUDA_CHECK(ctx, cudaGetLastError());
   ctx->launches++;
   return NVC_OK;

@@ -5,6 +5,7 @@ raises."""
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import Optional
 
 import torch
@@ -1120,34 +1121,35 @@ def gemm_fp8_grouped(ctx, q, scale, wq, wscale, tile_group, out_dtype=BF16, out=
 
 
 # ---------------------------------------------------------------- a paged key-value cache in 4 bits, and the attention that reads it
-class _Fp4CacheC(C.Structure):
-    _fields_ = [("k", C.c_void_p), ("k_scale", C.c_void_p), ("v", C.c_void_p), ("v_scale", C.c_void_p), ("num_blocks", C.c_int), ("kv", C.c_int), ("block_size", C.c_int)]
+_FP4_CACHE_C = struct.Struct("@4P3i4x")          # nvc_fp4_cache
+_BF16_ONLY, _U8 = (torch.bfloat16,), (torch.uint8,)
 
 
 class Fp4Cache:
     """Keys and values of one layer in 4 bits (the format: nvc_fp4_cache in nvc_b200.h), head_dim 128: k, v uint8 [num_blocks, kv, block_size, 64] and k_scale, v_scale uint8
     [num_blocks, kv, block_size, 8].  The slot of a token is block * block_size + offset, as in a bf16 cache, which takes 3.6 times the bytes."""
-    __slots__ = ("k", "k_scale", "v", "v_scale", "num_blocks", "kv", "block_size", "device", "c", "at")
+    __slots__ = ("k", "k_scale", "v", "v_scale", "num_blocks", "kv", "block_size", "device", "c")
 
     def __init__(self, k, k_scale, v, v_scale):
-        shape = k.shape
+        shape, device, u8 = k.shape, k.device, torch.uint8
         if len(shape) != 4 or shape[3] != 64 or shape[0] < 1 or shape[1] < 1 or shape[2] < 16 or shape[2] % 16:
             raise ValueError(f"k must be [num_blocks, kv, block_size, 64] with a block_size that is a multiple of 16, got {list(shape)}")
-        self.num_blocks, self.kv, self.block_size, _ = shape
-        if (self.num_blocks * self.block_size | self.kv) >> 31:
+        blocks, kv, bs, _ = shape
+        if (blocks * bs | kv) >> 31:
             raise ValueError(_TOO_FAR)
-        scales = (*shape[:3], 8)
-        self.device = k.get_device()
-        for name, t, want in (("k", k, shape), ("k_scale", k_scale, scales), ("v", v, shape), ("v_scale", v_scale, scales)):
-            if t.dtype is not torch.uint8:
-                raise TypeError(f"{name} must be torch.uint8, got {t.dtype}")
-            if t.shape != want or not t.is_contiguous():
-                raise ValueError(f"{name} must be {list(want)} and contiguous, got {list(t.shape)}")
-            if t.device != k.device:
-                raise ValueError("the cache's parts must be on one device")
+        scales = (blocks, kv, bs, 8)
+        if not (k.dtype is u8 and k_scale.dtype is u8 and v.dtype is u8 and v_scale.dtype is u8 and k_scale.shape == scales and v.shape == shape and v_scale.shape == scales
+                and k.is_contiguous() and k_scale.is_contiguous() and v.is_contiguous() and v_scale.is_contiguous() and k_scale.device == device and v.device == device
+                and v_scale.device == device):
+            for name, t, want in (("k", k, shape), ("k_scale", k_scale, scales), ("v", v, shape), ("v_scale", v_scale, scales)):
+                if t.dtype is not u8:
+                    raise TypeError(f"{name} must be torch.uint8, got {t.dtype}")
+                if t.shape != want or not t.is_contiguous():
+                    raise ValueError(f"{name} must be {list(want)} and contiguous, got {list(t.shape)}")
+            raise ValueError("the cache's parts must be on one device")
+        self.num_blocks, self.kv, self.block_size, self.device = blocks, kv, bs, k.get_device()
         self.k, self.k_scale, self.v, self.v_scale = k, k_scale, v, v_scale
-        self.c = _Fp4CacheC(k.data_ptr(), k_scale.data_ptr(), v.data_ptr(), v_scale.data_ptr(), self.num_blocks, self.kv, self.block_size)
-        self.at = C.addressof(self.c)
+        self.c = _FP4_CACHE_C.pack(k.data_ptr(), k_scale.data_ptr(), v.data_ptr(), v_scale.data_ptr(), blocks, kv, bs)
 
     @classmethod
     def zeros(cls, num_blocks: int, block_size: int, kv: int, device="cuda:0") -> "Fp4Cache":
@@ -1155,54 +1157,52 @@ class Fp4Cache:
         return cls(new(64), new(8), new(64), new(8))
 
 
-_BF16_ONLY = (torch.bfloat16,)
-
-
-def _rows_stride(ctx, name, t, rows: int, width: int) -> int:
-    """The row stride of bf16 rows that need not lie together."""
-    if t.dtype is not BF16 or t.get_device() != ctx.device or t.shape != (rows, width) or (t.stride(1) != 1 and width > 1):
-        _refuse(ctx, (name, t, _BF16_ONLY, (rows, width), False))
-    return t.stride(0) if rows > 1 else width          # a single row's distance to the next says nothing
-
-
-def _numbers(ctx, name, t, n: int) -> int:
-    """The address of n whole numbers."""
-    if t.dtype is not torch.int32 or t.get_device() != ctx.device or t.shape != (n,) or not t.is_contiguous():
-        _refuse(ctx, (name, t, _I32, (n,), True))
-    return t.data_ptr()
-
-
-def _fp4_cache_given(ctx, cache) -> int:
+def _refuse_fp4(ctx, cache, *facts):
     if not isinstance(cache, Fp4Cache):
         raise TypeError(f"cache must be an Fp4Cache, got {type(cache).__name__}")
     if cache.device != ctx.device:
         raise ValueError(f"cache must be on cuda:{ctx.device} (no CPU fallback on this path)")
-    return cache.at
+    _refuse(ctx, *facts)
 
 
 def qk_norm_rope_store_fp4(ctx, qkv, qw, kw, eps: float, cos_sin, positions, nh: int, cache: Fp4Cache, slot_mapping, q_out=None):
     """qk_norm_rope_store with a cache in 4 bits.  qkv: bf16 [N, (nh + 2 kv) * 128], rows may have any stride that is a multiple of 8; q and k heads normed (qw, kw: bf16 [128], both or
     neither) and rotated (cos_sin: fp32 [positions, 128], Context.rope_table) in place, or, with q_out [N, nh * 128], the q heads there and qkv left as it is.  k and v rows go to the
-    cache at slot_mapping (int32 [N]; a slot that the cache does not have: nowhere).  Gives qkv, or q_out."""
-    at, width, N = _fp4_cache_given(ctx, cache), (nh + 2 * cache.kv) * 128, qkv.shape[0] if qkv.dim() else 0
-    ld = _rows_stride(ctx, "qkv", qkv, N, width)
-    if (qw is None) != (kw is None):
-        raise ValueError("qw and kw: both or neither")
-    if qw is not None:
-        for name, w in (("qw", qw), ("kw", kw)):
-            if w.dtype is not BF16 or w.get_device() != ctx.device or w.shape != (128,) or not w.is_contiguous():
-                _refuse(ctx, (name, w, _BF16_ONLY, (128,), True))
-    if cos_sin.dtype is not torch.float32 or cos_sin.get_device() != ctx.device or cos_sin.dim() != 2 or cos_sin.shape[1] != 128 or not cos_sin.is_contiguous():
-        _refuse(ctx, ("cos_sin", cos_sin, _F32, (cos_sin.shape[0] if cos_sin.dim() else 0, 128), True))
-    pos, slots = _numbers(ctx, "positions", positions, N), _numbers(ctx, "slot_mapping", slot_mapping, N)
-    q_at, ldq = None, 0
-    if q_out is not None:
-        ldq, q_at = _rows_stride(ctx, "q_out", q_out, N, nh * 128), q_out.data_ptr()
-    if (N | ld | ldq | nh | cos_sin.shape[0]) >> 31:
+    cache at slot_mapping (int32 [N]; a slot that the cache does not have: nowhere; none may come twice).  Gives qkv, or q_out."""
+    dev, i32 = ctx.device, torch.int32
+    shape, turns = qkv.shape, cos_sin.shape
+    N = shape[0] if len(shape) == 2 else -1
+    good = (type(cache) is Fp4Cache and cache.device == dev and qkv.dtype is BF16 and qkv.get_device() == dev and N >= 0 and shape[1] == (nh + 2 * cache.kv) * 128
+            and positions.dtype is i32 and positions.get_device() == dev and positions.shape == (N,) and slot_mapping.dtype is i32 and slot_mapping.get_device() == dev
+            and slot_mapping.shape == (N,) and cos_sin.dtype is torch.float32 and cos_sin.get_device() == dev and len(turns) == 2 and turns[1] == 128 and positions.is_contiguous()
+            and slot_mapping.is_contiguous() and cos_sin.is_contiguous())
+    if good:
+        ld, one = qkv.stride()
+        ld, good = (ld if N > 1 else shape[1]), one == 1          # a single row's distance to the next says nothing
+    qw_at = kw_at = q_at = None
+    ldq = 0
+    if good and (qw is not None or kw is not None):
+        if qw is None or kw is None:
+            raise ValueError("qw and kw: both or neither")
+        qw_at, kw_at = qw.data_ptr(), kw.data_ptr()
+        good = (qw.dtype is BF16 and kw.dtype is BF16 and qw.get_device() == dev and kw.get_device() == dev and qw.shape == (128,) and kw.shape == (128,) and qw.is_contiguous()
+                and kw.is_contiguous())
+    if good and q_out is not None:
+        q_at = q_out.data_ptr()
+        good = q_out.dtype is BF16 and q_out.get_device() == dev and q_out.shape == (N, nh * 128)
+        if good:
+            ldq, one = q_out.stride()
+            ldq, good = (ldq if N > 1 else nh * 128), one == 1
+    if not good:
+        kv = getattr(cache, "kv", 0)
+        _refuse_fp4(ctx, cache, ("qkv", qkv, _BF16_ONLY, (max(N, 0), (nh + 2 * kv) * 128), False), ("qw", qw, _BF16_ONLY, (128,), True), ("kw", kw, _BF16_ONLY, (128,), True),
+                    ("cos_sin", cos_sin, _F32, (turns[0] if len(turns) else 0, 128), True), ("positions", positions, _I32, (max(N, 0),), True),
+                    ("slot_mapping", slot_mapping, _I32, (max(N, 0),), True), ("q_out", q_out, _BF16_ONLY, (max(N, 0), nh * 128), False))
+    if (N | ld | ldq | nh | turns[0]) >> 31:
         raise ValueError(_TOO_FAR)
     if N:
-        st = ctx.l.nvc_qk_norm_rope_store_fp4(ctx.h, qkv.data_ptr(), ld, _ptr(qw), _ptr(kw), eps, cos_sin.data_ptr(), cos_sin.shape[0], pos, slots, at, q_at, ldq, N, nh,
-                                              torch._C._cuda_getCurrentRawStream(ctx.device))
+        st = ctx.l.nvc_qk_norm_rope_store_fp4(ctx.h, qkv.data_ptr(), ld, qw_at, kw_at, eps, cos_sin.data_ptr(), turns[0], positions.data_ptr(), slot_mapping.data_ptr(), cache.c, q_at,
+                                              ldq, N, nh, torch._C._cuda_getCurrentRawStream(dev))
         if st:
             check(st, "nvc_qk_norm_rope_store_fp4", ctx.h)
     return qkv if q_out is None else q_out
@@ -1210,13 +1210,23 @@ def qk_norm_rope_store_fp4(ctx, qkv, qw, kw, eps: float, cos_sin, positions, nh:
 
 def store_kvcache_fp4(ctx, k, v, cache: Fp4Cache, slot_mapping) -> None:
     """store_kvcache with a cache in 4 bits: rows k, v bf16 [N, kv * 128], as they are, each with its row stride (a multiple of 8), to slot_mapping (int32 [N])."""
-    at, width, N = _fp4_cache_given(ctx, cache), cache.kv * 128, k.shape[0] if k.dim() else 0
-    ldk, ldv = _rows_stride(ctx, "k", k, N, width), _rows_stride(ctx, "v", v, N, width)
-    slots = _numbers(ctx, "slot_mapping", slot_mapping, N)
+    dev, shape = ctx.device, k.shape
+    N = shape[0] if len(shape) == 2 else -1
+    good = (type(cache) is Fp4Cache and cache.device == dev and k.dtype is BF16 and v.dtype is BF16 and k.get_device() == dev and v.get_device() == dev and N >= 0
+            and shape[1] == cache.kv * 128 and v.shape == shape and slot_mapping.dtype is torch.int32 and slot_mapping.get_device() == dev and slot_mapping.shape == (N,)
+            and slot_mapping.is_contiguous())
+    if good:
+        (ldk, one), (ldv, two) = k.stride(), v.stride()
+        good = one == 1 and two == 1
+        if N == 1:
+            ldk = ldv = shape[1]
+    if not good:
+        want = (max(N, 0), getattr(cache, "kv", 0) * 128)
+        _refuse_fp4(ctx, cache, ("k", k, _BF16_ONLY, want, False), ("v", v, _BF16_ONLY, want, False), ("slot_mapping", slot_mapping, _I32, (max(N, 0),), True))
     if (N | ldk | ldv) >> 31:
         raise ValueError(_TOO_FAR)
     if N:
-        st = ctx.l.nvc_store_kvcache_fp4(ctx.h, k.data_ptr(), ldk, v.data_ptr(), ldv, at, slots, N, torch._C._cuda_getCurrentRawStream(ctx.device))
+        st = ctx.l.nvc_store_kvcache_fp4(ctx.h, k.data_ptr(), ldk, v.data_ptr(), ldv, cache.c, slot_mapping.data_ptr(), N, torch._C._cuda_getCurrentRawStream(dev))
         if st:
             check(st, "nvc_store_kvcache_fp4", ctx.h)
 
@@ -1224,44 +1234,57 @@ def store_kvcache_fp4(ctx, k, v, cache: Fp4Cache, slot_mapping) -> None:
 def read_kvcache_fp4(ctx, cache: Fp4Cache, slots):
     """Rows of a 4-bit cache: (k e4m3 [N, kv, 128], k_scale bf16 [N, kv, 8], v, v_scale), number = k * k_scale of its block of 16, both exact.  slots: int32 [N]; zeros where the cache has
     no such slot."""
-    at, N, kv = _fp4_cache_given(ctx, cache), slots.numel(), cache.kv
-    at_slots = _numbers(ctx, "slots", slots, N)
+    dev, shape = ctx.device, slots.shape
+    if not (type(cache) is Fp4Cache and cache.device == dev and slots.dtype is torch.int32 and slots.get_device() == dev and len(shape) == 1 and slots.is_contiguous()):
+        _refuse_fp4(ctx, cache, ("slots", slots, _I32, (slots.numel(),), True))
+    N, kv = shape[0], cache.kv
     if N >> 31:
         raise ValueError(_TOO_FAR)
-    k, v = slots.new_empty(2, N, kv, 128, dtype=FP8)
-    ks, vs = slots.new_empty(2, N, kv, 8, dtype=BF16)
+    k, ks = slots.new_empty(N, kv, 128, dtype=FP8), slots.new_empty(N, kv, 8, dtype=BF16)
+    v, vs = slots.new_empty(N, kv, 128, dtype=FP8), slots.new_empty(N, kv, 8, dtype=BF16)
     if N:
-        st = ctx.l.nvc_read_kvcache_fp4(ctx.h, at, at_slots, k.data_ptr(), ks.data_ptr(), v.data_ptr(), vs.data_ptr(), N, torch._C._cuda_getCurrentRawStream(ctx.device))
+        st = ctx.l.nvc_read_kvcache_fp4(ctx.h, cache.c, slots.data_ptr(), k.data_ptr(), ks.data_ptr(), v.data_ptr(), vs.data_ptr(), N, torch._C._cuda_getCurrentRawStream(dev))
         if st:
             check(st, "nvc_read_kvcache_fp4", ctx.h)
     return k, ks, v, vs
 
 
-def _attn_fp4(ctx, q, cache, block_tables, context_lens, nh, out, B, most: int):
-    """Checks of both attentions: (addresses and strides of q, tables, lengths and the result, the result, the workspace)."""
-    width, rows = nh * 128, q.shape[0] if q.dim() else 0
-    ldq = _rows_stride(ctx, "q", q, rows, width)
-    if block_tables.dtype is not torch.int32 or block_tables.get_device() != ctx.device or block_tables.dim() != 2 or block_tables.shape[0] != B or not block_tables.is_contiguous():
-        _refuse(ctx, ("block_tables", block_tables, _I32, (B, block_tables.shape[1] if block_tables.dim() == 2 else 1), True))
-    lens = _numbers(ctx, "context_lens", context_lens, B)
-    if out is None:
-        out, ldo = q.new_empty(rows, width), width
-    else:
-        ldo = _rows_stride(ctx, "out", out, rows, width)
-    if (rows | B | nh | ldq | ldo | block_tables.shape[1]) >> 31:
+def _attn_fp4(ctx, q, cache, block_tables, context_lens, nh, out, B, cu, most: int):
+    """Checks of both attentions: (rows, q's row stride, the result and its, the workspace and its size)."""
+    dev, i32, shape, width = ctx.device, torch.int32, q.shape, nh * 128
+    rows = shape[0] if len(shape) == 2 else -1
+    good = (type(cache) is Fp4Cache and cache.device == dev and q.dtype is BF16 and q.get_device() == dev and rows >= 0 and shape[1] == width and block_tables.dtype is i32
+            and block_tables.get_device() == dev and block_tables.dim() == 2 and block_tables.shape[0] == B and block_tables.is_contiguous() and context_lens.dtype is i32
+            and context_lens.get_device() == dev and context_lens.shape == (B,) and context_lens.is_contiguous()
+            and (cu is None or cu.dtype is i32 and cu.get_device() == dev and cu.shape == (B + 1,) and cu.is_contiguous()))
+    if good:
+        ldq, one = q.stride()
+        ldq, good = (ldq if rows > 1 else width), one == 1 or not width
+    ldo = width
+    if good and out is not None:
+        good = out.dtype is BF16 and out.get_device() == dev and out.shape == shape
+        if good:
+            ldo, one = out.stride()
+            ldo, good = (ldo if rows > 1 else width), one == 1
+    if not good:
+        want = (max(rows, 0), width)
+        _refuse_fp4(ctx, cache, ("q", q, _BF16_ONLY, want, False), ("block_tables", block_tables, _I32, (B, block_tables.shape[1] if block_tables.dim() == 2 else 1), True),
+                    ("context_lens", context_lens, _I32, (B,), True), ("cu_seqlens_q", cu, _I32, (B + 1,), True), ("out", out, _BF16_ONLY, want, False))
+    if (rows | B | nh | ldq | ldo | block_tables.shape[1] | most) >> 31:
         raise ValueError(_TOO_FAR)
+    if out is None:
+        out = q.new_empty(rows, width)
     need = ctx.l.nvc_attn_fp4_workspace_bytes(ctx.h, nh, cache.kv, min(most, rows))
-    ws = q.new_empty(need, dtype=torch.uint8)          # of this call alone: other streams and captured graphs have their own
-    return rows, ldq, lens, out, ldo, ws, need
+    return rows, ldq, out, ldo, q.new_empty(need, dtype=torch.uint8), need          # a workspace of this call alone: other streams and captured graphs have their own
 
 
 def paged_decode_attn_fp4(ctx, q, cache: Fp4Cache, block_tables, context_lens, nh: int, scale: float, out=None) -> torch.Tensor:
     """paged_decode_attn over a cache in 4 bits.  q: bf16 [B, nh * 128] (rows of any stride that is a multiple of 8), block_tables int32 [B, max_blocks], context_lens int32 [B] (0: zeros)."""
-    at, B = _fp4_cache_given(ctx, cache), q.shape[0] if q.dim() else 0
-    _, ldq, lens, out, ldo, ws, need = _attn_fp4(ctx, q, cache, block_tables, context_lens, nh, out, B, 1)
+    B = q.shape[0] if q.dim() else 0
+    _, ldq, out, ldo, ws, need = _attn_fp4(ctx, q, cache, block_tables, context_lens, nh, out, B, None, 1)
     if B:
-        st = ctx.l.nvc_paged_decode_attn_fp4(ctx.h, q.data_ptr(), ldq, at, block_tables.data_ptr(), block_tables.shape[1], lens, B, nh, scale, out.data_ptr(), ldo, ws.data_ptr(), need,
-                                             torch._C._cuda_getCurrentRawStream(ctx.device))
+        st = ctx.l.nvc_paged_decode_attn_fp4(ctx.h, q.data_ptr(), ldq, cache.c, block_tables.data_ptr(), block_tables.shape[1], context_lens.data_ptr(), B, nh, scale, out.data_ptr(), ldo,
+                                             ws.data_ptr(), need, torch._C._cuda_getCurrentRawStream(ctx.device))
         if st:
             check(st, "nvc_paged_decode_attn_fp4", ctx.h)
     return out
@@ -1270,16 +1293,13 @@ def paged_decode_attn_fp4(ctx, q, cache: Fp4Cache, block_tables, context_lens, n
 def prefill_attn_paged_fp4(ctx, q, cache: Fp4Cache, block_tables, context_lens, cu_seqlens_q, max_seqlen_q: int, nh: int, scale: float, out=None) -> torch.Tensor:
     """prefill_attn_paged over a cache in 4 bits: q bf16 [N, nh * 128] = the last q_len_b positions of each context, whose rows are in the cache; cu_seqlens_q int32 [B + 1]; max_seqlen_q at
     least the longest q_len.  A row that sees no key is zeros; rows behind the last sequence are left as they are (in a result of this call's own: anything)."""
-    at, B = _fp4_cache_given(ctx, cache), cu_seqlens_q.numel() - 1
+    B = cu_seqlens_q.numel() - 1
     if B < 0:
         raise ValueError("cu_seqlens_q must have B + 1 entries")
-    if max_seqlen_q >> 31:
-        raise ValueError(_TOO_FAR)
-    cu = _numbers(ctx, "cu_seqlens_q", cu_seqlens_q, B + 1)
-    rows, ldq, lens, out, ldo, ws, need = _attn_fp4(ctx, q, cache, block_tables, context_lens, nh, out, B, max_seqlen_q)
+    rows, ldq, out, ldo, ws, need = _attn_fp4(ctx, q, cache, block_tables, context_lens, nh, out, B, cu_seqlens_q, max_seqlen_q)
     if rows and B:
-        st = ctx.l.nvc_prefill_attn_paged_fp4(ctx.h, q.data_ptr(), ldq, at, block_tables.data_ptr(), block_tables.shape[1], lens, cu, B, rows, max_seqlen_q, nh, scale, out.data_ptr(), ldo,
-                                              ws.data_ptr(), need, torch._C._cuda_getCurrentRawStream(ctx.device))
+        st = ctx.l.nvc_prefill_attn_paged_fp4(ctx.h, q.data_ptr(), ldq, cache.c, block_tables.data_ptr(), block_tables.shape[1], context_lens.data_ptr(), cu_seqlens_q.data_ptr(), B, rows,
+                                              max_seqlen_q, nh, scale, out.data_ptr(), ldo, ws.data_ptr(), need, torch._C._cuda_getCurrentRawStream(ctx.device))
         if st:
             check(st, "nvc_prefill_attn_paged_fp4", ctx.h)
     return out
