@@ -762,8 +762,8 @@ int nvc_gemm_fp8_grouped(nvc_ctx* ctx, const nvc_fp8* A, int lda, const float* a
  * an infinity or a NaN (scale byte 255) reads as NaN.
  * Layout: k, v [num_blocks, kv, block_size, 64] (number 2i in the low half of byte i), k_scale, v_scale [num_blocks, kv, block_size, 8], each 16-byte aligned: a
  * page's rows of one key head lie together.  block_size % 16 == 0, num_blocks * block_size < 2^31; the slot of a token is block * block_size + offset, as above.
- * head_dim is 128.  Static operands (launch order, above) of the attention calls are block_tables, context_lens and cu_seqlens_q; those that store and read rows have none, and
- * queries and cached rows may come from any earlier work of the stream. */
+ * head_dim is 128.  Static operands (launch order, above) are block_tables, context_lens, cu_seqlens_q, slot_mapping, positions and cos_sin; queries, keys, values, norm weights, cached
+ * rows and the slots of nvc_read_kvcache_fp4 may come from any earlier work of the stream. */
 typedef struct nvc_fp4_cache {
   uint8_t *k, *k_scale, *v, *v_scale;
   int num_blocks, kv, block_size;

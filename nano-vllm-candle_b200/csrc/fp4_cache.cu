@@ -4,6 +4,7 @@
 #include "internal.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -23,46 +24,24 @@ struct StoreArgs {
 };
 
 // 8 lanes per (token, head): lane l owns the numbers [8l, 8l + 8) and [64 + 8l, 64 + 8l + 8), so that a rotation's pairs are one lane's and a block of 16 is two
-// neighbouring lanes'.  A warp takes `span` fours of one token's heads, so that the token's angles, slot and the norms' weights are read once for them, two fours ahead of their use.
-// Memory-bound: per token (nh + 2 kv) * 256 bytes in, nh * 256 (and kv * 256 in place) + kv * 144 out.
-__global__ void __launch_bounds__(128) store_fp4_kernel(const StoreArgs p, int span, int warps_per_token) {
+// neighbouring lanes'.  A warp takes `span` fours of one token's heads (fours of q heads, then of k, then of v heads), so that the token's angles and slot and the norms' weights are read once for
+// them.  Per token (nh + 2 kv) * 256 bytes in, nh * 256 (and kv * 256 in place) + kv * 144 out.  Kinds of heads in loops of their own: with one loop for all, the instructions were what bound it (370 a
+// four, 95 us for 16 000 tokens of 32 + 16 heads).
+__global__ void __launch_bounds__(128, 5) store_fp4_kernel(const StoreArgs p, int span, int warps_per_token) {
   pdl_trigger();
-  const int units = p.nh + 2 * p.kv;
   const int64_t warp = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31, l = lane & 7;
+  const int lane = threadIdx.x & 31, l = lane & 7, sub = lane >> 3;
   const unsigned mask = 0xffu << (lane & ~7);
-  const int n = (int)(warp / warps_per_token), first = (int)(warp - (int64_t)n * warps_per_token) * span;
-  pdl_wait();
+  const int n = warps_per_token == 1 ? (int)min(warp, (int64_t)p.N) : (int)((uint32_t)warp / (uint32_t)warps_per_token);      // several warps a token: below 2^32 in all
+  const int first = warps_per_token == 1 ? 0 : (int)((uint32_t)warp - (uint32_t)n * warps_per_token) * span;
   if (n >= p.N) return;
-  auto source = [&](int u) {
-    const nvc_bf16* src = u < p.nh ? p.q + n * p.ldq : u < p.nh + p.kv ? p.k + n * p.ldk : p.v + n * p.ldv;
-    const int h = u < p.nh ? u : u < p.nh + p.kv ? u - p.nh : u - p.nh - p.kv;
-    return reinterpret_cast<const uint4*>(src + (int64_t)h * 128);
-  };
-  constexpr int kAhead = 2;
-  uint4 a[kAhead], b[kAhead];
-  auto load = [&](int i, uint4& x, uint4& y) {
-    const int u = 4 * (first + i) + (lane >> 3);
-    if (i < span && u < units) {
-      const uint4* row = source(u);
-      x = ld_once_u4(row + l);
-      y = ld_once_u4(row + l + 8);
-    } else {
-      x = y = make_uint4(0, 0, 0, 0);
-    }
-  };
-#pragma unroll
-  for (int i = 0; i < kAhead; ++i) load(i, a[i], b[i]);
+  // what no kernel of a step writes - slot, position, angles - in front of the wait for the one that writes the rows
   const int slot = p.slot_mapping[n];
   float4 c0, c1, s0, s1;
-  uint4 wq0 = make_uint4(0, 0, 0, 0), wq1 = wq0, wk0 = wq0, wk1 = wq0;
   c0 = c1 = s0 = s1 = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (p.table) {
+  const int q_fours = (p.nh + 3) >> 2, kv_fours = (p.kv + 3) >> 2;
+  if (p.table && first < q_fours + kv_fours) {
     const int pos = p.positions[n];
-    if (p.qw) {
-      wq0 = p.qw[l]; wq1 = p.qw[l + 8];
-      wk0 = p.kw[l]; wk1 = p.kw[l + 8];
-    }
     if ((unsigned)pos < (unsigned)p.max_pos) {
       const float4* cs = p.table + (int64_t)pos * 32;                        // cos[64], sin[64]
       c0 = cs[2 * l]; c1 = cs[2 * l + 1]; s0 = cs[16 + 2 * l]; s1 = cs[16 + 2 * l + 1];
@@ -74,45 +53,58 @@ __global__ void __launch_bounds__(128) store_fp4_kernel(const StoreArgs p, int s
   const bool stored = (unsigned)slot < (unsigned)p.slots;
   const int block = stored ? slot / p.block_size : 0;
   const int64_t page_row = (int64_t)block * p.kv * p.block_size + (stored ? slot - block * p.block_size : 0);
-#pragma unroll 1
-  for (int i0 = 0; i0 < span; i0 += kAhead) {
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      uint4 x = a[j], y = b[j];
-      load(i0 + j + kAhead, a[j], b[j]);
-      const int u = 4 * (first + i0 + j) + (lane >> 3);
-      if (i0 + j >= span || u >= units) continue;                            // (a unit's eight lanes alike)
-      const bool is_q = u < p.nh, is_v = u >= p.nh + p.kv;
-      const int h = is_q ? u : is_v ? u - p.nh - p.kv : u - p.nh;
-      if (!is_v && p.table) {
+  pdl_wait();
+
+  // heads 4 * i + sub of one kind, i from `from` to `to`; the next row on its way while one is worked on
+  auto heads = [&](auto kind, const nvc_bf16* src, nvc_bf16* dst, const uint4* w, uint8_t* codes_to, uint8_t* scales_to, int count, int from, int to) {
+    constexpr bool kTurn = decltype(kind)::value != 2, kStore = decltype(kind)::value != 0;
+    if (from >= to) return;
+    uint4 w0 = make_uint4(0, 0, 0, 0), w1 = w0;
+    if (kTurn && w) { w0 = w[l]; w1 = w[l + 8]; }
+    const uint4* row = reinterpret_cast<const uint4*>(src) + (int64_t)(4 * from + sub) * 16 + l;
+    uint4* out = reinterpret_cast<uint4*>(dst) + (int64_t)(4 * from + sub) * 16 + l;
+    uint4 a = make_uint4(0, 0, 0, 0), b = a;
+    if (4 * from + sub < count) { a = ld_once_u4(row); b = ld_once_u4(row + 8); }
+#pragma unroll 2
+    for (int i = from; i < to; ++i, out += 64) {
+      uint4 x = a, y = b;
+      row += 64;
+      if (i + 1 < to && 4 * i + 4 + sub < count) { a = ld_once_u4(row); b = ld_once_u4(row + 8); }
+      if (4 * i + sub >= count) break;                                       // (a head's eight lanes alike)
+      if (kTurn && p.table) {
         uint4 o1, o2;
-        qk_norm_rope8(x, y, mask, p.qw != nullptr, is_q ? wq0 : wk0, is_q ? wq1 : wk1, p.eps, c0, c1, s0, s1, o1, o2);
+        qk_norm_rope8(x, y, mask, w != nullptr, w0, w1, p.eps, c0, c1, s0, s1, o1, o2);
         x = o1;
         y = o2;
-        nvc_bf16* out = is_q ? p.q_out + n * p.ldqo : p.k_out ? p.k_out + n * p.ldko : nullptr;
-        if (out) {
-          uint4* o = reinterpret_cast<uint4*>(out + (int64_t)h * 128);
-          o[l] = x;
-          o[l + 8] = y;
+        if (dst) {
+          out[0] = x;
+          out[8] = y;
         }
       }
-      if (is_q) continue;
-      uint32_t ma = fp4_amax8(x), mb = fp4_amax8(y);
-      ma = max(ma, __shfl_xor_sync(mask, ma, 1));
-      mb = max(mb, __shfl_xor_sync(mask, mb, 1));
-      if (!stored) continue;
-      const uint32_t sa = fp4_scale_byte(ma), sb = fp4_scale_byte(mb);
-      const int64_t at = page_row + (int64_t)h * p.block_size;
-      uint32_t* codes = reinterpret_cast<uint32_t*>((is_v ? p.vc : p.kc) + at * kFp4Codes);
-      uint8_t* scales = (is_v ? p.vs : p.ks) + at * kFp4Scales;
-      codes[l] = sa == 255u ? 0u : fp4_codes8(x, fp4_inverse(sa));
-      codes[l + 8] = sb == 255u ? 0u : fp4_codes8(y, fp4_inverse(sb));
-      if (!(l & 1)) {
-        scales[l >> 1] = (uint8_t)sa;
-        scales[4 + (l >> 1)] = (uint8_t)sb;
+      if (kStore) {
+        uint32_t ma = fp4_amax8(x), mb = fp4_amax8(y);
+        ma = max(ma, __shfl_xor_sync(mask, ma, 1));
+        mb = max(mb, __shfl_xor_sync(mask, mb, 1));
+        const uint32_t sa = fp4_scale_byte(ma), sb = fp4_scale_byte(mb);
+        if (stored) {
+          const int64_t at = page_row + (int64_t)(4 * i + sub) * p.block_size;
+          uint32_t* codes = reinterpret_cast<uint32_t*>(codes_to + at * kFp4Codes);
+          uint8_t* scales = scales_to + at * kFp4Scales;
+          codes[l] = sa == 255u ? 0u : fp4_codes8(x, fp4_inverse(sa));
+          codes[l + 8] = sb == 255u ? 0u : fp4_codes8(y, fp4_inverse(sb));
+          if (!(l & 1)) {
+            scales[l >> 1] = (uint8_t)sa;
+            scales[4 + (l >> 1)] = (uint8_t)sb;
+          }
+        }
       }
     }
-  }
+  };
+  const int last = first + span;
+  const nvc_bf16* none = nullptr;
+  heads(std::integral_constant<int, 0>(), p.nh ? p.q + n * p.ldq : none, p.nh ? p.q_out + n * p.ldqo : nullptr, p.qw, nullptr, nullptr, p.nh, first, min(last, q_fours));
+  heads(std::integral_constant<int, 1>(), p.k + n * p.ldk, p.k_out ? p.k_out + n * p.ldko : nullptr, p.kw, p.kc, p.ks, p.kv, max(first - q_fours, 0), min(last - q_fours, kv_fours));
+  heads(std::integral_constant<int, 2>(), p.v + n * p.ldv, nullptr, nullptr, p.vc, p.vs, p.kv, max(first - q_fours - kv_fours, 0), min(last - q_fours - kv_fours, kv_fours));
 }
 
 // 8 lanes per (row, head, side), 16 numbers a lane
@@ -151,7 +143,7 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 int launch_store(nvc_ctx* ctx, const StoreArgs& p, void* stream) {
   // few tokens: their heads over many warps; many: all heads of a token in one
-  const int fours = (p.nh + 2 * p.kv + 3) / 4;
+  const int fours = (p.nh + 3) / 4 + 2 * ((p.kv + 3) / 4);
   const int64_t room = (int64_t)ctx->num_sms * 32;
   const int span = (int)std::min<int64_t>(fours, std::max<int64_t>(1, (int64_t)p.N * fours / room)), per_token = (fours + span - 1) / span;
   const int64_t blocks = ((int64_t)p.N * per_token + 3) / 4;
