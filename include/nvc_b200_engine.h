@@ -48,7 +48,8 @@ typedef struct nvc_runner_options {
   int32_t allreduce_f32;           /* TP: reduce fp32 partials instead of bf16 (default 0)                   */
   int32_t dtype;                   /* registry models: NVC_DT_BF16 (0, serving) or NVC_DT_F32 (exact mode)   */
   int32_t max_logit_rows;          /* most rows nvc_runner_set_logit_rows may arm (0 = max_num_seqs)         */
-  int32_t reserved[2];
+  int32_t kv_cache_bits;           /* Qwen3: 0 or 16 = bf16 cache, 4 = the 4-bit cache of nvc_b200.h (nvc_fp4_cache) */
+  int32_t reserved[1];
 } nvc_runner_options;
 
 /* ------------------------------------------------------------------ runner */

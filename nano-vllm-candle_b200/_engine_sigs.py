@@ -16,7 +16,7 @@ class Qwen3ConfigC(C.Structure):
 class RunnerOptionsC(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("num_kvcache_blocks", "kvcache_block_size", "max_num_seqs",
                                          "max_num_batched_tokens", "max_model_len", "use_cuda_graph",
-                                         "allreduce_f32", "dtype", "max_logit_rows")] + [("reserved", C.c_int32 * 2)]
+                                         "allreduce_f32", "dtype", "max_logit_rows", "kv_cache_bits")] + [("reserved", C.c_int32 * 1)]
 
 
 class SchedulerConfigC(C.Structure):

@@ -72,10 +72,26 @@ int run_layers(nvc_runner* r, int N, bool decode, int B, int max_seqlen, int blo
     }
     xn_ready = false;
     // QKV projection + q/k-norm + RoPE + KV scatter: one kernel at prefill sizes, GEMM + K2 otherwise (same bits)
-    rc = nvc_qkv_proj_norm_rope(ctx, r->xn, H, Ly.w_qkv, r->qkv, N, H, Ly.q_norm, Ly.k_norm, c.rms_norm_eps, r->rope, r->d_pos,
-                                r->d_slots, Ly.k_cache, Ly.v_cache, r->nh_l, r->kv_l, hd, st);
+    if (r->fp4()) {
+      rc = nvc_gemm_bf16(ctx, r->xn, H, Ly.w_qkv, r->qkv, r->qkv_l, NVC_DT_BF16, N, r->qkv_l, H, st);
+      if (rc == NVC_OK)
+        rc = nvc_qk_norm_rope_store_fp4(ctx, r->qkv, r->qkv_l, Ly.q_norm, Ly.k_norm, c.rms_norm_eps, r->rope, r->opt.max_model_len, r->d_pos, r->d_slots, &Ly.fp4, nullptr, 0, N,
+                                        r->nh_l, st);
+    } else {
+      rc = nvc_qkv_proj_norm_rope(ctx, r->xn, H, Ly.w_qkv, r->qkv, N, H, Ly.q_norm, Ly.k_norm, c.rms_norm_eps, r->rope, r->d_pos,
+                                  r->d_slots, Ly.k_cache, Ly.v_cache, r->nh_l, r->kv_l, hd, st);
+    }
     if (rc) return rc;
-    if (decode) {
+    if (r->fp4() && (decode || paged_prefill)) {
+      // the same rows of the step over the 4-bit cache
+      const int single = decode ? B : num_decode, ldo = r->nh_l * hd;
+      if (single > 0)
+        rc = nvc_paged_decode_attn_fp4(ctx, r->qkv, r->qkv_l, &Ly.fp4, r->d_bt, r->max_blocks_cap, r->d_ctx, single, r->nh_l, scale, r->attn, ldo, r->decode_ws, r->decode_ws_bytes, st);
+      if (rc == NVC_OK && !decode && B > num_decode)
+        rc = nvc_prefill_attn_paged_fp4(ctx, r->qkv + (size_t)num_decode * r->qkv_l, r->qkv_l, &Ly.fp4, r->d_bt + (size_t)num_decode * r->max_blocks_cap, r->max_blocks_cap,
+                                        r->d_ctx + num_decode, num_decode ? r->d_cu2 : r->d_cu, B - num_decode, N - num_decode, max_seqlen, r->nh_l, scale,
+                                        r->attn + (size_t)num_decode * ldo, ldo, r->decode_ws, r->decode_ws_bytes, st);
+    } else if (decode) {
       rc = nvc_paged_decode_attn_ex(ctx, r->qkv, r->qkv_l, Ly.k_cache, Ly.v_cache, r->d_bt, r->max_blocks_cap, blocks_hint,
                                     r->d_ctx, B, r->nh_l, r->kv_l, hd, r->opt.kvcache_block_size, scale, r->attn,
                                     r->decode_ws, r->decode_ws_bytes, st);
@@ -329,6 +345,8 @@ int nvc_runner_create(nvc_ctx* ctx, const nvc_qwen3_config* cfg, const nvc_runne
                        (opt->kvcache_block_size > 0 && opt->kvcache_block_size % 128 == 0), NVC_ESHAPE,
               "kvcache_block_size must be 16, 32, 64 or a multiple of 128");
   NVC_REQUIRE(ctx, opt->allreduce_f32 == 0, NVC_ENOTIMPL, "allreduce_f32 is not implemented");
+  NVC_REQUIRE(ctx, opt->kv_cache_bits == 0 || opt->kv_cache_bits == 16 || opt->kv_cache_bits == 4, NVC_EINVAL, "kv_cache_bits must be 16 (or 0) or 4");
+  NVC_REQUIRE(ctx, opt->kv_cache_bits != 4 || (int64_t)opt->num_kvcache_blocks * opt->kvcache_block_size <= 0x7fffffffLL, NVC_ESHAPE, "a 4-bit cache has at most 2^31 - 1 slots");
   NVC_REQUIRE(ctx, opt->num_kvcache_blocks > 0 && opt->max_num_seqs > 0 && opt->max_num_batched_tokens > 0 &&
                        opt->max_model_len > 0, NVC_EINVAL, "bad runner options");
   NVC_CUDA_CHECK(ctx, cudaSetDevice(ctx->device));
@@ -361,8 +379,18 @@ int nvc_runner_create(nvc_ctx* ctx, const nvc_qwen3_config* cfg, const nvc_runne
     if ((rc = dev_alloc(r, &L.w_down, (size_t)H * r->I_l))) return rc;
     if ((rc = dev_alloc(r, &L.ln1, H))) return rc;
     if ((rc = dev_alloc(r, &L.ln2, H))) return rc;
-    if ((rc = dev_alloc(r, &L.k_cache, cache_elems))) return rc;
-    if ((rc = dev_alloc(r, &L.v_cache, cache_elems))) return rc;
+    if (r->fp4()) {
+      const size_t rows = cache_elems / 128;
+      L.fp4.num_blocks = opt->num_kvcache_blocks;
+      L.fp4.kv = r->kv_l;
+      L.fp4.block_size = opt->kvcache_block_size;
+      if ((rc = dev_alloc(r, &L.fp4.k, rows * 64)) || (rc = dev_alloc(r, &L.fp4.k_scale, rows * 8)) || (rc = dev_alloc(r, &L.fp4.v, rows * 64)) ||
+          (rc = dev_alloc(r, &L.fp4.v_scale, rows * 8)))
+        return rc;
+    } else {
+      if ((rc = dev_alloc(r, &L.k_cache, cache_elems))) return rc;
+      if ((rc = dev_alloc(r, &L.v_cache, cache_elems))) return rc;
+    }
     r->weight_bytes += 2 * ((int64_t)r->qkv_l * H + (int64_t)H * r->nh_l * hd + 2 * hd + 3 * (int64_t)r->I_l * H + 2 * H);
   }
   if ((rc = dev_alloc(r, &r->embed, (size_t)cfg->vocab_size * H))) return rc;
@@ -397,6 +425,9 @@ int nvc_runner_create(nvc_ctx* ctx, const nvc_qwen3_config* cfg, const nvc_runne
   r->decode_ws_bytes = 0;
   for (int b = 1; b <= opt->max_num_seqs; ++b)
     r->decode_ws_bytes = std::max(r->decode_ws_bytes, nvc_paged_decode_workspace_bytes(b, r->nh_l, hd, ctx->num_sms));
+  if (r->fp4())
+    r->decode_ws_bytes = std::max(nvc_attn_fp4_workspace_bytes(ctx, r->nh_l, r->kv_l, 1),
+                                  std::max(nvc_attn_fp4_workspace_bytes(ctx, r->nh_l, r->kv_l, 16), nvc_attn_fp4_workspace_bytes(ctx, r->nh_l, r->kv_l, opt->max_num_batched_tokens)));
   if ((rc = dev_alloc(r, reinterpret_cast<uint8_t**>(&r->decode_ws), r->decode_ws_bytes))) return rc;
   if ((rc = alloc_step_buffers(r))) return rc;
   return NVC_OK;
@@ -941,6 +972,10 @@ extern "C" int nvc_runner_time_op(nvc_runner* r, int op, int iters, float* ms_pe
       Layer& L = r->layers[li];
       switch (op) {
         case NVC_OP_PAGED_DECODE:
+          if (r->fp4()) {
+            rc = nvc_paged_decode_attn_fp4(ctx, r->qkv, r->qkv_l, &L.fp4, r->d_bt, r->max_blocks_cap, r->d_ctx, B, r->nh_l, scale, r->attn, r->nh_l * hd, r->decode_ws, r->decode_ws_bytes, st);
+            break;
+          }
           rc = nvc_paged_decode_attn_ex(ctx, r->qkv, r->qkv_l, L.k_cache, L.v_cache, r->d_bt, r->max_blocks_cap,
                                         r->last_decode_hint, r->d_ctx, B, r->nh_l, r->kv_l, hd,
                                         r->opt.kvcache_block_size, scale, r->attn, r->decode_ws, r->decode_ws_bytes, st);
@@ -1035,6 +1070,7 @@ extern "C" int nvc_runner_create_from_config(nvc_ctx* ctx, const nvc_model_confi
               "architecture " + mc->architecture + " has no model body");
   NVC_REQUIRE(ctx, ctx->tp_size == 1, NVC_ENOTIMPL, mc->architecture + " runs on one GPU");
   NVC_REQUIRE(ctx, opt->dtype == NVC_DT_BF16 || opt->dtype == NVC_DT_F32, NVC_EINVAL, "dtype must be NVC_DT_BF16 or NVC_DT_F32");
+  NVC_REQUIRE(ctx, opt->kv_cache_bits == 0 || opt->kv_cache_bits == 16, NVC_ENOTIMPL, mc->architecture + " keeps its cache in its own formats");
   NVC_REQUIRE(ctx, opt->num_kvcache_blocks > 0 && opt->kvcache_block_size > 0 && opt->max_num_seqs > 0 &&
                        opt->max_num_batched_tokens > 0 && opt->max_model_len > 0, NVC_EINVAL, "bad runner options");
   NVC_CUDA_CHECK(ctx, cudaSetDevice(ctx->device));

@@ -58,6 +58,7 @@ struct nvc_qwen3_layer {
   nvc_bf16 *w_qkv = nullptr, *w_o = nullptr, *q_norm = nullptr, *k_norm = nullptr;
   nvc_bf16 *w_gu = nullptr, *w_down = nullptr, *ln1 = nullptr, *ln2 = nullptr;
   nvc_bf16 *k_cache = nullptr, *v_cache = nullptr;
+  nvc_fp4_cache fp4{};              // kv_cache_bits = 4: in place of them
 };
 
 struct nvc_arg_pair { float val; int32_t idx; };
@@ -88,6 +89,7 @@ struct nvc_runner {
   float *res_last = nullptr, *logits = nullptr;
   void* decode_ws = nullptr;
   size_t decode_ws_bytes = 0;
+  bool fp4() const { return opt.kv_cache_bits == 4; }
   // step inputs on device + pinned staging
   int32_t* d_state_slots = nullptr;   // state slot of every sequence of the step (bodies with recurrent state)
   std::vector<int32_t> armed_state_slots;

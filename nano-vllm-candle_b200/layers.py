@@ -289,7 +289,9 @@ class Attention:
     """Attention{num_heads, head_dim, scale, softcapping} (attention.rs:4-9) + num_kv_heads and the
     paged KV cache.  forward(q, k, v): q [N, nh*hd], k / v [N, kv*hd] token-major (views into a
     fused qkv buffer are fine); writes k, v to the cache at slot_mapping, then varlen causal flash
-    (prefill) or paged attention over block_tables (decode)."""
+    (prefill) or paged attention over block_tables (decode).
+    fp4_cache (ops.Fp4Cache) in place of k_cache / v_cache keeps the rows in 4 bits; a prefill with block_tables then reads its
+    whole context from there (portions behind a cached prefix), one without attends to its own k, v."""
 
     def __init__(self, ctx, num_heads: int, head_dim: int, scale: float, num_kv_heads: int, softcapping: float = 1.0,
                  block_size: int = 256):
@@ -299,10 +301,20 @@ class Attention:
         self.num_kv_heads, self.block_size = num_kv_heads, block_size
         self.k_cache: Optional[torch.Tensor] = None      # [num_blocks, block_size, kv, hd]
         self.v_cache: Optional[torch.Tensor] = None
+        self.fp4_cache: Optional[ops.Fp4Cache] = None    # num_blocks pages of its own block_size
 
     def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
         c = get_context()
         nh, kv, hd = self.num_heads, self.num_kv_heads, self.head_dim
+        if self.fp4_cache is not None:
+            if self.k_cache is not None:
+                raise RuntimeError("one cache: fp4_cache, or k_cache and v_cache")
+            if c.slot_mapping is not None:
+                ops.store_kvcache_fp4(self.ctx, k, v, self.fp4_cache, c.slot_mapping)
+            if not c.is_prefill:
+                return ops.paged_decode_attn_fp4(self.ctx, q, self.fp4_cache, c.block_tables, c.context_lens, nh, self.scale)
+            if c.block_tables is not None:
+                return ops.prefill_attn_paged_fp4(self.ctx, q, self.fp4_cache, c.block_tables, c.context_lens, c.cu_seqlens, c.max_seqlen, nh, self.scale)
         if self.k_cache is not None and c.slot_mapping is not None:
             self.ctx.store_kvcache(k, v, self.k_cache, self.v_cache, c.slot_mapping, kv, hd)
         if c.is_prefill:
