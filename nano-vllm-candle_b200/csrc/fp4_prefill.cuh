@@ -570,17 +570,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const Args p) {
         const int at_row = x.s.begin + tok;
         const bool there = first + r < real && (unsigned)at_row < (unsigned)p.rows;
         uint4* dst = reinterpret_cast<uint4*>(p.out + at_row * p.ldo + (int64_t)(x.h * p.group + first + r - tok * p.group) * 128);
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          uint32_t v[32];
-          ptx::tmem_ld_32x32b_x32(tmem_o(w) + lane_at + 32 * c, v);
-          ptx::tmem_ld_wait();
-          if (there) {
+        uint32_t v[128];
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              dst[4 * c + k] = make_uint4(pack_bf16(__uint_as_float(v[8 * k]) * inv, __uint_as_float(v[8 * k + 1]) * inv), pack_bf16(__uint_as_float(v[8 * k + 2]) * inv, __uint_as_float(v[8 * k + 3]) * inv),
-                                          pack_bf16(__uint_as_float(v[8 * k + 4]) * inv, __uint_as_float(v[8 * k + 5]) * inv), pack_bf16(__uint_as_float(v[8 * k + 6]) * inv, __uint_as_float(v[8 * k + 7]) * inv));
-          }
+        for (int c = 0; c < 4; ++c) ptx::tmem_ld_32x32b_x32(tmem_o(w) + lane_at + 32 * c, v + 32 * c);
+        ptx::tmem_ld_wait();
+        if (there) {
+#pragma unroll
+          for (int k = 0; k < 16; ++k)
+            dst[k] = make_uint4(pack_bf16(__uint_as_float(v[8 * k]) * inv, __uint_as_float(v[8 * k + 1]) * inv), pack_bf16(__uint_as_float(v[8 * k + 2]) * inv, __uint_as_float(v[8 * k + 3]) * inv),
+                                pack_bf16(__uint_as_float(v[8 * k + 4]) * inv, __uint_as_float(v[8 * k + 5]) * inv), pack_bf16(__uint_as_float(v[8 * k + 6]) * inv, __uint_as_float(v[8 * k + 7]) * inv));
         }
       } else {
         if (begins) note = make_int4(x.b, x.j, x.h, (int)blockIdx.x + 1 + (x.tiles - 1 - x.end) / per);
