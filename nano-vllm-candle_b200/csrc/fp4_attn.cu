@@ -12,8 +12,7 @@ namespace {
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-template <int NT> constexpr int kCtasPerSm = NT == 1 ? 4 : 3;
-template <int NT> int64_t parts_bytes(const nvc_ctx* ctx) { return (int64_t)ctx->num_sms * kCtasPerSm<NT> * (16 + 2 * fp4d::kRecord<NT> * 4); }
+template <int NT> int64_t parts_bytes(const nvc_ctx* ctx) { return (int64_t)ctx->num_sms * fp4d::kCtas<NT> * (16 + 2 * fp4d::kRecord<NT> * 4); }
 
 template <int NT>
 int launch_few(nvc_ctx* ctx, fp4d::Args& p, int64_t most_rows, cudaStream_t stream, size_t workspace_bytes) {
@@ -21,7 +20,7 @@ int launch_few(nvc_ctx* ctx, fp4d::Args& p, int64_t most_rows, cudaStream_t stre
   NVC_REQUIRE(ctx, units * p.B <= 0x7fffffffLL, NVC_ESHAPE, "too many rows and heads");
   const int64_t most = units * p.B * (((int64_t)p.bt_stride * p.block_size + fp4d::kTile - 1) / fp4d::kTile + fp4d::kUnitCost);      // the list's length, at most
   const int64_t a_cta = (1 + fp4d::kUnitCost) * fp4d::kWarps;
-  const int grid = (int)std::min<int64_t>((int64_t)ctx->num_sms * kCtasPerSm<NT>, (most + a_cta - 1) / a_cta);
+  const int grid = (int)std::min<int64_t>((int64_t)ctx->num_sms * fp4d::kCtas<NT>, (most + a_cta - 1) / a_cta);
   NVC_REQUIRE(ctx, p.notes && ((uintptr_t)p.notes & 15) == 0 && workspace_bytes >= (size_t)parts_bytes<NT>(ctx), NVC_ENOMEM, "workspace too small");
   p.parts = reinterpret_cast<float*>(p.notes + grid);
   p.warps = grid * fp4d::kWarps;

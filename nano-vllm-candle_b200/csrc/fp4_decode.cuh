@@ -22,10 +22,9 @@
 
 namespace fp4d {
 
-constexpr int kTile = 32, kHalf = 16, kStages = 2, kWarps = 4;
+constexpr int kTile = 32, kHalf = 16, kWarps = 4;
 constexpr int kAtV = kTile * kFp4Codes, kAtKs = 2 * kAtV, kAtVs = kAtKs + kTile * kFp4Scales;      // of a stage: K codes, V codes, K scales, V scales
 constexpr int kStageBytes = kAtVs + kTile * kFp4Scales;
-constexpr int kRingBytes = kStages * kStageBytes;
 constexpr float kFloor = -3.0e38f;                                     // a piece's reference for a column that saw nothing in it
 constexpr float kShift = 7.0f, kMost = 15.0f;
 constexpr int kUnitCost = 2;
@@ -43,6 +42,10 @@ struct Args {
   int warps;                                                           // of the attention kernel's grid
 };
 
+// CTAs of an SM.  16 columns: 229 registers, of 168 (three CTAs) some go to memory: 256 contexts of 2 000, us: 186 / 172, 32 of 1 750 37 / 31.  8 columns: 4 and 3 CTAs alike
+template <int NT> constexpr int kCtas = NT == 1 ? 4 : 2;
+constexpr int kRing = 2;                                               // tiles of a warp's ring (three and four: no difference)
+constexpr int kRingBytes = kRing * kStageBytes;
 template <int NT> constexpr int kCols = 8 * NT;
 template <int NT> constexpr int kRecord = kCols<NT> * 130;             // floats: O [cols][128], reference [cols], sum [cols]
 template <int NT> constexpr int kWarpBytes = kRingBytes + kRecord<NT> * 4;     // a stretch's last piece goes where the ring was
@@ -200,10 +203,10 @@ __device__ __forceinline__ bool column(const Args& p, const Seq& s, int b, int u
 }
 
 template <int NT>
-__global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 3) attn_kernel(const Args p) {
+__global__ void __launch_bounds__(32 * kWarps, kCtas<NT>) attn_kernel(const Args p) {
   pdl_trigger();
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ __align__(8) uint64_t bars[kWarps][kStages];
+  __shared__ __align__(8) uint64_t bars[kWarps][kRing];
   __shared__ int4 pieces[kWarps][2];                  // sequence (-1: no piece), unit, first tile, tile behind the last
   __shared__ int tiles_of[kWarps][2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -211,7 +214,7 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 3) attn_kernel(cons
   const uint32_t bar = smem_u32(&bars[warp][0]);
   if (lane == 0) {
 #pragma unroll
-    for (int i = 0; i < kStages; ++i) ptx::mbar_init(bar + 8 * i, 1);
+    for (int i = 0; i < kRing; ++i) ptx::mbar_init(bar + 8 * i, 1);
     ptx::fence_barrier_init();
   }
   __syncwarp();
@@ -222,7 +225,7 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 3) attn_kernel(cons
   Piece at;
   bool any = first_piece<NT>(p, list, (int64_t)per * (blockIdx.x * kWarps + warp), per, lane, at);
 
-  // ---- the reading side: a tile ahead.  Lane 0 copies; the others know which rows are not there
+  // ---- the reading side: ahead by what the ring holds.  Lane 0 copies; the others know which rows are not there
   const int per_page = p.block_size / kHalf, last_page = p.bt_stride - 1;
   const bool whole = (per_page & 1) == 0;             // a tile lies in one page
   Piece rd = at;
@@ -436,15 +439,17 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 4 : 3) attn_kernel(cons
     const uint32_t at_v = (uint32_t)(kAtV + rv * kFp4Codes + g * 8), at_v1 = (uint32_t)(kAtV + (rv ^ 1) * kFp4Codes + g * 8);
     const uint32_t at_vs = (uint32_t)(kAtVs + rv * kFp4Scales + g), at_vs1 = (uint32_t)(kAtVs + (rv ^ 1) * kFp4Scales + g);
     load_q();
-    issue(0);
+#pragma unroll
+    for (int i = 0; i < kRing - 1; ++i) issue(i);
     begin();
 #pragma unroll 1
     for (int i = 0;; ++i) {
       __syncwarp();                                   // everyone is done with the stage that is filled now
-      issue((i + 1) & 1);
-      uint32_t st = ring + (i & 1) * kStageBytes;
-      wait_bar(bar + 8 * (i & 1), (i >> 1) & 1);
-      const uint32_t gone = (absent >> (2 * (i & 1))) & 3u;
+      issue((i + kRing - 1) % kRing);
+      const int stage = i % kRing;
+      uint32_t st = ring + stage * kStageBytes;
+      wait_bar(bar + 8 * stage, (i / kRing) & 1);
+      const uint32_t gone = (absent >> (2 * stage)) & 3u;
       if (gone || (at.t + 1) * kTile > at.s.len) {    // rows that are not there: scales of 0, whatever their codes are
         if ((gone >> (lane >> 4)) & 1 || at.t * kTile + lane >= at.s.len) {
           asm volatile("st.shared.v2.u32 [%0], {%1, %1};" ::"r"(st + kAtKs + lane * kFp4Scales), "r"(0) : "memory");
