@@ -17,7 +17,6 @@ template <int NT> int64_t parts_bytes(const nvc_ctx* ctx) { return (int64_t)ctx-
 template <int NT>
 int launch_few(nvc_ctx* ctx, fp4d::Args& p, int64_t most_rows, cudaStream_t stream, size_t workspace_bytes) {
   const int64_t units = p.kv * ((most_rows + fp4d::kCols<NT> - 1) / fp4d::kCols<NT>);          // of a sequence, at most
-  NVC_REQUIRE(ctx, units * p.B <= 0x7fffffffLL, NVC_ESHAPE, "too many rows and heads");
   const int64_t most = units * p.B * (((int64_t)p.bt_stride * p.block_size + fp4d::kTile - 1) / fp4d::kTile + fp4d::kUnitCost);      // the list's length, at most
   const int64_t a_cta = (1 + fp4d::kUnitCost) * fp4d::kWarps;
   const int grid = (int)std::min<int64_t>((int64_t)ctx->num_sms * fp4d::kCtas<NT>, (most + a_cta - 1) / a_cta);
@@ -60,11 +59,11 @@ int attn_fp4(nvc_ctx* ctx, const nvc_bf16* q, int ldq, const nvc_fp4_cache* cach
   if (B == 0 || rows == 0 || max_qlen == 0) return NVC_OK;
   const int group = nh / cache->kv;
   const int64_t most_rows = most_rows_of(rows, max_qlen, group);             // of a sequence and key head
-  NVC_REQUIRE(ctx, most_rows <= 0x7ffffff0LL, NVC_ESHAPE, "too many rows");
+  NVC_REQUIRE(ctx, (int64_t)rows * group <= 0x7fffffffLL, NVC_ESHAPE, "too many rows");
   fp4d::Args p{q, out, ldq, ldo, cache->k, cache->k_scale, cache->v, cache->v_scale, block_tables, context_lens, cu_seqlens_q, bt_stride, cache->num_blocks, cache->kv,
                cache->block_size, B, group, rows, scale * 1.4426950408889634f, static_cast<int4*>(workspace), nullptr, 0};
   DeviceGuard guard(ctx->device);
-  if (most_rows > kFewRows) return launch_many(ctx, p, scale, nvc_stream(stream), workspace_bytes);
+  if (cu_seqlens_q && most_rows > kFewRows) return launch_many(ctx, p, scale, nvc_stream(stream), workspace_bytes);
   return most_rows <= 8 ? launch_few<1>(ctx, p, most_rows, nvc_stream(stream), workspace_bytes) : launch_few<2>(ctx, p, most_rows, nvc_stream(stream), workspace_bytes);
 }
 
@@ -80,7 +79,8 @@ extern "C" int nvc_fp4_attn_init(nvc_ctx* ctx) {
 extern "C" size_t nvc_attn_fp4_workspace_bytes(const nvc_ctx* ctx, int nh, int kv, int max_seqlen_q) {
   if (!ctx || nh <= 0 || kv <= 0 || max_seqlen_q <= 0) return 0;
   const int64_t rows = most_rows_of(max_seqlen_q, max_seqlen_q, (nh + kv - 1) / kv);
-  return rows > kFewRows ? many_bytes(ctx) : (size_t)(rows <= 8 ? parts_bytes<1>(ctx) : parts_bytes<2>(ctx));
+  const size_t few = (size_t)(rows <= 8 ? parts_bytes<1>(ctx) : parts_bytes<2>(ctx));          // (decode: whatever its rows are)
+  return rows > kFewRows ? std::max(few, many_bytes(ctx)) : few;
 }
 
 extern "C" int nvc_paged_decode_attn_fp4(nvc_ctx* ctx, const nvc_bf16* q, int ldq, const nvc_fp4_cache* cache, const int32_t* block_tables, int bt_stride,

@@ -162,6 +162,7 @@ int nvc_fp4_cache_check(nvc_ctx* ctx, const nvc_fp4_cache* c) {
   NVC_REQUIRE(ctx, c->num_blocks > 0 && c->kv > 0 && c->block_size > 0, NVC_EINVAL, "bad sizes of the cache");
   NVC_REQUIRE(ctx, c->block_size % 16 == 0, NVC_ESHAPE, "block_size must be a multiple of 16");
   NVC_REQUIRE(ctx, (int64_t)c->num_blocks * c->block_size <= 0x7fffffffLL, NVC_ESHAPE, "a cache has at most 2^31 - 1 slots");
+  NVC_REQUIRE(ctx, (int64_t)c->num_blocks * (c->block_size / 16) * c->kv <= 0xffffffffLL, NVC_ESHAPE, "a cache has at most 2^36 rows");
   NVC_REQUIRE(ctx, aligned16(c->k) && aligned16(c->k_scale) && aligned16(c->v) && aligned16(c->v_scale), NVC_EINVAL, "the cache's parts must be 16-byte aligned");
   return NVC_OK;
 }

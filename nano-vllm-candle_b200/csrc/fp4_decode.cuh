@@ -14,6 +14,9 @@
 // GPU once; a unit counts as kUnitCost tiles more than it has, for its queries and its result.  A unit inside a warp's stretch is written by it; the pieces of others are joined in shared memory
 // where the warps are of one CTA, and by a second kernel (combine) where not.  Contexts of any mixture of lengths thus take the time of their sum.
 //
+// A cached value that is no number counts for the columns that see it, and for no other: where a tile is not seen whole by every column, such a value goes in as 0 (a weight of 0 would not keep
+// it out), and the first token that has one in each block of 16 dims is remembered for the columns that do see it.
+//
 // The exponentials are taken against a reference that follows a column's maximum only when that grew by more than 2^8 (a vote; nothing is exchanged otherwise), shifted by 2^7: weights lie
 // below 2^15, inside fp16, and those down to 2^-31 of the largest are kept.  Queries are brought to fp16 behind a power of two of their own, that the score's factor takes back.
 #pragma once
@@ -85,6 +88,11 @@ __device__ __forceinline__ uint4 lds128(uint32_t a) {
 __device__ __forceinline__ uint2 lds64(uint32_t a) {
   uint2 v;
   asm("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint2 lds64_now(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
   return v;
 }
 __device__ __forceinline__ uint32_t lds16(uint32_t a) {
@@ -209,6 +217,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<NT>) attn_kernel(const Args
   __shared__ __align__(8) uint64_t bars[kWarps][kRing];
   __shared__ int4 pieces[kWarps][2];                  // sequence (-1: no piece), unit, first tile, tile behind the last
   __shared__ int tiles_of[kWarps][2];
+  __shared__ int nan_from[kWarps][8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   if (lane < 2) pieces[warp][lane] = make_int4(-1, 0, 0, 0);
   const uint32_t bar = smem_u32(&bars[warp][0]);
@@ -334,6 +343,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<NT>) attn_kernel(const Args
     int lim[NT][2], least = 0;                        // keys that this thread's columns see, and the unit's column that sees least
     int begun = 0;                                    // first tile of this piece
     bool head_piece = true;                           // the stretch's first
+    bool odd = false;                                 // nan_from has something
     bool fresh = true;                                // no tile of the piece has been looked at: the references are 0, and take the first maximum
     int limit[NT];                                    // of column g
 
@@ -351,6 +361,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<NT>) attn_kernel(const Args
     auto begin = [&] {
       begun = at.t;
       fresh = true;
+      odd = false;
       least = at.s.len;
 #pragma unroll
       for (int x = 0; x < NT; ++x) {
@@ -393,6 +404,17 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<NT>) attn_kernel(const Args
         for (int c = 0; c < 2; ++c)
 #pragma unroll
           for (int w = 4; w < 32; w <<= 1) sum[x][c] += __shfl_xor_sync(0xffffffffu, sum[x][c], w);
+      if (odd) {                                        // this thread's dims are block g
+        const int from = nan_from[warp][g];
+#pragma unroll
+        for (int x = 0; x < NT; ++x)
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+            if (from < lim[x][c]) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) o[x][j][c] = o[x][j][c + 2] = __uint_as_float(0x7fffffffu);
+            }
+      }
       if (begins && ends) {
 #pragma unroll
         for (int x = 0; x < NT; ++x)
@@ -457,6 +479,22 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<NT>) attn_kernel(const Args
         }
         ptx::fence_proxy_async_smem();
         __syncwarp();
+      }
+      if (p.cu_seqlens && (at.t + 1) * kTile > least) {
+        const uint2 scales = lds64_now(st + kAtVs + lane * kFp4Scales);
+        const uint32_t lo = __vcmpeq4(scales.x, 0xffffffffu), hi = __vcmpeq4(scales.y, 0xffffffffu);
+        if (__any_sync(0xffffffffu, lo | hi)) {
+          if (!odd && lane < 8) nan_from[warp][lane] = 0x7fffffff;
+          odd = true;
+          __syncwarp();
+          if (lo | hi) {
+            for (int i = 0; i < 8; ++i)
+              if ((i < 4 ? lo : hi) >> (8 * (i & 3)) & 1) atomicMin(&nan_from[warp][i], at.t * kTile + lane);
+            asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(st + kAtVs + lane * kFp4Scales), "r"(scales.x & ~lo), "r"(scales.y & ~hi) : "memory");
+          }
+          ptx::fence_proxy_async_smem();
+          __syncwarp();
+        }
       }
       asm volatile("" : "+r"(st)::"memory");
       // ---- S^T = K Q^T: of each half, rows g and g + 8

@@ -9,6 +9,9 @@
 // Queries are brought to fp16 behind a power of two of their own row, that the score's factor takes back.  The sign of the scale goes with them, so that a row's maximum may be taken in front of
 // the factor.
 //
+// A cached value that is no number counts for the rows that see it, and for no other.  A weight of 0 would not keep it from them, so it goes in as 0, and the first token with a NaN in each
+// block of 16 dims is remembered: a row that sees it has NaN there.
+//
 // Work is cut as in the kernel for few rows: the key tiles of all (sequence, 256 rows, key head) units in one list, an equal stretch for each CTA; units that lie in several CTAs are joined by
 // combine_kernel from records in the workspace.
 #pragma once
@@ -20,10 +23,11 @@ namespace fp4p {
 constexpr int kKT = 128, kRows = 256, kThreads = 512;
 constexpr int kTileBytes = 128 * 128 * 2;                  // fp16, two halves of 64 dims: [128 rows][128 bytes], 16-byte chunks permuted by the row
 constexpr int kHalf = kTileBytes / 2;
-constexpr int kOffQ = 0, kOffK = 2 * kTileBytes, kOffV = kOffK + 2 * kTileBytes, kOffFactor = kOffV + 2 * kTileBytes, kOffBar = kOffFactor + kRows * 4;
+constexpr int kOffQ = 0, kOffK = 2 * kTileBytes, kOffV = kOffK + 2 * kTileBytes, kOffFactor = kOffV + 2 * kTileBytes, kOffNan = kOffFactor + kRows * 4, kOffPark = kOffNan + 4 * 48;
+constexpr int kOffBar = kOffPark + 8 * 96 + 16;
 constexpr int kNumBars = 18;
 constexpr int kSmemBytes = kOffBar + kNumBars * 8 + 16 + 1024;          // and room to begin at a multiple of 1024
-constexpr int kUnitCost = 4;                               // a unit's queries and result, in tiles (a prompt of 8 191: 2 635 us, 3 534, 4 517, 6 530)
+constexpr int kUnitCost = 5;                               // a unit's queries and result, in tiles (a prompt of 8 191 in us: 4 470, 5 438, 6 439, 9 451)
 constexpr float kFloor = -1.0e30f, kShift = 7.0f, kGrow = 8.0f;
 constexpr int kRecord = kRows * 130;                       // floats: O [32 groups of 4 dims][256 rows][4], reference [256], sum [256]
 constexpr int kChunk = 2048;                               // sequences whose weights are looked at together (in shared memory)
@@ -128,6 +132,12 @@ struct Piece {
     t = max(0, into - kUnitCost);
     end = min(tiles, rest - kUnitCost);
     return end > t;
+  }
+  __device__ __forceinline__ void park(volatile int* to) const {
+    to[0] = b; to[1] = j; to[2] = h; to[3] = t; to[4] = end; to[5] = tiles; to[6] = rest; to[7] = s.len; to[8] = s.qlen; to[9] = s.begin; to[10] = s.blocks;
+  }
+  __device__ __forceinline__ void take(const volatile int* from) {
+    b = from[0]; j = from[1]; h = from[2]; t = from[3]; end = from[4]; tiles = from[5]; rest = from[6]; s.len = from[7]; s.qlen = from[8]; s.begin = from[9]; s.blocks = from[10];
   }
 };
 __device__ __forceinline__ bool next_piece(const Args& p, Piece& x) {
@@ -345,6 +355,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const Args p) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     // ------------------------------------------------------------ the cache's rows, decoded: a thread has a token of the tile
     const int r = threadIdx.x - 256;
+    int* const nan_from = reinterpret_cast<int*>(gen + kOffNan);      // [piece % 4][block; 8: whether there is one; 3 more]
     struct Raw { uint4 c[4]; uint2 s; };
     const int last_page = p.bt_stride - 1;
     auto block_of = [&](const Piece& x, int tile) {        // of this thread's token; -1 where it has none
@@ -386,7 +397,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const Args p) {
       ptx::fence_proxy_async_smem();
       ptx::mbar_arrive(bar);
     };
-    uint32_t g = 0;
+    uint32_t g = 0, done = 0;
     bool more = true;
     Raw rk, rv;
     int b1 = block_of(at, at.t), b2 = at.t + 1 < at.end ? block_of(at, at.t + 1) : -1, b3;
@@ -400,6 +411,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const Args p) {
       write(rk, base + kOffK + (g & 1) * kTileBytes, k_full(g & 1));
       if (x.t + 1 < x.end) rk = load(x, x.t + 1, b2, p.kc, p.ks);
       else if (more) rk = load(at, at.t, nb, p.kc, p.ks);
+      // (the piece four before this one has been written out: the last V went in when a tile of the one three before, at the latest, was through its P V)
+      if (r < 9) nan_from[12 * (done & 3) + r] = r < 8 ? 0x7fffffff : 0;
+      ptx::named_bar_sync(1, 128);
       for (int j = x.t; j < x.end; ++j, ++g) {
         // b2: the next tile's block; K runs a tile ahead of V
         b3 = j + 2 < x.end ? block_of(x, j + 2) : -1;
@@ -410,10 +424,21 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const Args p) {
           else if (more) rk = load(at, at.t, nb, p.kc, p.ks);
         }
         wait_bar(v_empty(g & 1), ((g >> 1) & 1) ^ 1u);
+        {
+          uint32_t bad[2] = {__vcmpeq4(rv.s.x, 0xffffffffu), __vcmpeq4(rv.s.y, 0xffffffffu)};
+          if (bad[0] | bad[1]) {
+            for (int i = 0; i < 8; ++i)
+              if (bad[i >> 2] >> (8 * (i & 3)) & 1) atomicMin(nan_from + 12 * (done & 3) + i, j * kKT + r);
+            nan_from[12 * (done & 3) + 8] = 1;
+            rv.s.x &= ~bad[0];
+            rv.s.y &= ~bad[1];
+          }
+        }
         write(rv, base + kOffV + (g & 1) * kTileBytes, v_full(g & 1));
         if (j + 1 < x.end) rv = load(x, j + 1, b2, p.vc, p.vs);
         b2 = b3;
       }
+      ++done;
       if (more) {
         rv = load(at, at.t, nb, p.vc, p.vs);
         b2 = at.t + 1 < at.end ? block_of(at, at.t + 1) : -1;
@@ -426,9 +451,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const Args p) {
     const uint32_t lane_at = (uint32_t)(quad * 32) << 16;
     float* const factors = reinterpret_cast<float*>(gen + kOffFactor) + w * 128;
     uint8_t* const q_tile = gen + kOffQ + w * kTileBytes;
-    uint32_t g = 0;
+    const int* const nan_from = reinterpret_cast<const int*>(gen + kOffNan);
+    // what a piece's tiles do not need lies in shared memory meanwhile (with it in registers some of a row's scores went to memory: a prompt of 8 191 in 537 us for 456)
+    volatile int* const park = reinterpret_cast<volatile int*>(gen + kOffPark) + warp * 24;
+    int4* const note = reinterpret_cast<int4*>(gen + kOffPark + 8 * 96);
+    if (threadIdx.x == 0) *note = make_int4(-1, 0, 0, 0);
+    uint32_t g = 0, done = 0;
     bool more = true;
-    int4 note = make_int4(-1, 0, 0, 0);
     // This warp's 32 rows of a piece's Q, 16 lanes a row: all of it on its way, then to shared memory (that every product of the piece before has read: its last S has been seen)
     uint4 y[16];
     auto fetch = [&](const Piece& x) {
@@ -469,22 +498,27 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const Args p) {
     fetch(at);
     place();
     while (more) {
-      const Piece x = at;
-      more = next_piece(p, at);                            // (its lengths are on their way meanwhile)
-      const int first = kRows * x.j + 128 * w;             // packed row of the tile's first
-      const int real = x.s.qlen * p.group;                 // (at most 2^31: the host's check)
+      int lim, least, n, t0;                               // the last key that the row sees, and the warp's first row; tiles; the next tile's first key
+      {
+        const Piece x = at;
+        more = next_piece(p, at);                          // (its lengths are on their way meanwhile)
+        if (lane == 0) {
+          x.park(park);
+          at.park(park + 11);
+        }
+        const int first = kRows * x.j + 128 * w;           // packed row of the tile's first
+        lim = x.s.len - x.s.qlen + min(p.by_group(first + r), x.s.qlen - 1);
+        least = x.s.len - x.s.qlen + p.by_group(first + quad * 32);
+        n = x.end - x.t;
+        t0 = x.t * kKT;
+        if (more) ahead(at);
+      }
       __syncwarp();
       const float factor = factors[r];
-      const int tok = p.by_group(first + r);
-      const int lim = x.s.len - x.s.qlen + min(tok, x.s.qlen - 1);          // the last key that the row sees
-      const int least = x.s.len - x.s.qlen + p.by_group(first + quad * 32);   // of the warp's rows
-      if (more) ahead(at);
       float ref = kFloor, sum = 0.f;
-      const int n = x.end - x.t;
-      for (int j = 0; j < n; ++j, ++g) {
+      for (int j = 0; j < n; ++j, ++g, t0 += kKT) {
         wait_bar(s_full(w), g & 1);
         ptx::tcgen05_fence_after();
-        const int t0 = (x.t + j) * kKT;
         const bool cut = t0 + kKT - 1 > least;
         const int l = lim - t0;
         uint32_t sv[128];
@@ -520,20 +554,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const Args p) {
         }
         uint64_t s0 = 0, s1 = 0;                           // two sums each
         const uint64_t by = pair(factor, factor), less = pair(-ref, -ref);
-        auto weights = [&](int from) {                     // of 64 columns
+        auto weights = [&](int from, uint32_t* to) {       // of 32 columns
 #pragma unroll
-          for (int i = from; i < from + 64; i += 4) {
-            const uint64_t y = fma2(pair(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])), by, less), z = fma2(pair(__uint_as_float(sv[i + 2]), __uint_as_float(sv[i + 3])), by, less);
+          for (int i = 0; i < 32; i += 4) {
+            const uint64_t y = fma2(pair(__uint_as_float(sv[from + i]), __uint_as_float(sv[from + i + 1])), by, less), z = fma2(pair(__uint_as_float(sv[from + i + 2]), __uint_as_float(sv[from + i + 3])), by, less);
             const float p0 = ex2(lo_of(y)), p1 = ex2(hi_of(y)), p2 = ex2(lo_of(z)), p3 = ex2(hi_of(z));
             s0 = add2(s0, pair(p0, p1));
             s1 = add2(s1, pair(p2, p3));
-            sv[i >> 1] = halves(p0, p1);
-            sv[(i >> 1) + 1] = halves(p2, p3);
+            to[i >> 1] = halves(p0, p1);
+            to[(i >> 1) + 1] = halves(p2, p3);
           }
         };
-        weights(0);
         if (j > 0) {
-          // the product of the tile before has been added to O.  Looked at in every tile, so that no phase of the barrier is missed
+          // the product of the tile before has been added to O, and has read its P.  Looked at in every tile, so that no phase of the barrier is missed
           wait_bar(o_done(w), (g - 1) & 1);
           if (move) {
             ptx::tcgen05_fence_after();
@@ -548,23 +581,47 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const Args p) {
             }
           }
         }
-        ptx::tmem_st_32x32b_x32(tmem_p(w) + lane_at, sv);
-        weights(64);
+        uint32_t pw[16];
+        weights(0, pw);
+        tmem_st_x16(tmem_p(w) + lane_at + 0, pw);
+        weights(32, pw);
+        tmem_st_x16(tmem_p(w) + lane_at + 16, pw);
+        weights(64, pw);
+        tmem_st_x16(tmem_p(w) + lane_at + 32, pw);
+        weights(96, pw);
+        tmem_st_x16(tmem_p(w) + lane_at + 48, pw);
         s0 = add2(s0, s1);
         sum = sum * alpha + (lo_of(s0) + hi_of(s0));
-        ptx::tmem_st_32x32b_x32(tmem_p(w) + lane_at + 32, sv + 32);
         ptx::tmem_st_wait();
         ptx::tcgen05_fence_before();
         ptx::mbar_arrive(p_full(w));
       }
       // ---- the result, or this CTA's part of it
+      at.take(park + 11);
       if (more) {                                          // the next one's queries first: its S is made while this one's O is written
         fetch(at);
         place();
       }
+      Piece x;
+      x.take(park);
+      const int first = kRows * x.j + 128 * w, real = x.s.qlen * p.group, tok = p.by_group(first + r);          // (below 2^31: the host's check)
       wait_bar(o_done(w), (g - 1) & 1);
       ptx::tcgen05_fence_after();
       const bool begins = x.t == 0, ends = x.end == x.tiles;
+      const int* const from = nan_from + 12 * (done++ & 3);
+      if (from[8]) {                                       // (a NaN in the cache: into O where the row sees it, 16 columns at a time)
+#pragma unroll 1
+        for (int c = 0; c < 8; ++c) {
+          uint32_t v[16];
+          ptx::tmem_ld_32x32b_x16(tmem_o(w) + lane_at + 16 * c, v);
+          ptx::tmem_ld_wait();
+          const bool bad = from[c] <= lim;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] = bad ? 0x7fffffffu : v[i];
+          tmem_st_x16(tmem_o(w) + lane_at + 16 * c, v);
+        }
+        ptx::tmem_st_wait();
+      }
       if (begins && ends) {
         const float inv = sum == 0.f ? 0.f : 1.0f / sum;   // seen nothing: zeros
         const int at_row = x.s.begin + tok;
@@ -581,7 +638,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const Args p) {
                                 pack_bf16(__uint_as_float(v[8 * k + 4]) * inv, __uint_as_float(v[8 * k + 5]) * inv), pack_bf16(__uint_as_float(v[8 * k + 6]) * inv, __uint_as_float(v[8 * k + 7]) * inv));
         }
       } else {
-        if (begins) note = make_int4(x.b, x.j, x.h, (int)blockIdx.x + 1 + (x.tiles - 1 - x.end) / per);
+        if (begins && threadIdx.x == 0) *note = make_int4(x.b, x.j, x.h, (int)blockIdx.x + 1 + (x.tiles - 1 - x.end) / per);
         float* part = p.parts + ((int64_t)blockIdx.x * 2 + (begins ? 1 : 0)) * kRecord;
         const int row = 128 * w + r;
 #pragma unroll 1
@@ -598,7 +655,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const Args p) {
       }
       ptx::tcgen05_fence_before();                         // O has been read: the next P V may write it (p_full)
     }
-    if (threadIdx.x == 0) p.notes[blockIdx.x] = note;
+    if (threadIdx.x == 0) p.notes[blockIdx.x] = *note;
   }
   ptx::tcgen05_fence_before();
   __syncthreads();

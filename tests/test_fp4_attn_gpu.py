@@ -209,3 +209,95 @@ def test_captured_and_replayed_on_other_streams(ctx):
         torch.cuda.synchronize()
         for c, _, _, _, out in sides:
             _near(out, c)
+
+
+MANY = dict(new=[70, 33], before=[30, 150], nh=8, kv=2, bs=16)          # 280 rows of a key head: the kernel on tcgen05; 4 rows a token
+
+
+def _many(seed=0, **over):
+    m = {**MANY, **over}
+    return _case([n + b for n, b in zip(m["new"], m["before"])], m["nh"], m["kv"], m["bs"], new=m["new"], seed=seed, size=m.get("size", 1.0))
+
+
+@pytest.mark.parametrize("size,scale", [(0.01, 1.0), (30.0, 128 ** -0.5), (1.0, -0.1), (1.0, 0.0), (300.0, 1.0), (300.0, -1.0)])
+def test_long_portions_of_flat_and_peaked_rows(ctx, size, scale):
+    c = _many(seed=9, size=size)
+    _near(_portions(ctx, c, scale), c, scale)
+
+
+@pytest.mark.parametrize("size", [2.0 ** -60, 2.0 ** 15, 2.0 ** 60])
+def test_long_portions_with_queries_of_any_size(ctx, size):
+    c = _many(seed=12)
+    c["q"] = (c["q"].float() * size).to(BF16)
+    _near(_portions(ctx, c, 128 ** -0.5 / size), c, 128 ** -0.5 / size)
+
+
+@pytest.mark.parametrize("new,kv,group", [([5], 2, 1), ([9, 4], 2, 4), ([70, 33], 2, 4), ([40], 1, 12)])
+def test_numbers_that_are_none_behind_a_mask(ctx, new, kv, group):
+    """A cached value or key that is no number, among the portion's own tokens: the rows in front of it do not see it, and are what they are without it."""
+    nh = kv * group
+    c = _case([n + 40 for n in new], nh, kv, 16, new=new, seed=21)
+    clean = _portions(ctx, c).view(-1, nh, 128)
+    at = 40 + new[0] // 2                                              # a token of the first sequence
+    blk, off = int(c["tables"][0, at // 16]), at % 16
+    c["cache"].v_scale[blk, 0, off, 2] = 255
+    got = _portions(ctx, c).view(-1, nh, 128)
+    first = at - 40
+    mine = slice(0, group)
+    assert torch.equal(got[:first], clean[:first]) and torch.equal(got[new[0]:], clean[new[0]:]) and torch.equal(got[:, group:], clean[:, group:])
+    seen = got[first:new[0], mine]
+    assert torch.isnan(seen[..., 32:48]).all() and torch.isfinite(seen[..., :32]).all() and torch.isfinite(seen[..., 48:]).all()
+    c["cache"].k_scale[blk, 0, off, 7] = 255
+    got = _portions(ctx, c).view(-1, nh, 128)
+    assert torch.equal(got[:first], clean[:first]) and torch.isnan(got[first:new[0], mine]).all() and torch.equal(got[:, group:], clean[:, group:])
+
+
+def test_queries_of_long_portions_that_are_none(ctx):
+    c = _many(seed=8)
+    clean = _portions(ctx, c).view(-1, 8, 128)
+    c["q"][3, 130], c["q"][60, 5 * 128] = float("nan"), float("inf")
+    got = _portions(ctx, c).view(-1, 8, 128)
+    assert torch.isnan(got[3, 1]).all() and torch.isnan(got[60, 5]).all()
+    same = torch.ones(got.shape[:2], dtype=torch.bool, device=DEV)
+    same[3, 1] = same[60, 5] = False
+    assert torch.equal(got[same], clean[same])
+
+
+@pytest.mark.parametrize("nh,kv", [(72, 1), (130, 1), (65, 1), (96, 4)])
+def test_decode_of_many_heads_to_a_key_head(ctx, nh, kv):
+    c = _case([50, 0, 3], nh, kv, 16, seed=4)
+    _near(_decode(ctx, c), c)
+
+
+def test_many_sequences(ctx):
+    """More sequences than the schedule looks at in one go: 2 100 of one token and 65 heads, and 700 of decode."""
+    g = torch.Generator().manual_seed(3)
+    lens = torch.randint(0, 40, (2100,), generator=g).tolist()
+    c = _case(lens, 65, 1, 16, seed=5)
+    _near(_portions(ctx, c), c)
+    d = _case(lens[:700], 4, 2, 16, seed=6)
+    _near(_decode(ctx, d), d)
+
+
+def test_pages_far_into_a_long_cache(ctx):
+    """Pages beyond 2^32 bytes of codes."""
+    kv, bs, blocks, nh = 8, 256, 36000, 16
+    k, ks = torch.empty(blocks, kv, bs, 64, dtype=U8, device=DEV), torch.empty(blocks, kv, bs, 8, dtype=U8, device=DEV)
+    cache = ops.Fp4Cache(k, ks, torch.empty_like(k), torch.empty_like(ks))
+    table = torch.tensor([[blocks - 1, 33333, 0]], dtype=I32, device=DEV)
+    n = 300
+    pos = torch.arange(n, device=DEV)
+    slots = (table[0, pos // bs] * bs + pos % bs).to(I32)
+    rows = [torch.randn(n, kv * 128, generator=_g(i), device=DEV).to(BF16) for i in (1, 2)]
+    ops.store_kvcache_fp4(ctx, *rows, cache, slots)
+    for new in ([1], [5], [40]):
+        c = dict(q=torch.randn(new[0], nh * 128, generator=_g(3), device=DEV).to(BF16), cache=cache, tables=table, lens=torch.tensor([n], dtype=I32, device=DEV),
+                 cu=torch.tensor([0] + new, dtype=I32, device=DEV), new=new, nh=nh)
+        _near(_portions(ctx, c) if new[0] > 1 else _decode(ctx, c), c)
+
+
+def test_portions_of_a_bound_that_is_too_low(ctx):
+    """max_seqlen_q chooses the kernel; a row's result does not depend on its being right."""
+    c = _many(seed=30)
+    got = ops.prefill_attn_paged_fp4(ctx, c["q"], c["cache"], c["tables"], c["lens"], c["cu"], 2, 8, 128 ** -0.5)
+    _near(got, c)
