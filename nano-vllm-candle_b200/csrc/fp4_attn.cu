@@ -23,7 +23,7 @@ int launch_few(nvc_ctx* ctx, fp4d::Args& p, int64_t most_rows, cudaStream_t stre
   NVC_REQUIRE(ctx, p.notes && ((uintptr_t)p.notes & 15) == 0 && workspace_bytes >= (size_t)parts_bytes<NT>(ctx), NVC_ENOMEM, "workspace too small");
   p.parts = reinterpret_cast<float*>(p.notes + grid);
   p.warps = grid * fp4d::kWarps;
-  NVC_CUDA_CHECK(ctx, nvc_launch(ctx, fp4d::attn_kernel<NT>, dim3(grid), dim3(32 * fp4d::kWarps), (size_t)fp4d::kSmem<NT>, stream, p));
+  NVC_CUDA_CHECK(ctx, nvc_launch(ctx, p.cu_seqlens ? fp4d::attn_kernel<NT, true> : fp4d::attn_kernel<NT, false>, dim3(grid), dim3(32 * fp4d::kWarps), (size_t)fp4d::kSmem<NT>, stream, p));
   NVC_CUDA_CHECK(ctx, nvc_launch(ctx, fp4d::combine_kernel<NT>, dim3(grid), dim3(32 * fp4d::kCols<NT>), 0, stream, p));
   NVC_CUDA_CHECK(ctx, cudaGetLastError());
   ctx->launches += 2;
@@ -70,8 +70,8 @@ int attn_fp4(nvc_ctx* ctx, const nvc_bf16* q, int ldq, const nvc_fp4_cache* cach
 }  // namespace
 
 extern "C" int nvc_fp4_attn_init(nvc_ctx* ctx) {
-  NVC_CUDA_CHECK(ctx, cudaFuncSetAttribute(fp4d::attn_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, fp4d::kSmem<1>));
-  NVC_CUDA_CHECK(ctx, cudaFuncSetAttribute(fp4d::attn_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, fp4d::kSmem<2>));
+  for (auto kernel : {fp4d::attn_kernel<1, false>, fp4d::attn_kernel<1, true>}) NVC_CUDA_CHECK(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, fp4d::kSmem<1>));
+  for (auto kernel : {fp4d::attn_kernel<2, false>, fp4d::attn_kernel<2, true>}) NVC_CUDA_CHECK(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, fp4d::kSmem<2>));
   NVC_CUDA_CHECK(ctx, cudaFuncSetAttribute(fp4p::attn_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, fp4p::kSmemBytes));
   return NVC_OK;
 }
