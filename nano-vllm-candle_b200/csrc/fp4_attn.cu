@@ -17,16 +17,19 @@ template <int NT> int64_t parts_bytes(const nvc_ctx* ctx) { return (int64_t)ctx-
 template <int NT>
 int launch_few(nvc_ctx* ctx, fp4d::Args& p, int64_t most_rows, cudaStream_t stream, size_t workspace_bytes) {
   const int64_t units = p.kv * ((most_rows + fp4d::kCols<NT> - 1) / fp4d::kCols<NT>);          // of a sequence, at most
-  const int64_t most = units * p.B * (((int64_t)p.bt_stride * p.block_size + fp4d::kTile - 1) / fp4d::kTile + fp4d::kUnitCost);      // the list's length, at most
+  const int64_t tiles = ((int64_t)p.bt_stride * p.block_size + fp4d::kTile - 1) / fp4d::kTile;        // of a sequence, at most
+  const bool alone = !p.cu_seqlens && fp4d::alone<NT>(ctx->num_sms, units * p.B, tiles);
+  const int64_t most = units * p.B * (tiles + fp4d::kUnitCost);      // the list's length, at most
   const int64_t a_cta = (1 + fp4d::kUnitCost) * fp4d::kWarps;
-  const int grid = (int)std::min<int64_t>((int64_t)ctx->num_sms * fp4d::kCtas<NT>, (most + a_cta - 1) / a_cta);
+  const int grid = alone ? (int)(units * p.B) : (int)std::min<int64_t>((int64_t)ctx->num_sms * fp4d::kCtas<NT>, (most + a_cta - 1) / a_cta);
   NVC_REQUIRE(ctx, p.notes && ((uintptr_t)p.notes & 15) == 0 && workspace_bytes >= (size_t)parts_bytes<NT>(ctx), NVC_ENOMEM, "workspace too small");
   p.parts = reinterpret_cast<float*>(p.notes + grid);
   p.warps = grid * fp4d::kWarps;
+  p.alone = alone ? (int)units : 0;
   NVC_CUDA_CHECK(ctx, nvc_launch(ctx, p.cu_seqlens ? fp4d::attn_kernel<NT, true> : fp4d::attn_kernel<NT, false>, dim3(grid), dim3(32 * fp4d::kWarps), (size_t)fp4d::kSmem<NT>, stream, p));
-  NVC_CUDA_CHECK(ctx, nvc_launch(ctx, fp4d::combine_kernel<NT>, dim3(grid), dim3(32 * fp4d::kCols<NT>), 0, stream, p));
+  if (!alone) NVC_CUDA_CHECK(ctx, nvc_launch(ctx, fp4d::combine_kernel<NT>, dim3(grid), dim3(32 * fp4d::kCols<NT>), 0, stream, p));
   NVC_CUDA_CHECK(ctx, cudaGetLastError());
-  ctx->launches += 2;
+  ctx->launches += alone ? 1 : 2;
   return NVC_OK;
 }
 
@@ -61,7 +64,7 @@ int attn_fp4(nvc_ctx* ctx, const nvc_bf16* q, int ldq, const nvc_fp4_cache* cach
   const int64_t most_rows = most_rows_of(rows, max_qlen, group);             // of a sequence and key head
   NVC_REQUIRE(ctx, (int64_t)rows * group <= 0x7fffffffLL, NVC_ESHAPE, "too many rows");
   fp4d::Args p{q, out, ldq, ldo, cache->k, cache->k_scale, cache->v, cache->v_scale, block_tables, context_lens, cu_seqlens_q, bt_stride, cache->num_blocks, cache->kv,
-               cache->block_size, B, group, rows, scale * 1.4426950408889634f, static_cast<int4*>(workspace), nullptr, 0};
+               cache->block_size, B, group, rows, scale * 1.4426950408889634f, static_cast<int4*>(workspace), nullptr, 0, 0};
   DeviceGuard guard(ctx->device);
   if (cu_seqlens_q && most_rows > kFewRows) return launch_many(ctx, p, scale, nvc_stream(stream), workspace_bytes);
   return most_rows <= 8 ? launch_few<1>(ctx, p, most_rows, nvc_stream(stream), workspace_bytes) : launch_few<2>(ctx, p, most_rows, nvc_stream(stream), workspace_bytes);

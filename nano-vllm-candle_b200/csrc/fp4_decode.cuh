@@ -43,10 +43,15 @@ struct Args {
   int4* notes;                                                         // of each CTA, what begins there and ends in another: sequence (-1: nothing), unit, last CTA
   float* parts;                                                        // two records of each CTA
   int warps;                                                           // of the attention kernel's grid
+  int alone;                                                           // > 0: units of a sequence, each in a CTA of its own (no list, no joining kernel)
 };
 
 // CTAs of an SM.  16 columns: 229 registers, of 168 (three CTAs) some go to memory: 256 contexts of 2 000, us: 186 / 172, 32 of 1 750 37 / 31.  8 columns: 4 and 3 CTAs alike
 template <int NT> constexpr int kCtas = NT == 1 ? 4 : 2;
+// Decode of short contexts: a CTA for each unit, which needs neither the list nor the joining kernel, where all units run at once and the longest that the tables have room for would not hold up the
+// others for long.  In us, with the list / without (caches cold; 16 heads to 8): 1 x 128 10.3 / 6.2, 1 x 512 10.3 / 8.3, 1 x 1 024 11.1 / 12.3, 37 x 256 14.3 / 9.2, 37 x 1 024 22.5 / 16.4; of
+// lengths from 1 on, a call behind the other, 74 x 1 024 18.9 / 18.2, 74 x 1 536 22.8 / 24.6; in more than one wave 112 x 1 024 40.6 / 43.0
+template <int NT> bool alone(int sms, int64_t units, int64_t tiles) { return units <= (int64_t)sms * kCtas<NT> && tiles <= std::min<int64_t>(32, 24 + units / 12); }
 constexpr int kRing = 2;                                               // tiles of a warp's ring (three and four: no difference)
 constexpr int kRingBytes = kRing * kStageBytes;
 template <int NT> constexpr int kCols = 8 * NT;
@@ -228,12 +233,28 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<NT>) attn_kernel(const Args
     ptx::fence_barrier_init();
   }
   __syncwarp();
-  const List list = list_of<NT>(p, lane);
-  const int per = max((int)divide(list.total + p.warps - 1, p.warps), 1 + kUnitCost);          // (a stretch of 2^31 tiles would be 10 TB of cache)
+  const bool alone = !kPortions && p.alone > 0;
+  int per = 0;
+  bool any, idle;                                     // this warp has tiles; the CTA has none
+  Piece at;
   uint8_t* const mine = smem + warp * kWarpBytes<NT>;
   const uint32_t ring = smem_u32(mine);
-  Piece at;
-  bool any = first_piece<NT>(p, list, (int64_t)per * (blockIdx.x * kWarps + warp), per, lane, at);
+  if (alone) {                                        // the unit's tiles, shared by the CTA's warps
+    at.b = blockIdx.x / p.alone;
+    at.u = blockIdx.x - at.b * p.alone;
+    at.s = seq_of<NT>(p, at.b);
+    const int share = (at.s.tiles + kWarps - 1) / kWarps;
+    at.t = min(warp * share, at.s.tiles);
+    at.end = min(at.t + share, at.s.tiles);
+    at.rest = 0;                                      // no piece behind it
+    any = at.t < at.end;
+    idle = at.s.tiles == 0;
+  } else {
+    const List list = list_of<NT>(p, lane);
+    per = max((int)divide(list.total + p.warps - 1, p.warps), 1 + kUnitCost);          // (a stretch of 2^31 tiles would be 10 TB of cache)
+    any = first_piece<NT>(p, list, (int64_t)per * (blockIdx.x * kWarps + warp), per, lane, at);
+    idle = (int64_t)per * (blockIdx.x * kWarps) >= list.total;
+  }
 
   // ---- the reading side: ahead by what the ring holds.  Lane 0 copies; the others know which rows are not there
   const int per_page = p.block_size / kHalf, last_page = p.bt_stride - 1;
@@ -268,8 +289,8 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<NT>) attn_kernel(const Args
           for (int c = lane; c < p.kv * p.group * 16; c += 32) reinterpret_cast<uint4*>(p.out + row * p.ldo)[c] = make_uint4(0, 0, 0, 0);
       }
   }
-  if ((int64_t)per * (blockIdx.x * kWarps) >= list.total) {      // the whole CTA
-    if (threadIdx.x == 0) p.notes[blockIdx.x] = make_int4(-1, 0, 0, 0);
+  if (idle) {
+    if (threadIdx.x == 0 && !alone) p.notes[blockIdx.x] = make_int4(-1, 0, 0, 0);
     return;
   }
 
@@ -681,7 +702,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<NT>) attn_kernel(const Args
     }
     i = last + 1;
   }
-  if (threadIdx.x == 0) p.notes[blockIdx.x] = note;
+  if (threadIdx.x == 0 && !alone) p.notes[blockIdx.x] = note;
 }
 
 // Units that lie in several CTAs, by the CTA in which they begin; a warp per column.

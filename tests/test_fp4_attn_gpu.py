@@ -301,3 +301,25 @@ def test_portions_of_a_bound_that_is_too_low(ctx):
     c = _many(seed=30)
     got = ops.prefill_attn_paged_fp4(ctx, c["q"], c["cache"], c["tables"], c["lens"], c["cu"], 2, 8, 128 ** -0.5)
     _near(got, c)
+
+
+def _room(c, tokens=4096):
+    """The same tables with room for more pages: decode of contexts that could be long shares its work in another way."""
+    more = -(-tokens // c["cache"].block_size)
+    return dict(c, tables=torch.cat((c["tables"], torch.full((len(c["new"]), more), -1, dtype=I32, device=DEV)), 1))
+
+
+@pytest.mark.parametrize("lens,nh,kv,bs", [
+    ([1], 1, 1, 16), ([17], 8, 8, 16), ([255, 256, 257], 16, 8, 256), ([1, 0, 33, 700], 32, 8, 48), ([5, 64, 63, 65, 0, 0, 129], 40, 8, 32), ([90], 12, 1, 16), ([300, 31], 16, 1, 256),
+    ([70, 200], 24, 1, 16), ([100] * 37, 4, 4, 16), ([0, 0], 8, 2, 16), ([50, 0, 3], 96, 4, 16), ([700, 1, 0, 128], 5, 1, 16)])
+def test_decode_with_room_for_more(ctx, lens, nh, kv, bs):
+    c = _case(lens, nh, kv, bs, seed=21)
+    for d in (c, _room(c, 600), _room(c)):
+        _near(_decode(ctx, d), d)
+    for blk in c["tables"][:, 0].tolist():                              # a NaN in each context's first row: its key head's rows, and no other's, whichever way
+        if blk >= 0:
+            c["cache"].v_scale[blk, 0, 0] = 255
+    group, bad = nh // kv, torch.tensor([n > 0 for n in lens], device=DEV)
+    for d in (c, _room(c)):
+        got = _decode(ctx, d).view(len(lens), nh, 128)
+        assert torch.isnan(got[bad, :group]).all() and torch.isfinite(got[bad, group:]).all() and not got[~bad].any()
