@@ -37,16 +37,20 @@ constexpr int kFewRows = 64;          // of a key head: up to here the kernel fo
 int64_t most_rows_of(int rows, int max_qlen, int group) { return std::min(rows, max_qlen) * (int64_t)group; }
 size_t many_bytes(const nvc_ctx* ctx) { return (size_t)ctx->num_sms * (16 + 2 * fp4p::kRecord * 4); }
 
-int launch_many(nvc_ctx* ctx, const fp4d::Args& f, float scale, cudaStream_t stream, size_t workspace_bytes) {
+int launch_many(nvc_ctx* ctx, const fp4d::Args& f, int64_t most_rows, float scale, cudaStream_t stream, size_t workspace_bytes) {
   NVC_REQUIRE(ctx, f.notes && ((uintptr_t)f.notes & 15) == 0 && workspace_bytes >= many_bytes(ctx), NVC_ENOMEM, "workspace too small");
-  const int grid = ctx->num_sms;
+  // A unit for each CTA where all of them run at once, by max_seqlen_q; the grid has room for whatever cu_seqlens say
+  const int64_t room = f.kv * ((int64_t)f.rows * f.group / fp4p::kRows + f.B), tiles = ((int64_t)f.bt_stride * f.block_size + fp4p::kKT - 1) / fp4p::kKT;          // units at most; tiles of one
+  const int64_t units = std::min(room, f.kv * (int64_t)f.B * ((most_rows + fp4p::kRows - 1) / fp4p::kRows));
+  const bool alone = units <= ctx->num_sms && tiles <= fp4p::kAloneTiles;
+  const int grid = alone ? (int)room : ctx->num_sms;
   const fp4p::Args p{f.q, f.out, f.ldq, f.ldo, f.kc, f.ks, f.vc, f.vs, f.block_tables, f.context_lens, f.cu_seqlens, f.bt_stride, f.num_blocks, f.kv, f.block_size, f.B, f.group,
                      f.rows, fp4p::make_div(f.group), fp4p::make_div(f.block_size), scale > 0.f ? 1.f : scale < 0.f ? -1.f : 0.f,
-                     scale == 0.f ? 1.f : std::fabs(scale) * 1.4426950408889634f, f.notes, reinterpret_cast<float*>(f.notes + grid)};
+                     scale == 0.f ? 1.f : std::fabs(scale) * 1.4426950408889634f, f.notes, reinterpret_cast<float*>(f.notes + grid), alone};
   NVC_CUDA_CHECK(ctx, nvc_launch(ctx, fp4p::attn_kernel, dim3(grid), dim3(fp4p::kThreads), (size_t)fp4p::kSmemBytes, stream, p));
-  NVC_CUDA_CHECK(ctx, nvc_launch(ctx, fp4p::combine_kernel, dim3(grid * 8), dim3(256), 0, stream, p));
+  if (!alone) NVC_CUDA_CHECK(ctx, nvc_launch(ctx, fp4p::combine_kernel, dim3(grid * 8), dim3(256), 0, stream, p));
   NVC_CUDA_CHECK(ctx, cudaGetLastError());
-  ctx->launches += 2;
+  ctx->launches += alone ? 1 : 2;
   return NVC_OK;
 }
 
@@ -66,7 +70,7 @@ int attn_fp4(nvc_ctx* ctx, const nvc_bf16* q, int ldq, const nvc_fp4_cache* cach
   fp4d::Args p{q, out, ldq, ldo, cache->k, cache->k_scale, cache->v, cache->v_scale, block_tables, context_lens, cu_seqlens_q, bt_stride, cache->num_blocks, cache->kv,
                cache->block_size, B, group, rows, scale * 1.4426950408889634f, static_cast<int4*>(workspace), nullptr, 0, 0};
   DeviceGuard guard(ctx->device);
-  if (cu_seqlens_q && most_rows > kFewRows) return launch_many(ctx, p, scale, nvc_stream(stream), workspace_bytes);
+  if (cu_seqlens_q && most_rows > kFewRows) return launch_many(ctx, p, most_rows, scale, nvc_stream(stream), workspace_bytes);
   return most_rows <= 8 ? launch_few<1>(ctx, p, most_rows, nvc_stream(stream), workspace_bytes) : launch_few<2>(ctx, p, most_rows, nvc_stream(stream), workspace_bytes);
 }
 

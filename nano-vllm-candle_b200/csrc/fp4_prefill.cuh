@@ -28,6 +28,9 @@ constexpr int kOffBar = kOffPark + 8 * 96 + 16;
 constexpr int kNumBars = 18;
 constexpr int kSmemBytes = kOffBar + kNumBars * 8 + 16 + 1024;          // and room to begin at a multiple of 1024
 constexpr int kUnitCost = 5;                               // a unit's queries and result, in tiles (a prompt of 8 191 in us: 4 470, 5 438, 6 439, 9 451)
+// Where the tables have room for no more, and all units run at once, each has a CTA (in us, stretches and joining / a CTA for each, caches cold, 16 heads to 8: 1 x 100 tokens 22.4 / 12.2, 333 24.6 / 16.3,
+// 1 024 30.7 / 25.0, 64 behind 1 000 27.1 / 24.9, behind 2 000 28.9 / 38.9; 32 to 2, 64 behind 1 000 25.9 / 26.6)
+constexpr int kAloneTiles = 9;
 constexpr float kFloor = -1.0e30f, kShift = 7.0f, kGrow = 8.0f;
 constexpr int kRecord = kRows * 130;                       // floats: O [32 groups of 4 dims][256 rows][4], reference [256], sum [256]
 constexpr int kChunk = 2048;                               // sequences whose weights are looked at together (in shared memory)
@@ -55,6 +58,7 @@ struct Args {
   float q_sign, factor;                                    // -1, 0 or 1; what scores are multiplied with (positive)
   int4* notes;                                             // of each CTA, the unit that begins there and ends in another: sequence (-1: none), 256 rows' number, key head, last CTA
   float* parts;                                            // two records of each CTA
+  bool alone;                                              // a unit for each CTA (no joining kernel)
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -165,10 +169,11 @@ __device__ __forceinline__ int64_t sum64(int64_t x) {
 __device__ __forceinline__ bool plan(const Args& p, int64_t* weights, int warp, int lane, Piece& x, int& per, int64_t& total) {
   constexpr int kW = kThreads / 32;
   __shared__ int64_t sums[kW];
+  auto cost_of = [&](int j, const Seq& s) { return p.alone ? 1 : tiles_of(p, s, j) + kUnitCost; };
   auto weigh = [&](int b) {                                // a sequence's weight, of a whole warp
     const Seq s = seq_of(p, b);
     int64_t mine = 0;
-    for (int j = lane; j < s.blocks; j += 32) mine += tiles_of(p, s, j) + kUnitCost;
+    for (int j = lane; j < s.blocks; j += 32) mine += cost_of(j, s);
     return sum64(mine) * p.kv;
   };
   int64_t mine = 0;
@@ -182,7 +187,7 @@ __device__ __forceinline__ bool plan(const Args& p, int64_t* weights, int warp, 
   total = 0;
 #pragma unroll
   for (int i = 0; i < kW; ++i) total += sums[i];
-  per = max((int)((total + gridDim.x - 1) / gridDim.x), 2 + kUnitCost);
+  per = p.alone ? 1 : max((int)((total + gridDim.x - 1) / gridDim.x), 2 + kUnitCost);
   int64_t at = (int64_t)per * blockIdx.x;
   if (at >= total) return false;
   int b0 = 0;
@@ -219,7 +224,7 @@ __device__ __forceinline__ bool plan(const Args& p, int64_t* weights, int warp, 
   }
   x.s = seq_of(p, x.b);
   for (int j0 = 0;; j0 += 32) {                            // within the sequence: 256 rows after 256 rows
-    const int64_t w = j0 + lane < x.s.blocks ? (int64_t)(tiles_of(p, x.s, j0 + lane) + kUnitCost) * p.kv : 0;
+    const int64_t w = j0 + lane < x.s.blocks ? (int64_t)cost_of(j0 + lane, x.s) * p.kv : 0;
     int64_t upto = w;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -236,6 +241,12 @@ __device__ __forceinline__ bool plan(const Args& p, int64_t* weights, int warp, 
     at -= __shfl_sync(0xffffffffu, upto, 31);
   }
   x.tiles = tiles_of(p, x.s, x.j);
+  if (p.alone) {
+    x.h = (int)at;
+    x.t = x.rest = 0;                                      // all of it, and nothing behind it
+    x.end = x.tiles;
+    return true;
+  }
   const int unit = x.tiles + kUnitCost;
   x.h = (int)((uint32_t)at / (uint32_t)unit);              // a unit's heads: below 2^32 in all
   const int into = (int)at - x.h * unit;

@@ -323,3 +323,19 @@ def test_decode_with_room_for_more(ctx, lens, nh, kv, bs):
     for d in (c, _room(c)):
         got = _decode(ctx, d).view(len(lens), nh, 128)
         assert torch.isnan(got[bad, :group]).all() and torch.isfinite(got[bad, group:]).all() and not got[~bad].any()
+
+
+@pytest.mark.parametrize("new,before,nh,kv,bs", [
+    ([128], [0], 4, 2, 32), ([129, 1, 64], [31, 700, 0], 16, 4, 16), ([70], [333], 40, 8, 16), ([64, 0, 65], [0, 9, 1], 8, 1, 16), ([300, 2, 0, 90], [0, 100, 0, 800], 8, 8, 48),
+    ([100] * 20, [0] * 20, 32, 8, 16), ([65] * 3, [1000, 0, 512], 24, 1, 128)])
+def test_portions_with_room_for_more(ctx, new, before, nh, kv, bs):
+    """Short portions in one way, and, with tables that have room for long ones, in the other; a bound of their length that is too low included."""
+    c = _case([n + b for n, b in zip(new, before)], nh, kv, bs, new=new, seed=23)
+    for d in (c, _room(c)):
+        _near(_portions(ctx, d), d)
+        _near(ops.prefill_attn_paged_fp4(ctx, d["q"], d["cache"], d["tables"], d["lens"], d["cu"], 64, nh, 128 ** -0.5), d)
+    c["cache"].v_scale[int(c["tables"][0, 0]), 0, 0, 0] = 255              # the first context's first row: every row of its key head
+    group = nh // kv
+    for d in (c, _room(c)):
+        got = _portions(ctx, d).view(-1, nh, 128)
+        assert torch.isnan(got[:new[0], :group, :16]).all() and torch.isfinite(got[:new[0], :group, 16:]).all() and torch.isfinite(got[:new[0], group:]).all() and torch.isfinite(got[new[0]:]).all()
