@@ -14,14 +14,18 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 template <int NT> int64_t parts_bytes(const nvc_ctx* ctx) { return (int64_t)ctx->num_sms * fp4d::kCtas<NT> * (16 + 2 * fp4d::kRecord<NT> * 4); }
 
+constexpr int kMostAlone = 65535;          // CTAs
+
 template <int NT>
 int launch_few(nvc_ctx* ctx, fp4d::Args& p, int64_t most_rows, cudaStream_t stream, size_t workspace_bytes) {
   const int64_t units = p.kv * ((most_rows + fp4d::kCols<NT> - 1) / fp4d::kCols<NT>);          // of a sequence, at most
   const int64_t tiles = ((int64_t)p.bt_stride * p.block_size + fp4d::kTile - 1) / fp4d::kTile;        // of a sequence, at most
-  const bool alone = !p.cu_seqlens && fp4d::alone<NT>(ctx->num_sms, units * p.B, tiles);
+  // units at most by max_seqlen_q, and whatever cu_seqlens say
+  const int64_t room = p.cu_seqlens ? p.kv * ((int64_t)p.rows * p.group / fp4d::kCols<NT> + p.B) : units * p.B;
+  const bool alone = fp4d::alone<NT>(ctx->num_sms, std::min(units * p.B, room), tiles) && room <= kMostAlone;
   const int64_t most = units * p.B * (tiles + fp4d::kUnitCost);      // the list's length, at most
   const int64_t a_cta = (1 + fp4d::kUnitCost) * fp4d::kWarps;
-  const int grid = alone ? (int)(units * p.B) : (int)std::min<int64_t>((int64_t)ctx->num_sms * fp4d::kCtas<NT>, (most + a_cta - 1) / a_cta);
+  const int grid = alone ? (int)room : (int)std::min<int64_t>((int64_t)ctx->num_sms * fp4d::kCtas<NT>, (most + a_cta - 1) / a_cta);
   NVC_REQUIRE(ctx, p.notes && ((uintptr_t)p.notes & 15) == 0 && workspace_bytes >= (size_t)parts_bytes<NT>(ctx), NVC_ENOMEM, "workspace too small");
   p.parts = reinterpret_cast<float*>(p.notes + grid);
   p.warps = grid * fp4d::kWarps;
@@ -42,7 +46,7 @@ int launch_many(nvc_ctx* ctx, const fp4d::Args& f, int64_t most_rows, float scal
   // A unit for each CTA where all of them run at once, by max_seqlen_q; the grid has room for whatever cu_seqlens say
   const int64_t room = f.kv * ((int64_t)f.rows * f.group / fp4p::kRows + f.B), tiles = ((int64_t)f.bt_stride * f.block_size + fp4p::kKT - 1) / fp4p::kKT;          // units at most; tiles of one
   const int64_t units = std::min(room, f.kv * (int64_t)f.B * ((most_rows + fp4p::kRows - 1) / fp4p::kRows));
-  const bool alone = units <= ctx->num_sms && tiles <= fp4p::kAloneTiles;
+  const bool alone = units <= ctx->num_sms && room <= kMostAlone && tiles <= fp4p::kAloneTiles;
   const int grid = alone ? (int)room : ctx->num_sms;
   const fp4p::Args p{f.q, f.out, f.ldq, f.ldo, f.kc, f.ks, f.vc, f.vs, f.block_tables, f.context_lens, f.cu_seqlens, f.bt_stride, f.num_blocks, f.kv, f.block_size, f.B, f.group,
                      f.rows, fp4p::make_div(f.group), fp4p::make_div(f.block_size), scale > 0.f ? 1.f : scale < 0.f ? -1.f : 0.f,

@@ -43,7 +43,7 @@ struct Args {
   int4* notes;                                                         // of each CTA, what begins there and ends in another: sequence (-1: nothing), unit, last CTA
   float* parts;                                                        // two records of each CTA
   int warps;                                                           // of the attention kernel's grid
-  int alone;                                                           // > 0: units of a sequence, each in a CTA of its own (no list, no joining kernel)
+  int alone;                                                           // > 0: each unit in a CTA of its own (no joining kernel); in decode, units of a sequence
 };
 
 // CTAs of an SM.  16 columns: 229 registers, of 168 (three CTAs) some go to memory: 256 contexts of 2 000, us: 186 / 172, 32 of 1 750 37 / 31.  8 columns: 4 and 3 CTAs alike
@@ -130,7 +130,7 @@ __device__ __forceinline__ Seq seq_of(const Args& p, int b) {
   s.units = p.kv * ((s.qlen * p.group + kCols<NT> - 1) / kCols<NT>);
   return s;
 }
-__device__ __forceinline__ int64_t weight(const Seq& s) { return s.tiles ? (int64_t)s.units * (s.tiles + kUnitCost) : 0; }
+__device__ __forceinline__ int64_t weight(const Seq& s, bool alone = false) { return s.tiles ? (int64_t)s.units * (alone ? 1 : s.tiles + kUnitCost) : 0; }
 // n / d; the short division where the numbers allow it
 __device__ __forceinline__ int64_t divide(int64_t n, int64_t d) {
   return (uint64_t)(n | d) >> 32 ? n / d : (int64_t)((uint32_t)n / (uint32_t)d);
@@ -139,7 +139,7 @@ __device__ __forceinline__ int64_t divide(int64_t n, int64_t d) {
 // The list, summed: a lane has the sequences [lane * m, lane * m + m)
 struct List { int m; int64_t upto, total; };            // upto: this lane's last sequence included
 template <int NT>
-__device__ __forceinline__ List list_of(const Args& p, int lane) {
+__device__ __forceinline__ List list_of(const Args& p, int lane, bool alone = false) {
   List x;
   x.m = (p.B + 31) / 32;
   x.upto = 0;
@@ -147,7 +147,7 @@ __device__ __forceinline__ List list_of(const Args& p, int lane) {
   for (int i = 0; i < x.m; ++i) {
     const int b = lane * x.m + i;
     const Seq s = seq_of<NT>(p, min(b, p.B - 1));
-    x.upto += b < p.B ? weight(s) : 0;
+    x.upto += b < p.B ? weight(s, alone) : 0;
   }
 #pragma unroll
   for (int w = 1; w < 32; w <<= 1) {
@@ -168,18 +168,23 @@ struct Piece {
     return end > t;
   }
 };
+// place `at` of the list: its sequence, and what is left of `at` in it
 template <int NT>
-__device__ __forceinline__ bool first_piece(const Args& p, const List& list, int64_t at, int per, int lane, Piece& x) {
-  if (at >= list.total) return false;
+__device__ __forceinline__ void find(const Args& p, const List& list, int64_t& at, Piece& x, bool alone = false) {
   const int f = __ffs(__ballot_sync(0xffffffffu, list.upto > at)) - 1;
   const int64_t before = __shfl_sync(0xffffffffu, list.upto, max(f - 1, 0));
   at -= f ? before : 0;
   for (x.b = f * list.m;; ++x.b) {
     x.s = seq_of<NT>(p, x.b);
-    const int64_t w = weight(x.s);
+    const int64_t w = weight(x.s, alone);
     if (at < w) break;
     at -= w;
   }
+}
+template <int NT>
+__device__ __forceinline__ bool first_piece(const Args& p, const List& list, int64_t at, int per, Piece& x) {
+  if (at >= list.total) return false;
+  find<NT>(p, list, at, x);
   const int unit = x.s.tiles + kUnitCost;
   x.u = (int)divide(at, unit);
   const int into = (int)(at - (int64_t)x.u * unit);
@@ -233,26 +238,34 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<NT>) attn_kernel(const Args
     ptx::fence_barrier_init();
   }
   __syncwarp();
-  const bool alone = !kPortions && p.alone > 0;
+  const bool alone = p.alone > 0;
   int per = 0;
-  bool any, idle;                                     // this warp has tiles; the CTA has none
-  Piece at;
+  bool any, idle = false;                             // this warp has tiles; the CTA has none
+  Piece at{};
   uint8_t* const mine = smem + warp * kWarpBytes<NT>;
   const uint32_t ring = smem_u32(mine);
-  if (alone) {                                        // the unit's tiles, shared by the CTA's warps
-    at.b = blockIdx.x / p.alone;
-    at.u = blockIdx.x - at.b * p.alone;
-    at.s = seq_of<NT>(p, at.b);
+  if (alone) {                                        // a unit's tiles, shared by the CTA's warps
+    if constexpr (kPortions) {
+      const List list = list_of<NT>(p, lane, true);
+      int64_t place = blockIdx.x;
+      idle = place >= list.total;
+      if (!idle) find<NT>(p, list, place, at, true);
+      at.u = (int)place;
+    } else {
+      at.b = blockIdx.x / p.alone;
+      at.u = blockIdx.x - at.b * p.alone;
+      at.s = seq_of<NT>(p, at.b);
+      idle = at.s.tiles == 0;
+    }
     const int share = (at.s.tiles + kWarps - 1) / kWarps;
     at.t = min(warp * share, at.s.tiles);
     at.end = min(at.t + share, at.s.tiles);
     at.rest = 0;                                      // no piece behind it
-    any = at.t < at.end;
-    idle = at.s.tiles == 0;
+    any = !idle && at.t < at.end;
   } else {
     const List list = list_of<NT>(p, lane);
     per = max((int)divide(list.total + p.warps - 1, p.warps), 1 + kUnitCost);          // (a stretch of 2^31 tiles would be 10 TB of cache)
-    any = first_piece<NT>(p, list, (int64_t)per * (blockIdx.x * kWarps + warp), per, lane, at);
+    any = first_piece<NT>(p, list, (int64_t)per * (blockIdx.x * kWarps + warp), per, at);
     idle = (int64_t)per * (blockIdx.x * kWarps) >= list.total;
   }
 

@@ -339,3 +339,17 @@ def test_portions_with_room_for_more(ctx, new, before, nh, kv, bs):
     for d in (c, _room(c)):
         got = _portions(ctx, d).view(-1, nh, 128)
         assert torch.isnan(got[:new[0], :group, :16]).all() and torch.isfinite(got[:new[0], :group, 16:]).all() and torch.isfinite(got[:new[0], group:]).all() and torch.isfinite(got[new[0]:]).all()
+
+
+@pytest.mark.parametrize("new,before,nh,kv,bs", [
+    ([1], [0], 4, 2, 16), ([5], [0], 8, 8, 16), ([3, 1, 8], [0, 40, 500], 32, 8, 256), ([17, 2], [1, 200], 8, 1, 48), ([1] * 40, list(range(0, 200, 5)), 8, 8, 16), ([33], [64], 4, 1, 64),
+    ([2, 0, 3, 0], [0, 9, 100, 700], 12, 2, 16), ([4] * 30, [90] * 30, 32, 4, 32)])
+def test_portions_of_few_rows_with_room_for_more(ctx, new, before, nh, kv, bs):
+    c = _case([n + b for n, b in zip(new, before)], nh, kv, bs, new=new, seed=24)
+    for d in (c, _room(c)):
+        _near(_portions(ctx, d), d)
+        _near(ops.prefill_attn_paged_fp4(ctx, d["q"], d["cache"], d["tables"], d["lens"], d["cu"], 1, nh, 128 ** -0.5), d)
+    c["lens"][0] = 0                                                       # a context of nothing: zeros
+    for d in (c, _room(c)):
+        got = _portions(ctx, d)
+        assert not got[:new[0]].any() and torch.isfinite(got).all()
