@@ -60,3 +60,15 @@ __device__ __forceinline__ uint4 fp4_halves8(uint32_t codes) {
   return r;
 }
 #endif
+// n / d for n < 2^31 and a d of the host's: d's inverse, rounded up, with as many bits as that takes
+struct Fp4Div {
+  unsigned long long mul;
+  int shift;
+  __device__ __forceinline__ int operator()(int n) const { return (int)((unsigned long long)(unsigned)n * mul >> shift); }
+};
+inline Fp4Div fp4_div(int d) {
+  int s = 0;
+  while ((1ll << s) < d) ++s;
+  return Fp4Div{((1ull << (32 + s)) + (unsigned long long)d - 1) / (unsigned long long)d, 32 + s};
+}
+

@@ -49,7 +49,7 @@ int launch_many(nvc_ctx* ctx, const fp4d::Args& f, int64_t most_rows, float scal
   const bool alone = units <= ctx->num_sms && room <= kMostAlone && tiles <= fp4p::kAloneTiles;
   const int grid = alone ? (int)room : ctx->num_sms;
   const fp4p::Args p{f.q, f.out, f.ldq, f.ldo, f.kc, f.ks, f.vc, f.vs, f.block_tables, f.context_lens, f.cu_seqlens, f.bt_stride, f.num_blocks, f.kv, f.block_size, f.B, f.group,
-                     f.rows, fp4p::make_div(f.group), fp4p::make_div(f.block_size), scale > 0.f ? 1.f : scale < 0.f ? -1.f : 0.f,
+                     f.rows, fp4_div(f.group), fp4_div(f.block_size), scale > 0.f ? 1.f : scale < 0.f ? -1.f : 0.f,
                      scale == 0.f ? 1.f : std::fabs(scale) * 1.4426950408889634f, f.notes, reinterpret_cast<float*>(f.notes + grid), alone};
   NVC_CUDA_CHECK(ctx, nvc_launch(ctx, fp4p::attn_kernel, dim3(grid), dim3(fp4p::kThreads), (size_t)fp4p::kSmemBytes, stream, p));
   if (!alone) NVC_CUDA_CHECK(ctx, nvc_launch(ctx, fp4p::combine_kernel, dim3(grid * 8), dim3(256), 0, stream, p));

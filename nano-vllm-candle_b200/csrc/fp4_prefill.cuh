@@ -35,18 +35,6 @@ constexpr float kFloor = -1.0e30f, kShift = 7.0f, kGrow = 8.0f;
 constexpr int kRecord = kRows * 130;                       // floats: O [32 groups of 4 dims][256 rows][4], reference [256], sum [256]
 constexpr int kChunk = 2048;                               // sequences whose weights are looked at together (in shared memory)
 
-// n / d for n < 2^31 and a d of the host's: d's inverse, rounded up, with as many bits as that takes
-struct Div {
-  unsigned long long mul;
-  int shift;
-  __device__ __forceinline__ int operator()(int n) const { return (int)((unsigned long long)(unsigned)n * mul >> shift); }
-};
-inline Div make_div(int d) {
-  int s = 0;
-  while ((1ll << s) < d) ++s;
-  return Div{((1ull << (32 + s)) + (unsigned long long)d - 1) / (unsigned long long)d, 32 + s};
-}
-
 struct Args {
   const nvc_bf16* q;
   nvc_bf16* out;
@@ -54,7 +42,7 @@ struct Args {
   const uint8_t *kc, *ks, *vc, *vs;
   const int32_t *block_tables, *context_lens, *cu_seqlens;
   int bt_stride, num_blocks, kv, block_size, B, group, rows;
-  Div by_group, by_block;
+  Fp4Div by_group, by_block;
   float q_sign, factor;                                    // -1, 0 or 1; what scores are multiplied with (positive)
   int4* notes;                                             // of each CTA, the unit that begins there and ends in another: sequence (-1: none), 256 rows' number, key head, last CTA
   float* parts;                                            // two records of each CTA
