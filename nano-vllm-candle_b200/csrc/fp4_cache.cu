@@ -27,7 +27,8 @@ struct StoreArgs {
 // neighbouring lanes'.  A warp takes `span` fours of one token's heads (fours of q heads, then of k, then of v heads), so that the token's angles and slot and the norms' weights are read once for
 // them.  Per token (nh + 2 kv) * 256 bytes in, nh * 256 (and kv * 256 in place) + kv * 144 out.  Kinds of heads in loops of their own: with one loop for all, the instructions were what bound it (370 a
 // four, 95 us for 16 000 tokens of 32 + 16 heads).
-__global__ void __launch_bounds__(128, 5) store_fp4_kernel(const StoreArgs p, int span, int warps_per_token) {
+constexpr int kStoreCtas = 5;           // of an SM
+__global__ void __launch_bounds__(128, kStoreCtas) store_fp4_kernel(const StoreArgs p, int span, int warps_per_token) {
   pdl_trigger();
   const int64_t warp = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31, l = lane & 7, sub = lane >> 3;
@@ -146,10 +147,11 @@ read_fp4_kernel(const uint8_t* kc, const uint8_t* ks, const uint8_t* vc, const u
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 int launch_store(nvc_ctx* ctx, const StoreArgs& p, void* stream) {
-  // few tokens: their heads over many warps; many: all heads of a token in one
+  // few tokens: their heads over many warps, as long as all run at once; many: all heads of a token in one (2 048 tokens of 32 + 16 heads, us: 12 fours a warp 14.5, 6 16.4, 4 18.4; 1 024: 12.3, 10.2,
+  // 12.2; 512: 12.3, 8.3, 8.1, and 3 6.8)
   const int fours = (p.nh + 3) / 4 + 2 * ((p.kv + 3) / 4);
-  const int64_t room = (int64_t)ctx->num_sms * 32;
-  const int span = (int)std::min<int64_t>(fours, std::max<int64_t>(1, (int64_t)p.N * fours / room)), per_token = (fours + span - 1) / span;
+  const int64_t room = (int64_t)ctx->num_sms * 4 * kStoreCtas;
+  const int most = (int)std::max<int64_t>(1, std::min<int64_t>(fours, room / p.N)), span = (fours + most - 1) / most, per_token = (fours + span - 1) / span;
   const int64_t blocks = ((int64_t)p.N * per_token + 3) / 4;
   NVC_REQUIRE(ctx, blocks <= 0x7fffffffLL, NVC_ESHAPE, "too many rows");
   DeviceGuard guard(ctx->device);
