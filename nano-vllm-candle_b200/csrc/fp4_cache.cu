@@ -27,8 +27,10 @@ struct StoreArgs {
 // neighbouring lanes'.  A warp takes `span` fours of one token's heads (fours of q heads, then of k, then of v heads), so that the token's angles and slot and the norms' weights are read once for
 // them.  Per token (nh + 2 kv) * 256 bytes in, nh * 256 (and kv * 256 in place) + kv * 144 out.  Kinds of heads in loops of their own: with one loop for all, the instructions were what bound it (370 a
 // four, 95 us for 16 000 tokens of 32 + 16 heads).
-constexpr int kStoreCtas = 5;           // of an SM
-__global__ void __launch_bounds__(128, kStoreCtas) store_fp4_kernel(const StoreArgs p, int span, int warps_per_token) {
+// kTurned: heads are normed and turned.  CTAs of an SM: rows as they are take 58 registers for 96 (in one kernel with the others 16 000 of 8 heads took 30.8 us for 22.6)
+template <bool kTurned> constexpr int kStoreCtas = kTurned ? 5 : 8;
+template <bool kTurned>
+__global__ void __launch_bounds__(128, kStoreCtas<kTurned>) store_fp4_kernel(const StoreArgs p, int span, int warps_per_token) {
   pdl_trigger();
   const int64_t warp = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31, l = lane & 7, sub = lane >> 3;
@@ -41,7 +43,7 @@ __global__ void __launch_bounds__(128, kStoreCtas) store_fp4_kernel(const StoreA
   float4 c0, c1, s0, s1;
   c0 = c1 = s0 = s1 = make_float4(0.f, 0.f, 0.f, 0.f);
   const int q_fours = (p.nh + 3) >> 2, kv_fours = (p.kv + 3) >> 2;
-  if (p.table && first < q_fours + kv_fours) {
+  if (kTurned && first < q_fours + kv_fours) {
     const int pos = p.positions[n];
     if ((unsigned)pos < (unsigned)p.max_pos) {
       const float4* cs = p.table + (int64_t)pos * 32;                        // cos[64], sin[64]
@@ -58,7 +60,7 @@ __global__ void __launch_bounds__(128, kStoreCtas) store_fp4_kernel(const StoreA
 
   // heads 4 * i + sub of one kind, i from `from` to `to`; the next row on its way while one is worked on
   auto heads = [&](auto kind, const nvc_bf16* src, nvc_bf16* dst, const uint4* w, uint8_t* codes_to, uint8_t* scales_to, int count, int from, int to) {
-    constexpr bool kTurn = decltype(kind)::value != 2, kStore = decltype(kind)::value != 0;
+    constexpr bool kTurn = kTurned && decltype(kind)::value != 2, kStore = decltype(kind)::value != 0;
     if (from >= to) return;
     uint4 w0 = make_uint4(0, 0, 0, 0), w1 = w0;
     if (kTurn && w) { w0 = w[l]; w1 = w[l + 8]; }
@@ -72,7 +74,7 @@ __global__ void __launch_bounds__(128, kStoreCtas) store_fp4_kernel(const StoreA
       row += 64;
       if (i + 1 < to && 4 * i + 4 + sub < count) { a = ld_once_u4(row); b = ld_once_u4(row + 8); }
       if (4 * i + sub >= count) break;                                       // (a head's eight lanes alike)
-      if (kTurn && p.table) {
+      if constexpr (kTurn) {
         uint4 o1, o2;
         qk_norm_rope8(x, y, mask, w != nullptr, w0, w1, p.eps, c0, c1, s0, s1, o1, o2);
         x = o1;
@@ -103,7 +105,7 @@ __global__ void __launch_bounds__(128, kStoreCtas) store_fp4_kernel(const StoreA
   };
   const int last = first + span;
   const nvc_bf16* none = nullptr;
-  heads(std::integral_constant<int, 0>(), p.nh ? p.q + n * p.ldq : none, p.nh ? p.q_out + n * p.ldqo : nullptr, p.qw, nullptr, nullptr, p.nh, first, min(last, q_fours));
+  if (kTurned) heads(std::integral_constant<int, 0>(), p.nh ? p.q + n * p.ldq : none, p.nh ? p.q_out + n * p.ldqo : nullptr, p.qw, nullptr, nullptr, p.nh, first, min(last, q_fours));
   heads(std::integral_constant<int, 1>(), p.k + n * p.ldk, p.k_out ? p.k_out + n * p.ldko : nullptr, p.kw, p.kc, p.ks, p.kv, max(first - q_fours, 0), min(last - q_fours, kv_fours));
   heads(std::integral_constant<int, 2>(), p.v + n * p.ldv, nullptr, nullptr, p.vc, p.vs, p.kv, max(first - q_fours - kv_fours, 0), min(last - q_fours - kv_fours, kv_fours));
 }
@@ -150,12 +152,12 @@ int launch_store(nvc_ctx* ctx, const StoreArgs& p, void* stream) {
   // few tokens: their heads over many warps, as long as all run at once; many: all heads of a token in one (2 048 tokens of 32 + 16 heads, us: 12 fours a warp 14.5, 6 16.4, 4 18.4; 1 024: 12.3, 10.2,
   // 12.2; 512: 12.3, 8.3, 8.1, and 3 6.8)
   const int fours = (p.nh + 3) / 4 + 2 * ((p.kv + 3) / 4);
-  const int64_t room = (int64_t)ctx->num_sms * 4 * kStoreCtas;
+  const int64_t room = (int64_t)ctx->num_sms * 4 * (p.table ? kStoreCtas<true> : kStoreCtas<false>);
   const int most = (int)std::max<int64_t>(1, std::min<int64_t>(fours, room / p.N)), span = (fours + most - 1) / most, per_token = (fours + span - 1) / span;
   const int64_t blocks = ((int64_t)p.N * per_token + 3) / 4;
   NVC_REQUIRE(ctx, blocks <= 0x7fffffffLL, NVC_ESHAPE, "too many rows");
   DeviceGuard guard(ctx->device);
-  NVC_CUDA_CHECK(ctx, nvc_launch(ctx, store_fp4_kernel, dim3((unsigned)blocks), dim3(128), 0, nvc_stream(stream), p, span, per_token));
+  NVC_CUDA_CHECK(ctx, nvc_launch(ctx, p.table ? store_fp4_kernel<true> : store_fp4_kernel<false>, dim3((unsigned)blocks), dim3(128), 0, nvc_stream(stream), p, span, per_token));
   NVC_CUDA_CHECK(ctx, cudaGetLastError());
   ctx->launches++;
   return NVC_OK;
