@@ -37,7 +37,9 @@ int launch_few(nvc_ctx* ctx, fp4d::Args& p, int64_t most_rows, cudaStream_t stre
   return NVC_OK;
 }
 
-constexpr int kFewRows = 64;          // of a key head: up to here the kernel for few rows
+// Rows of a sequence and key head up to which the kernel for few rows takes them, in passes of 16 (64 rows, us, few / portions: 32 sequences behind 1 750 86 / 73, 4 22.5 / 28, one behind 16 000
+// 33 / 46, 64 of 300 47 / 55)
+constexpr int kFewRows = 64;
 int64_t most_rows_of(int rows, int max_qlen, int group) { return std::min(rows, max_qlen) * (int64_t)group; }
 size_t many_bytes(const nvc_ctx* ctx) { return (size_t)ctx->num_sms * (16 + 2 * fp4p::kRecord * 4); }
 

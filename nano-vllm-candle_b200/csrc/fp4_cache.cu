@@ -26,7 +26,7 @@ struct StoreArgs {
 // 8 lanes per (token, head): lane l owns the numbers [8l, 8l + 8) and [64 + 8l, 64 + 8l + 8), so that a rotation's pairs are one lane's and a block of 16 is two
 // neighbouring lanes'.  A warp takes `span` fours of one token's heads (fours of q heads, then of k, then of v heads), so that the token's angles and slot and the norms' weights are read once for
 // them.  Per token (nh + 2 kv) * 256 bytes in, nh * 256 (and kv * 256 in place) + kv * 144 out.  Kinds of heads in loops of their own: with one loop for all, the instructions were what bound it (370 a
-// four, 95 us for 16 000 tokens of 32 + 16 heads).
+// four, 95 us for 16 000 tokens of 32 + 16 heads).  Now 275: 80 us, 4.1 TB/s; loads' latency and instructions bound it alike (2.3 an SM and cycle).
 // kTurned: heads are normed and turned.  CTAs of an SM: rows as they are take 58 registers for 96 (in one kernel with the others 16 000 of 8 heads took 30.8 us for 22.6)
 template <bool kTurned> constexpr int kStoreCtas = kTurned ? 5 : 8;
 template <bool kTurned>

@@ -10,7 +10,7 @@ computation is a call through the C ABI (ops.Context).  No CPU path: a CPU tenso
 
 Beyond the reference: the linear layers run in 8 bits after to_fp8() (their loaded weights are converted) or load_fp8() (a checkpoint's own e4m3 weights with
 a scale for each 128 x 128), and take rows that are in 8 bits already - (q, scale), as RMSNorm.forward_fp8 and SiluAndMul.forward_fp8 give them - in place of
-a tensor.
+a tensor.  Attention.fp4_cache keeps keys and values in 4 bits (ops.Fp4Cache), 72 bytes a row of 128 numbers in place of 256.
 """
 from __future__ import annotations
 
