@@ -783,7 +783,7 @@ int nvc_read_kvcache_fp4(nvc_ctx* ctx, const nvc_fp4_cache* cache, const int32_t
                          void* stream);
 /* nvc_paged_decode_attn over such a cache.  q [B, nh * 128] stride ldq; block_tables [B, bt_stride]; out [B, nh * 128] stride ldo (multiples of 8).  A context of length 0 (or
  * less) gives zeros; a length beyond the table's bt_stride * block_size counts as that; a block outside the pool reads as rows of zeros.  Rows past a context
- * may hold anything.  The weights of a row's keys are rounded to fp16 for the second product (2^-11 of each).  workspace: nvc_attn_fp4_workspace_bytes with max_seqlen_q = 1, 16-byte
+ * may hold anything.  out shares no memory with q.  The weights of a row's keys are rounded to fp16 for the second product (2^-11 of each).  workspace: nvc_attn_fp4_workspace_bytes with max_seqlen_q = 1, 16-byte
  * aligned, of this call alone while it runs; nothing in it has to be cleared.
  * A row's sums are grouped by what the whole batch holds and the tables have room for: a call repeats itself bit by bit, a sequence beside others may differ in rounding. */
 size_t nvc_attn_fp4_workspace_bytes(const nvc_ctx* ctx, int nh, int kv, int max_seqlen_q);

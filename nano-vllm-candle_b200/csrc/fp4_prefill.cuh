@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const Args p) {
   pdl_wait();
 
   if (!any) {
-    if (threadIdx.x == 0) p.notes[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    if (threadIdx.x == 0 && !p.alone) p.notes[blockIdx.x] = make_int4(-1, 0, 0, 0);
   } else if (warp >= 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     // ------------------------------------------------------------ the products: a warp for each tile (two of the four).  A product is taken in only when the ones before it are
@@ -665,7 +665,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const Args p) {
       }
       ptx::tcgen05_fence_before();                         // O has been read: the next P V may write it (p_full)
     }
-    if (threadIdx.x == 0) p.notes[blockIdx.x] = *note;
+    if (threadIdx.x == 0 && !p.alone) p.notes[blockIdx.x] = *note;
   }
   ptx::tcgen05_fence_before();
   __syncthreads();

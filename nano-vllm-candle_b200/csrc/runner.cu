@@ -9,6 +9,7 @@
 //   -> fused_add_rmsnorm -> gate_up GEMM (+ SiLU-mul epilogue) -> down GEMM [-> all-reduce]
 // then: gather last rows -> final fused_add_rmsnorm -> lm_head GEMM (fp32) -> argmax.
 #include "runner.h"
+#include "fp4.cuh"
 #include "model_config.h"
 
 #include <algorithm>
@@ -459,7 +460,7 @@ int nvc_runner_get_options(const nvc_runner* r, nvc_runner_options* out) {
 }
 int64_t nvc_runner_kv_bytes_per_token(const nvc_runner* r) {
   if (r && r->body) return r->body->cache_bytes_per_token();
-  return r ? (int64_t)2 * r->cfg.num_hidden_layers * r->kv_l * r->cfg.head_dim * 2 : 0;
+  return r ? (int64_t)2 * r->cfg.num_hidden_layers * r->kv_l * (r->fp4() ? kFp4Codes + kFp4Scales : r->cfg.head_dim * 2) : 0;
 }
 
 }  // extern "C"

@@ -155,3 +155,12 @@ def test_engine_generates(ctx, prefix, chunked):
 def test_other_widths_are_refused(ctx):
     with pytest.raises(Exception, match="kv_cache_bits"):
         _runner(ctx, 8)
+
+
+def test_bytes_of_a_token(ctx):
+    sizes = {}
+    for bits in (16, 4):
+        runner, _ = _runner(ctx, bits)
+        sizes[bits] = runner.kv_bytes_per_token()
+        runner.close()
+    assert sizes[4] * 256 == sizes[16] * 72
