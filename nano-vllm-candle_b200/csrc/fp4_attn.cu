@@ -37,9 +37,9 @@ int launch_few(nvc_ctx* ctx, fp4d::Args& p, int64_t most_rows, cudaStream_t stre
   return NVC_OK;
 }
 
-// Rows of a sequence and key head up to which the kernel for few rows takes them, in passes of 16 (64 rows, us, few / portions: 32 sequences behind 1 750 86 / 73, 4 22.5 / 28, one behind 16 000
-// 33 / 46, 64 of 300 47 / 55)
-constexpr int kFewRows = 64;
+// Rows of a sequence and key head up to which the kernel for few rows takes them, in passes of 16: 32, and 64 where the portions' kernel would have few CTAs with work (us, few / portions; 32 rows: 32
+// sequences behind 1 750 50 / 62, 64 of 300 35 / 42; 48: 70 / 63, 42 / 43, 8 behind 16 000 123 / 110; 64: 88 / 65, 49 / 44, 160 / 111, 4 behind 2 000 25 / 27, one behind 16 000 33 / 39)
+constexpr int kFewRows = 32, kFewRowsOfFew = 64;
 int64_t most_rows_of(int rows, int max_qlen, int group) { return std::min(rows, max_qlen) * (int64_t)group; }
 size_t many_bytes(const nvc_ctx* ctx) { return (size_t)ctx->num_sms * (16 + 2 * fp4p::kRecord * 4); }
 
@@ -76,7 +76,8 @@ int attn_fp4(nvc_ctx* ctx, const nvc_bf16* q, int ldq, const nvc_fp4_cache* cach
   fp4d::Args p{q, out, ldq, ldo, cache->k, cache->k_scale, cache->v, cache->v_scale, block_tables, context_lens, cu_seqlens_q, bt_stride, cache->num_blocks, cache->kv,
                cache->block_size, B, group, rows, scale * 1.4426950408889634f, static_cast<int4*>(workspace), nullptr, 0, 0};
   DeviceGuard guard(ctx->device);
-  if (cu_seqlens_q && most_rows > kFewRows) return launch_many(ctx, p, most_rows, scale, nvc_stream(stream), workspace_bytes);
+  const int few = (int64_t)B * cache->kv <= ctx->num_sms / 4 ? kFewRowsOfFew : kFewRows;
+  if (cu_seqlens_q && most_rows > few) return launch_many(ctx, p, most_rows, scale, nvc_stream(stream), workspace_bytes);
   return most_rows <= 8 ? launch_few<1>(ctx, p, most_rows, nvc_stream(stream), workspace_bytes) : launch_few<2>(ctx, p, most_rows, nvc_stream(stream), workspace_bytes);
 }
 

@@ -521,11 +521,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const Args p) {
         least = x.s.len - x.s.qlen + p.by_group(first + quad * 32);
         n = x.end - x.t;
         t0 = x.t * kKT;
+        if (x.s.qlen * p.group - first <= 32 * quad) n = -n;          // a warp without rows
         if (more) ahead(at);
       }
       __syncwarp();
       const float factor = factors[r];
       float ref = kFloor, sum = 0.f;
+      if (n < 0) {                                         // its barriers go round alone, and it takes no issue slots from the others: 16 x 16 tokens behind 16 000 in 199 us for 214
+        for (int j = 0; j > n; --j, ++g) {
+          wait_bar(s_full(w), g & 1);
+          ptx::mbar_arrive(s_read(w));
+          if (j < 0) wait_bar(o_done(w), (g - 1) & 1);
+          ptx::mbar_arrive(p_full(w));
+        }
+      }
       for (int j = 0; j < n; ++j, ++g, t0 += kKT) {
         wait_bar(s_full(w), g & 1);
         ptx::tcgen05_fence_after();
@@ -615,11 +624,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const Args p) {
       Piece x;
       x.take(park);
       const int first = kRows * x.j + 128 * w, real = x.s.qlen * p.group, tok = p.by_group(first + r);          // (below 2^31: the host's check)
+      const bool rows = real - first > 32 * quad;
       wait_bar(o_done(w), (g - 1) & 1);
       ptx::tcgen05_fence_after();
       const bool begins = x.t == 0, ends = x.end == x.tiles;
       const int* const from = nan_from + 12 * (done++ & 3);
-      if (from[8]) {                                       // (a NaN in the cache: into O where the row sees it, 16 columns at a time)
+      if (rows && from[8]) {                               // (a NaN in the cache: into O where the row sees it, 16 columns at a time)
 #pragma unroll 1
         for (int c = 0; c < 8; ++c) {
           uint32_t v[16];
@@ -632,7 +642,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const Args p) {
         }
         ptx::tmem_st_wait();
       }
-      if (begins && ends) {
+      if (rows && begins && ends) {
         const float inv = sum == 0.f ? 0.f : 1.0f / sum;   // seen nothing: zeros
         const int at_row = x.s.begin + tok;
         const bool there = first + r < real && (unsigned)at_row < (unsigned)p.rows;
@@ -647,7 +657,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_kernel(const Args p) {
             dst[k] = make_uint4(pack_bf16(__uint_as_float(v[8 * k]) * inv, __uint_as_float(v[8 * k + 1]) * inv), pack_bf16(__uint_as_float(v[8 * k + 2]) * inv, __uint_as_float(v[8 * k + 3]) * inv),
                                 pack_bf16(__uint_as_float(v[8 * k + 4]) * inv, __uint_as_float(v[8 * k + 5]) * inv), pack_bf16(__uint_as_float(v[8 * k + 6]) * inv, __uint_as_float(v[8 * k + 7]) * inv));
         }
-      } else {
+      } else if (rows) {
         if (begins && threadIdx.x == 0) *note = make_int4(x.b, x.j, x.h, (int)blockIdx.x + 1 + (x.tiles - 1 - x.end) / per);
         float* part = p.parts + ((int64_t)blockIdx.x * 2 + (begins ? 1 : 0)) * kRecord;
         const int row = 128 * w + r;
@@ -682,6 +692,9 @@ __global__ void __launch_bounds__(256) combine_kernel(const Args p) {
   pdl_wait();
   const int4 note = __ldcg(p.notes + c0);
   if (note.x < 0) return;
+  const Seq s = seq_of(p, note.x);
+  const int packed = kRows * note.y + row, tok = p.by_group(packed), at_row = s.begin + tok;
+  if (packed >= s.qlen * p.group || (unsigned)at_row >= (unsigned)p.rows) return;          // (no row: its record holds anything)
   const int c1 = note.w;
   auto record = [&](int i) { return p.parts + ((int64_t)i * 2 + (i == c0 ? 1 : 0)) * kRecord; };
   // two records (most units lie in two CTAs) on their way at once, the sums against the larger reference so far
@@ -708,9 +721,6 @@ __global__ void __launch_bounds__(256) combine_kernel(const Args p) {
     }
     top = now;
   }
-  const Seq s = seq_of(p, note.x);
-  const int packed = kRows * note.y + row, tok = p.by_group(packed), at_row = s.begin + tok;
-  if (packed >= s.qlen * p.group || (unsigned)at_row >= (unsigned)p.rows) return;
   const float inv = l == 0.f ? 0.f : 1.0f / l;
   uint4* dst = reinterpret_cast<uint4*>(p.out + at_row * p.ldo + (int64_t)(note.z * p.group + packed - tok * p.group) * 128) + 2 * d0;
 #pragma unroll

@@ -353,3 +353,12 @@ def test_portions_of_few_rows_with_room_for_more(ctx, new, before, nh, kv, bs):
     for d in (c, _room(c)):
         got = _portions(ctx, d)
         assert not got[:new[0]].any() and torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("rows", [8, 9, 16, 17, 32, 33, 48, 64, 65])
+@pytest.mark.parametrize("seqs", [1, 40])
+def test_portions_around_the_kernels_ends(ctx, seqs, rows):
+    """Numbers of rows of a key head at which another kernel takes them, for few sequences and for many."""
+    c = _case([rows + 70] * seqs, 1, 1, 16, new=[rows] * seqs, seed=25)
+    for d in (c, _room(c)):
+        _near(_portions(ctx, d), d)
