@@ -17,9 +17,9 @@ template <int NT> int64_t parts_bytes(const nvc_ctx* ctx) { return (int64_t)ctx-
 constexpr int kMostAlone = 65535;          // CTAs
 
 template <int NT>
-int launch_few(nvc_ctx* ctx, fp4d::Args& p, int64_t most_rows, cudaStream_t stream, size_t workspace_bytes) {
+int launch_few(nvc_ctx* ctx, fp4d::Args& p, int64_t most_rows, int blocks, cudaStream_t stream, size_t workspace_bytes) {
   const int64_t units = p.kv * ((most_rows + fp4d::kCols<NT> - 1) / fp4d::kCols<NT>);          // of a sequence, at most
-  const int64_t tiles = ((int64_t)p.bt_stride * p.block_size + fp4d::kTile - 1) / fp4d::kTile;        // of a sequence, at most
+  const int64_t tiles = ((int64_t)blocks * p.block_size + fp4d::kTile - 1) / fp4d::kTile;        // of a sequence, at most (a hint that is too low costs time alone)
   // units at most by max_seqlen_q, and whatever cu_seqlens say
   const int64_t room = p.cu_seqlens ? p.kv * ((int64_t)p.rows * p.group / fp4d::kCols<NT> + p.B) : units * p.B;
   const bool alone = fp4d::alone<NT>(ctx->num_sms, std::min(units * p.B, room), tiles) && room <= kMostAlone;
@@ -60,7 +60,7 @@ int launch_many(nvc_ctx* ctx, const fp4d::Args& f, int64_t most_rows, float scal
   return NVC_OK;
 }
 
-int attn_fp4(nvc_ctx* ctx, const nvc_bf16* q, int ldq, const nvc_fp4_cache* cache, const int32_t* block_tables, int bt_stride, const int32_t* context_lens,
+int attn_fp4(nvc_ctx* ctx, const nvc_bf16* q, int ldq, const nvc_fp4_cache* cache, const int32_t* block_tables, int bt_stride, int blocks, const int32_t* context_lens,
              const int32_t* cu_seqlens_q, int B, int rows, int max_qlen, int nh, float scale, nvc_bf16* out, int ldo, void* workspace, size_t workspace_bytes, void* stream) {
   if (const int rc = nvc_fp4_cache_check(ctx, cache)) return rc;
   NVC_REQUIRE(ctx, q && block_tables && context_lens && out, NVC_EINVAL, "null pointer");
@@ -78,7 +78,7 @@ int attn_fp4(nvc_ctx* ctx, const nvc_bf16* q, int ldq, const nvc_fp4_cache* cach
   DeviceGuard guard(ctx->device);
   const int few = (int64_t)B * cache->kv <= ctx->num_sms / 4 ? kFewRowsOfFew : kFewRows;
   if (cu_seqlens_q && most_rows > few) return launch_many(ctx, p, most_rows, scale, nvc_stream(stream), workspace_bytes);
-  return most_rows <= 8 ? launch_few<1>(ctx, p, most_rows, nvc_stream(stream), workspace_bytes) : launch_few<2>(ctx, p, most_rows, nvc_stream(stream), workspace_bytes);
+  return most_rows <= 8 ? launch_few<1>(ctx, p, most_rows, blocks, nvc_stream(stream), workspace_bytes) : launch_few<2>(ctx, p, most_rows, blocks, nvc_stream(stream), workspace_bytes);
 }
 
 }  // namespace
@@ -99,12 +99,18 @@ extern "C" size_t nvc_attn_fp4_workspace_bytes(const nvc_ctx* ctx, int nh, int k
 
 extern "C" int nvc_paged_decode_attn_fp4(nvc_ctx* ctx, const nvc_bf16* q, int ldq, const nvc_fp4_cache* cache, const int32_t* block_tables, int bt_stride,
                                          const int32_t* context_lens, int B, int nh, float scale, nvc_bf16* out, int ldo, void* workspace, size_t workspace_bytes, void* stream) {
-  return attn_fp4(ctx, q, ldq, cache, block_tables, bt_stride, context_lens, nullptr, B, B, 1, nh, scale, out, ldo, workspace, workspace_bytes, stream);
+  return attn_fp4(ctx, q, ldq, cache, block_tables, bt_stride, bt_stride, context_lens, nullptr, B, B, 1, nh, scale, out, ldo, workspace, workspace_bytes, stream);
+}
+
+extern "C" int nvc_paged_decode_attn_fp4_ex(nvc_ctx* ctx, const nvc_bf16* q, int ldq, const nvc_fp4_cache* cache, const int32_t* block_tables, int bt_stride, int max_blocks_hint,
+                                            const int32_t* context_lens, int B, int nh, float scale, nvc_bf16* out, int ldo, void* workspace, size_t workspace_bytes, void* stream) {
+  const int blocks = max_blocks_hint > 0 ? std::min(max_blocks_hint, bt_stride) : bt_stride;
+  return attn_fp4(ctx, q, ldq, cache, block_tables, bt_stride, blocks, context_lens, nullptr, B, B, 1, nh, scale, out, ldo, workspace, workspace_bytes, stream);
 }
 
 extern "C" int nvc_prefill_attn_paged_fp4(nvc_ctx* ctx, const nvc_bf16* q, int ldq, const nvc_fp4_cache* cache, const int32_t* block_tables, int bt_stride,
                                           const int32_t* context_lens, const int32_t* cu_seqlens_q, int B, int total_q_tokens, int max_seqlen_q, int nh, float scale, nvc_bf16* out,
                                           int ldo, void* workspace, size_t workspace_bytes, void* stream) {
   NVC_REQUIRE(ctx, ctx && cu_seqlens_q, NVC_EINVAL, "null pointer");
-  return attn_fp4(ctx, q, ldq, cache, block_tables, bt_stride, context_lens, cu_seqlens_q, B, total_q_tokens, max_seqlen_q, nh, scale, out, ldo, workspace, workspace_bytes, stream);
+  return attn_fp4(ctx, q, ldq, cache, block_tables, bt_stride, bt_stride, context_lens, cu_seqlens_q, B, total_q_tokens, max_seqlen_q, nh, scale, out, ldo, workspace, workspace_bytes, stream);
 }

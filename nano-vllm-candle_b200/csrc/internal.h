@@ -10,6 +10,9 @@ int nvc_paged_decode_attn_ex(nvc_ctx* ctx, const nvc_bf16* q, int ldq, const nvc
                              const nvc_bf16* v_cache, const int32_t* block_tables, int bt_stride, int max_blocks_hint,
                              const int32_t* context_lens, int B, int nh, int kv, int hd, int block_size, float scale,
                              nvc_bf16* out, void* workspace, size_t workspace_bytes, void* stream);
+// nvc_paged_decode_attn_fp4 with the blocks that contexts take by the caller's knowledge, for the choice of schedule
+int nvc_paged_decode_attn_fp4_ex(nvc_ctx* ctx, const nvc_bf16* q, int ldq, const nvc_fp4_cache* cache, const int32_t* block_tables, int bt_stride, int max_blocks_hint,
+                                 const int32_t* context_lens, int B, int nh, float scale, nvc_bf16* out, int ldo, void* workspace, size_t workspace_bytes, void* stream);
 // pairs[b] = {val[b], idx[b]} as 8-byte records
 int nvc_pack_argmax_pairs(nvc_ctx* ctx, const float* val, const int32_t* idx, float* pairs, int B, void* stream);
 int nvc_gemm_bf16_ex(nvc_ctx* ctx, const nvc_bf16* A, int lda, const nvc_bf16* W, void* C, int ldc, int out_dtype,

@@ -87,7 +87,7 @@ int run_layers(nvc_runner* r, int N, bool decode, int B, int max_seqlen, int blo
       // the same rows of the step over the 4-bit cache
       const int single = decode ? B : num_decode, ldo = r->nh_l * hd;
       if (single > 0)
-        rc = nvc_paged_decode_attn_fp4(ctx, r->qkv, r->qkv_l, &Ly.fp4, r->d_bt, r->max_blocks_cap, r->d_ctx, single, r->nh_l, scale, r->attn, ldo, r->decode_ws, r->decode_ws_bytes, st);
+        rc = nvc_paged_decode_attn_fp4_ex(ctx, r->qkv, r->qkv_l, &Ly.fp4, r->d_bt, r->max_blocks_cap, blocks_hint, r->d_ctx, single, r->nh_l, scale, r->attn, ldo, r->decode_ws, r->decode_ws_bytes, st);
       if (rc == NVC_OK && !decode && B > num_decode)
         rc = nvc_prefill_attn_paged_fp4(ctx, r->qkv + (size_t)num_decode * r->qkv_l, r->qkv_l, &Ly.fp4, r->d_bt + (size_t)num_decode * r->max_blocks_cap, r->max_blocks_cap,
                                         r->d_ctx + num_decode, num_decode ? r->d_cu2 : r->d_cu, B - num_decode, N - num_decode, max_seqlen, r->nh_l, scale,
@@ -974,7 +974,7 @@ extern "C" int nvc_runner_time_op(nvc_runner* r, int op, int iters, float* ms_pe
       switch (op) {
         case NVC_OP_PAGED_DECODE:
           if (r->fp4()) {
-            rc = nvc_paged_decode_attn_fp4(ctx, r->qkv, r->qkv_l, &L.fp4, r->d_bt, r->max_blocks_cap, r->d_ctx, B, r->nh_l, scale, r->attn, r->nh_l * hd, r->decode_ws, r->decode_ws_bytes, st);
+            rc = nvc_paged_decode_attn_fp4_ex(ctx, r->qkv, r->qkv_l, &L.fp4, r->d_bt, r->max_blocks_cap, r->last_decode_hint, r->d_ctx, B, r->nh_l, scale, r->attn, r->nh_l * hd, r->decode_ws, r->decode_ws_bytes, st);
             break;
           }
           rc = nvc_paged_decode_attn_ex(ctx, r->qkv, r->qkv_l, L.k_cache, L.v_cache, r->d_bt, r->max_blocks_cap,
