@@ -47,6 +47,7 @@ __device__ __forceinline__ uint32_t fp4_amax8(const uint4& x) {
   const uint32_t m = __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
   return max(m & 0xffffu, m >> 16);
 }
+__device__ __forceinline__ void fp4_prefetch(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 // eight codes -> four pairs of fp16 numbers
 __device__ __forceinline__ uint4 fp4_halves8(uint32_t codes) {
   uint4 r;
