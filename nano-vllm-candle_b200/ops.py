@@ -1241,7 +1241,7 @@ def read_kvcache_fp4(ctx, cache: Fp4Cache, slots):
     if N >> 31:
         raise ValueError(_TOO_FAR)
     k, ks = slots.new_empty(N, kv, 128, dtype=FP8), slots.new_empty(N, kv, 8, dtype=BF16)
-    v, vs = slots.new_empty(N, kv, 128, dtype=FP8), slots.new_empty(N, kv, 8, dtype=BF16)
+    v, vs = torch.empty_like(k), torch.empty_like(ks)
     if N:
         st = ctx.l.nvc_read_kvcache_fp4(ctx.h, cache.c, slots.data_ptr(), k.data_ptr(), ks.data_ptr(), v.data_ptr(), vs.data_ptr(), N, torch._C._cuda_getCurrentRawStream(dev))
         if st:
