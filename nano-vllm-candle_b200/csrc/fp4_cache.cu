@@ -56,7 +56,8 @@ __global__ void __launch_bounds__(128, kStoreCtas<kTurned>) store_fp4_kernel(con
   const bool stored = (unsigned)slot < (unsigned)p.slots;
   const int block = stored ? slot / p.block_size : 0;
   const int64_t page_row = (int64_t)block * p.kv * p.block_size + (stored ? slot - block * p.block_size : 0);
-  if (kTurned && p.qw && warps_per_token > 1 && lane < 4) fp4_prefetch((lane < 2 ? p.qw : p.kw) + 8 * (lane & 1));          // few tokens (read behind the wait)
+  // (read behind the wait.  By one CTA: asked for by all, they cost 512 tokens 8.4 us for 7.0)
+  if (kTurned && p.qw && blockIdx.x == 0 && threadIdx.x < 4) fp4_prefetch((lane < 2 ? p.qw : p.kw) + 8 * (lane & 1));
   pdl_wait();
 
   // heads 4 * i + sub of one kind, i from `from` to `to`; the next row on its way while one is worked on

@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<NT>) attn_kernel(const Args
   if (rd_any) {
     enter();
     // the first rows on their way to L2, where whatever is still written finds them (they are read behind the wait).  With the store's weights alike a decode
-    // step of the 0.6B model takes 0.952 ms for 0.968 (one sequence of 100), 1.044 for 1.058 (of 500)
+    // step of the 0.6B model takes 0.956 ms for 0.967 (one sequence of 100), 1.048 for 1.058 (of 500)
     if (there) {
       const int tiles = whole ? min(min(kRing, rd.end - rd.t), page_left / 2) : 1, line = lane & 15;
       for (int i = 0; i < tiles; ++i) {
