@@ -349,7 +349,8 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<NT>) attn_kernel(const Args
       }
       page_left -= 2;
       half_at += 2;
-    } else {                                          // a barrier phase takes one arrival: behind both halves
+    } else {                                          // a barrier phase takes one arrival: behind both halves, by the lane that told it their bytes
+      const bool one = ptx::elect_one();
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         if (rd.t * kTile + h * kHalf < rd.s.len) {
@@ -358,7 +359,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<NT>) attn_kernel(const Args
             turn(next, 0);
           }
           if (there) {
-            if (ptx::elect_one()) {
+            if (one) {
               asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(stage_bar), "r"(kStageBytes / 2) : "memory");
               copy(st + h * kHalf * kFp4Codes, st + h * kHalf * kFp4Scales, stage_bar, kHalf);
             }
@@ -371,7 +372,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<NT>) attn_kernel(const Args
           gone |= 1u << h;
         }
       }
-      if (lane == 0) ptx::mbar_arrive(stage_bar);
+      if (one) ptx::mbar_arrive(stage_bar);
     }
     absent = (absent & ~(3u << (2 * stage))) | gone << (2 * stage);
     if (++rd.t == rd.end) {
