@@ -87,30 +87,25 @@ __device__ __forceinline__ uint32_t halves(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
   return d;
 }
-// (not volatile: they may be moved, but not in front of where their stage's address becomes known, behind the wait)
+// (volatile, and of memory: held behind the wait for their stage and in front of the warp's barrier that lets it be filled again.  Without either: the same times within half a percent)
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
   uint4 v;
-  asm("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
   return v;
 }
 __device__ __forceinline__ uint2 lds64(uint32_t a) {
-  uint2 v;
-  asm("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ uint2 lds64_now(uint32_t a) {
   uint2 v;
   asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
   return v;
 }
 __device__ __forceinline__ uint32_t lds16(uint32_t a) {
   uint16_t v;
-  asm("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a) : "memory");
   return v;
 }
 __device__ __forceinline__ uint32_t lds8(uint32_t a) {
   uint32_t v;
-  asm("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(a));
+  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
   return v;
 }
 // The copies that the barrier counts are of memory of this GPU, so that it always completes
@@ -534,7 +529,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtas<NT>) attn_kernel(const Args
         __syncwarp();
       }
       if (kPortions && (at.t + 1) * kTile > least) {
-        const uint2 scales = lds64_now(st + kAtVs + lane * kFp4Scales);
+        const uint2 scales = lds64(st + kAtVs + lane * kFp4Scales);
         const uint32_t lo = __vcmpeq4(scales.x, 0xffffffffu), hi = __vcmpeq4(scales.y, 0xffffffffu);
         if (__any_sync(0xffffffffu, lo | hi)) {
           if (lo | hi) {

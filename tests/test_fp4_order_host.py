@@ -22,3 +22,9 @@ def test_the_lane_that_counts_a_stage_s_bytes_arrives_for_it():
     assert "ptx::elect_one()" in halves and halves.count("elect_one") == 1      # one choice for the expected bytes, the copies and the arrival
     assert "lane == 0" not in halves
     assert re.search(r"if \(one\) \{\s*asm volatile\(\"mbarrier\.expect_tx", halves) and re.search(r"if \(one\) ptx::mbar_arrive\(stage_bar\)", halves)
+
+
+def test_a_stage_is_read_in_front_of_its_release():
+    """Shared loads that the compiler may move could come behind the warp's barrier, and so behind the copies that fill their stage again."""
+    loads = re.findall(r"asm[^;]*?ld\.shared[^;]*;[^;]*;", _source("fp4_decode.cuh"))
+    assert len(loads) == 4 and all(x.startswith("asm volatile(") and re.search(r":\s*\"memory\"\);$", x) for x in loads), loads
