@@ -93,7 +93,7 @@ extern "C" int nvc_fp4_attn_init(nvc_ctx* ctx) {
 extern "C" size_t nvc_attn_fp4_workspace_bytes(const nvc_ctx* ctx, int nh, int kv, int max_seqlen_q) {
   if (!ctx || nh <= 0 || kv <= 0 || max_seqlen_q <= 0) return 0;
   const int64_t rows = most_rows_of(max_seqlen_q, max_seqlen_q, (nh + kv - 1) / kv);
-  const size_t few = (size_t)(rows <= 8 ? parts_bytes<1>(ctx) : parts_bytes<2>(ctx));          // (decode: whatever its rows are)
+  const size_t few = (size_t)std::max(parts_bytes<1>(ctx), parts_bytes<2>(ctx));          // of either, so that a longer call's serves a shorter one
   return rows > kFewRows ? std::max(few, many_bytes(ctx)) : few;
 }
 

@@ -426,9 +426,7 @@ int nvc_runner_create(nvc_ctx* ctx, const nvc_qwen3_config* cfg, const nvc_runne
   r->decode_ws_bytes = 0;
   for (int b = 1; b <= opt->max_num_seqs; ++b)
     r->decode_ws_bytes = std::max(r->decode_ws_bytes, nvc_paged_decode_workspace_bytes(b, r->nh_l, hd, ctx->num_sms));
-  if (r->fp4())
-    r->decode_ws_bytes = std::max(nvc_attn_fp4_workspace_bytes(ctx, r->nh_l, r->kv_l, 1),
-                                  std::max(nvc_attn_fp4_workspace_bytes(ctx, r->nh_l, r->kv_l, 16), nvc_attn_fp4_workspace_bytes(ctx, r->nh_l, r->kv_l, opt->max_num_batched_tokens)));
+  if (r->fp4()) r->decode_ws_bytes = nvc_attn_fp4_workspace_bytes(ctx, r->nh_l, r->kv_l, opt->max_num_batched_tokens);
   if ((rc = dev_alloc(r, reinterpret_cast<uint8_t**>(&r->decode_ws), r->decode_ws_bytes))) return rc;
   if ((rc = alloc_step_buffers(r))) return rc;
   return NVC_OK;
