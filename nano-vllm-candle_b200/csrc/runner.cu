@@ -951,6 +951,11 @@ extern "C" int nvc_runner_time_op(nvc_runner* r, int op, int iters, float* ms_pe
   R_CUDA(cudaEventCreate(&e0));
   R_CUDA(cudaEventCreate(&e1));
   R_CUDA(cudaStreamSynchronize(r->stream));
+  int32_t* nowhere = nullptr;      // slots that the cache does not have: a 4-bit store that is timed leaves the cached rows as they are
+  if (op == NVC_OP_QK_NORM_ROPE && r->fp4()) {
+    R_CUDA(cudaMalloc(&nowhere, B * sizeof(int32_t)));
+    R_CUDA(cudaMemsetAsync(nowhere, 0xff, B * sizeof(int32_t), r->stream));
+  }
   int rc = NVC_OK, n = 0;
   const uint64_t l0 = ctx->launches;
   // one pass over the layers is captured into a CUDA graph and replayed `iters` times, so the
@@ -995,6 +1000,11 @@ extern "C" int nvc_runner_time_op(nvc_runner* r, int op, int iters, float* ms_pe
           rc = nvc_fused_add_rmsnorm(ctx, r->x, r->residual, r->residual, L.ln2, c.rms_norm_eps, r->xn, B, H, st);
           break;
         case NVC_OP_QK_NORM_ROPE:
+          if (r->fp4()) {      // all of the step's kernel but the writes of 144 bytes a key head
+            rc = nvc_qk_norm_rope_store_fp4(ctx, r->qkv, r->qkv_l, L.q_norm, L.k_norm, c.rms_norm_eps, r->rope, r->opt.max_model_len, r->d_pos, nowhere, &L.fp4, nullptr, 0, B, r->nh_l,
+                                            st);
+            break;
+          }
           // slot_mapping = NULL: do not scatter (the qkv buffer no longer holds this step's k/v)
           rc = nvc_qk_norm_rope_store(ctx, r->qkv, L.q_norm, L.k_norm, c.rms_norm_eps, r->rope, r->d_pos, nullptr,
                                       nullptr, nullptr, B, r->nh_l, r->kv_l, hd, st);
@@ -1036,6 +1046,7 @@ extern "C" int nvc_runner_time_op(nvc_runner* r, int op, int iters, float* ms_pe
   if (exec) cudaGraphExecDestroy(exec);
   cudaEventDestroy(e0);
   cudaEventDestroy(e1);
+  if (nowhere) cudaFree(nowhere);
   if (rc) return rc;
   R_CUDA(ce);
   const int kernels = (int)(ctx->launches - l0) * iters;
