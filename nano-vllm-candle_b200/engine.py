@@ -382,15 +382,17 @@ class ModelRunner(Qwen3ModelRunner):
     and `step_mixed` (the engine drives them the same way).
 
     dtype: "bfloat16" (serving: bf16 storage and tensor-core products, fp32 residual / norms /
-    softmax / routers) or "float32" (exact mode: everything in IEEE fp32 on the FMA pipe)."""
+    softmax / routers) or "float32" (exact mode: everything in IEEE fp32 on the FMA pipe).
+    kv_cache_bits: as in Qwen3ModelRunner; the other architectures keep their caches in formats of their own and refuse 4."""
 
     DTYPES = {"bfloat16": 0, "float32": 1}
 
     def __init__(self, ctx, config_handle, num_kvcache_blocks: int, kvcache_block_size: int = 64, max_num_seqs: int = 64,
                  max_num_batched_tokens: int = 4096, max_model_len: Optional[int] = None, use_cuda_graph: bool = True,
-                 dtype: str = "bfloat16", max_logit_rows: int = 0):
+                 dtype: str = "bfloat16", max_logit_rows: int = 0, kv_cache_bits: int = 16):
         self.l = _lib.lib()
         self.ctx = ctx
+        self.kv_cache_bits = kv_cache_bits
         self.architecture = self.l.nvc_model_config_architecture(config_handle).decode()
         self.dtype = dtype
         self.block_size = kvcache_block_size
@@ -399,7 +401,7 @@ class ModelRunner(Qwen3ModelRunner):
         self.max_model_len = max_model_len
         self.max_num_seqs, self.max_num_batched_tokens = max_num_seqs, max_num_batched_tokens
         opt = RunnerOptionsC(num_kvcache_blocks, kvcache_block_size, max_num_seqs, max_num_batched_tokens, max_model_len,
-                             1 if use_cuda_graph else 0, 0, self.DTYPES[dtype], max_logit_rows)
+                             1 if use_cuda_graph else 0, 0, self.DTYPES[dtype], max_logit_rows, kv_cache_bits)
         h = C.c_void_p()
         st = self.l.nvc_runner_create_from_config(ctx.h, config_handle, C.byref(opt), C.byref(h))
         self.handle = h

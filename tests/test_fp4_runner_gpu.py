@@ -169,3 +169,25 @@ def test_generations_against_the_model(ctx, prefix, chunked):
     outs = eng.LLMEngine(eng.Scheduler(_config(prefix, chunked)), runner, greedy=True).generate(prompts, eng.SamplingParams(1.0, 24, True))
     assert [o.token_ids for o in outs] == said
     runner.close()
+
+
+def test_registry_runner(ctx, tmp_path):
+    """ModelRunner over a Qwen3 directory with a 4-bit cache is Qwen3ModelRunner with one; an architecture with caches of its own refuses it."""
+    import test_hf_loader as H
+    import test_vizotar_model_gpu as V
+    w = synth.make_weights(CFG, seed=4, norm_jitter=0.1)
+    H._write_config(tmp_path, CFG, head_dim=CFG.head_dim, tie_word_embeddings=False)
+    H.save_file({k: v.to(torch.bfloat16).contiguous() for k, v in w.items()}, str(tmp_path / "model.safetensors"))
+    kw = dict(num_kvcache_blocks=16, kvcache_block_size=16, max_num_seqs=2, max_num_batched_tokens=256, max_model_len=256, kv_cache_bits=4)
+    logits = []
+    for kind in (lambda: eng.ModelRunner.from_dir(ctx, str(tmp_path), **kw), lambda: eng.Qwen3ModelRunner.from_hf_dir(ctx, str(tmp_path), **kw)):
+        r = kind()
+        assert r.kv_bytes_per_token() == CFG.num_hidden_layers * CFG.num_key_value_heads * 2 * 72
+        r.prefill(range(10, 31), range(21), [0, 21], range(16, 37))
+        r.decode([5], [21], [37], np.array([[1, 2]], dtype=np.int32), [22])
+        logits.append(r.last_logits(1).copy())
+        r.close()
+    assert np.array_equal(*logits)
+    cfg = V.Z.make_config(vocab=70, width=64, streams=2, layers=[V.Z.with_dense(V.Z.delta_cfg())])
+    with pytest.raises(Exception, match="formats"):
+        eng.ModelRunner.from_config(ctx, cfg, [], num_kvcache_blocks=2, kvcache_block_size=BS, max_num_seqs=1, max_num_batched_tokens=32, max_model_len=32, dtype="float32", kv_cache_bits=4)
