@@ -786,6 +786,7 @@ int nvc_read_kvcache_fp4(nvc_ctx* ctx, const nvc_fp4_cache* cache, const int32_t
  * may hold anything.  out shares no memory with q.  The weights of a row's keys are rounded to fp16 for the second product (2^-11 of each).  workspace: nvc_attn_fp4_workspace_bytes with max_seqlen_q = 1, 16-byte
  * aligned, of this call alone while it runs; nothing in it has to be cleared.
  * (A workspace for a longer max_seqlen_q of the same heads serves shorter calls and decode too.)
+ * Scores are formed in fp32 and have to stay below 2^22 in magnitude (scale * q . k; a row beyond that may come out as anything, NaN included, and touches no other).
  * A row's sums are grouped by what the whole batch holds and the tables have room for: a call repeats itself bit by bit, a sequence beside others may differ in rounding. */
 size_t nvc_attn_fp4_workspace_bytes(const nvc_ctx* ctx, int nh, int kv, int max_seqlen_q);
 int nvc_paged_decode_attn_fp4(nvc_ctx* ctx, const nvc_bf16* q, int ldq, const nvc_fp4_cache* cache, const int32_t* block_tables, int bt_stride,

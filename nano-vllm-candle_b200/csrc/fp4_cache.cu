@@ -26,7 +26,8 @@ struct StoreArgs {
 // 8 lanes per (token, head): lane l owns the numbers [8l, 8l + 8) and [64 + 8l, 64 + 8l + 8), so that a rotation's pairs are one lane's and a block of 16 is two
 // neighbouring lanes'.  A warp takes `span` fours of one token's heads (fours of q heads, then of k, then of v heads), so that the token's angles and slot and the norms' weights are read once for
 // them.  Per token (nh + 2 kv) * 256 bytes in, nh * 256 (and kv * 256 in place) + kv * 144 out.  Kinds of heads in loops of their own: with one loop for all, the instructions were what bound it (370 a
-// four, 95 us for 16 000 tokens of 32 + 16 heads).  Now 275: 80 us, 4.1 TB/s; loads' latency and instructions bound it alike (2.3 an SM and cycle).
+// four, 95 us for 16 000 tokens of 32 + 16 heads).  Now 275: 80 us, 4.1 TB/s: loads' latency, with a row ahead of 20 warps in flight, 20 KB an SM (2.3 instructions of 4 a
+// cycle).
 // kTurned: heads are normed and turned.  CTAs of an SM: rows as they are take 58 registers for 96 (in one kernel with the others 16 000 of 8 heads took 30.8 us for 22.6)
 template <bool kTurned> constexpr int kStoreCtas = kTurned ? 5 : 8;
 template <bool kTurned>
@@ -117,8 +118,8 @@ __device__ __forceinline__ uint32_t prmt_signs(uint32_t x, uint32_t selector) {
   asm("prmt.b32 %0, %1, %1, %2;" : "=r"(d) : "r"(x), "r"(selector));
   return d;
 }
-// 8 lanes per (row, head), 16 numbers of K and of V a lane.  288 bytes out for 144 in; the instructions are what bounds it (a side for 8 lanes, with divisions in 64 bits: 19 us for 16 000 tokens of
-// 8 heads)
+// 8 lanes per (row, head), 16 numbers of K and of V a lane.  288 bytes out for 144 in.  16 000 tokens of 8 heads: 12.5 us for 8.6 of bytes, a lane's one slot, row and store behind one another (1.45
+// instructions of 4 a cycle, memory at 18 %); a side for 8 lanes, with divisions in 64 bits: 19 us
 __global__ void __launch_bounds__(256)
 read_fp4_kernel(const uint8_t* kc, const uint8_t* ks, const uint8_t* vc, const uint8_t* vs, int kv, int block_size, Fp4Div by_heads, Fp4Div by_block, int slots, const int32_t* slot_list,
                 uint4* k, nvc_bf16* k_scale, uint4* v, nvc_bf16* v_scale, int units) {

@@ -17,7 +17,9 @@
 // A cached value that is no number counts for the columns that see it, and for no other: where a tile is not seen whole by every column, such a value goes in as 0 (a weight of 0 would not keep
 // it out), and the first token that has one in each block of 16 dims is remembered for the columns that do see it.
 //
-// What bounds it: a warp's instructions and their latency (2.5 an SM and cycle; half the ALU's rate, where every two numbers cost a conversion).  256 contexts of 1 to 4 000 tokens, 8 key heads of
+// What bounds it: a warp's instructions and their latency (2.5 of 4 an SM and cycle, the ALU at half its rate).  A tile takes 719 of them in pages of 16 and 629 in pages of 256, of which 288 are its
+// arithmetic (128 conversions of two numbers, 128 products with their scales, 32 matrix instructions); the others are on the ALU (163, 134: bytes of words taken apart and put together, scales widened,
+// masks, addresses) and the FMA pipe (106, 87: exponents, sums, references), and 55 to 75 loads, branches and barriers.  256 contexts of 1 to 4 000 tokens, 8 key heads of
 // 4 query heads: 136 us for 596 MB, 4.4 TB/s; 4 of 30 000 to 131 000, 8 query heads: 80 us, 4.6 TB/s.
 //
 // The exponentials are taken against a reference that follows a column's maximum only when that grew by more than 2^8 (a vote; nothing is exchanged otherwise), shifted by 2^7: weights lie

@@ -3,8 +3,9 @@
 // One CTA per SM, 256 query rows - the rows of all the query heads of a key head, head by head within a token - as two tiles of 128 against key tiles of 128 tokens:
 //   * 4 warps decode the cache's rows into fp16 tiles in shared memory (K and V, two of each), once for 256 rows: half a percent of what decoding for each head would cost.  A thread
 //     has a token's row: 64 bytes of codes and 8 of scales, requested two tiles ahead;
-//   * 1 warp issues the products, S_w = Q_w K^T and O_w += P_w V, tile 0's and tile 1's in turn, so that the tensor cores work on one while the other's softmax runs;
-//   * 4 warps for each tile: a thread owns a row.  P goes back into tensor memory over the S it came from (fp16 pairs) and is the A operand there.  The reference of the exponentials
+//   * a warp for each tile w issues its products, S_w = Q_w K^T and O_w += P_w V, so that the tensor cores work on one while the other's softmax runs.  There is room for one S: the tiles take
+//     it in turn, 128 columns of tensor memory that s_read of the other tile's rows lets go.  P_w (64 columns, fp16 pairs, the A operand) and O_w (128) have their own;
+//   * 4 warps for each tile: a thread owns a row, takes its S into registers at once, and writes P_w.  The reference of the exponentials
 //     follows the row's maximum when that grew by more than 2^8, shifted by 2^7, as in the kernel for few rows; only then O is rescaled.
 // Queries are brought to fp16 behind a power of two of their own row, that the score's factor takes back.  The sign of the scale goes with them, so that a row's maximum may be taken in front of
 // the factor.
@@ -12,7 +13,8 @@
 // A cached value that is no number counts for the rows that see it, and for no other.  A weight of 0 would not keep it from them, so it goes in as 0, and the first token with a NaN in each
 // block of 16 dims is remembered: a row that sees it has NaN there.
 //
-// What bounds it: the tensor cores' rate under the power cap where contexts are long - a prompt of 8 191 tokens, 32 heads to 8: 435 us, 1 260 TFLOP/s; 2 048 behind 13 952: 360 us, 1 390 -, a unit's
+// What bounds it: where contexts are long, the tensor cores' waits for softmax and for units' ends (their pipe is busy 62 and 57 % of the cycles) - 2 048 behind 13 952, 32 heads to 8: 360 us, 1 390
+// TFLOP/s of 1 675 that a call alone with cold caches may have, and 1 140 to 1 160 of the 1 410 that the power cap leaves calls behind one another; a prompt of 8 191: 435 us, 1 260 of 1 675 -, a unit's
 // queries and result where they are short (16 prompts of 1 024: 233 us, 590 TFLOP/s).
 //
 // Work is cut as in the kernel for few rows: the key tiles of all (sequence, 256 rows, key head) units in one list, an equal stretch for each CTA; units that lie in several CTAs are joined by
@@ -30,7 +32,8 @@ constexpr int kOffQ = 0, kOffK = 2 * kTileBytes, kOffV = kOffK + 2 * kTileBytes,
 constexpr int kOffBar = kOffPark + 8 * 96 + 16;
 constexpr int kNumBars = 18;
 constexpr int kSmemBytes = kOffBar + kNumBars * 8 + 16 + 1024;          // and room to begin at a multiple of 1024
-constexpr int kUnitCost = 5;                               // a unit's queries and result, in tiles (a prompt of 8 191 in us: 4 470, 5 438, 6 439, 9 451)
+constexpr int kUnitCost = 5;                               // a unit's queries and result, in tiles (a prompt of 8 191 in us: 4 470, 5 438, 6 439, 9 451; 3 / 5 / 8 for 16 of 1 024 253 / 241 / 251, 64 x 128 behind 400
+// 84 / 78 / 83, 8 x 300 behind 1 000 to 8 000 338 / 321 / 324, 2 048 behind 13 952 364 / 362 / 367)
 // Where the tables have room for no more, and all units run at once, each has a CTA (in us, stretches and joining / a CTA for each, caches cold, 16 heads to 8: 1 x 100 tokens 22.4 / 12.2, 333 24.6 / 16.3,
 // 1 024 30.7 / 25.0, 64 behind 1 000 27.1 / 24.9, behind 2 000 28.9 / 38.9; 32 to 2, 64 behind 1 000 25.9 / 26.6)
 constexpr int kAloneTiles = 9;
