@@ -14,7 +14,7 @@
 // block of 16 dims is remembered: a row that sees it has NaN there.
 //
 // What bounds it: where contexts are long, the tensor cores' waits for softmax and for units' ends (their pipe is busy 62 and 57 % of the cycles) - 2 048 behind 13 952, 32 heads to 8: 360 us, 1 390
-// TFLOP/s of 1 675 that a call alone with cold caches may have, and 1 140 to 1 160 of the 1 410 that the power cap leaves calls behind one another; a prompt of 8 191: 435 us, 1 260 of 1 675 -, a unit's
+// TFLOP/s of 1 675 that a call alone with cold caches may have, and 1 130 to 1 160 of the 1 410 that the power cap leaves calls behind one another; a prompt of 8 191: 435 us, 1 260 of 1 675 -, a unit's
 // queries and result where they are short (16 prompts of 1 024: 233 us, 590 TFLOP/s).
 //
 // Work is cut as in the kernel for few rows: the key tiles of all (sequence, 256 rows, key head) units in one list, an equal stretch for each CTA; units that lie in several CTAs are joined by
